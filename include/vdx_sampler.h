@@ -66,6 +66,8 @@ typedef struct vdxs_config {
 /* Logits element types. bf16 is widened exactly to fp32, then fp32 semantics apply. */
 #define VDXS_DTYPE_F32   0
 #define VDXS_DTYPE_BF16  1
+/* fp16: hidden states and norm weights of vdxs_rms_norm_i8 and its callers only. */
+#define VDXS_DTYPE_F16   2
 
 /* Tie modes.
  * FAITHFUL (default): the token equals what TVdxSampler.Process returns. Rows whose
@@ -389,6 +391,170 @@ VDXS_API int32_t vdxs_sample_unembed_q4_0(vdxs_context* ctx, const vdxs_config* 
                                           int64_t history_stride, const int32_t* d_history_count,
                                           const float* d_uniform, int32_t* d_out_tokens,
                                           void* stream);
+
+/* ----------------------------------------------------------------------------
+ * Unembedding in 8-bit integers, for every batch size: the final norm with an 8-bit
+ * output, the product on the integer tensor cores, and the sampler behind them.
+ * Replaces the same TVdxModel.UnembedToLogits (src/VindexLLM.Model.pas:1258-1271: norm,
+ * then the tied-embedding product) where the reference's order of sums is not wanted;
+ * the reference has no 8-bit activations, so logits differ from the Q4_0 path's by the
+ * quantisation of both operands.
+ * ---------------------------------------------------------------------------- */
+/* Widest row of vdxs_rms_norm_i8 and vdxs_i8_prepare. */
+#define VDXS_I8_MAX_DIM 32768
+
+/* Residual's addition, root-mean-square norm and 8-bit output of `rows` rows:
+ *   h = x + residual, rounded to `dtype`   (h = x where d_residual is NULL)
+ *   y = h * weight / sqrt(mean(h^2) + eps)
+ *   scale[row] = max|y| / 127 (fp32),  q = y / (max|y| / 127) rounded to nearest even
+ * Sums and the values next to a rounding border are taken in 64 bits, so q is the exact
+ * rounding of the row's values. A row of zeros has scale 0 and q 0; a row that holds a
+ * NaN or an infinity (in x, the residual or the weights) has scale NaN and q 0, so the
+ * logits made from it are NaN.
+ *   d_x           [rows, x_stride] dtype F32, BF16 or F16 (first `dim` used)
+ *   d_residual    [rows, residual_stride] of the same type, or NULL
+ *   d_weight      [dim], weight_dtype F32, BF16 or F16
+ *   d_out_hidden  [rows, hidden_stride] receives h, or NULL; it may be d_x or d_residual
+ *                 itself with the same stride (in place), otherwise it overlaps neither
+ *   d_q           [rows, q_stride] int8; what lies between dim and q_stride is not written
+ *   d_scale       [rows] fp32
+ * Pointers are aligned to their element size. 1 <= dim <= VDXS_I8_MAX_DIM. */
+VDXS_API int32_t vdxs_rms_norm_i8(vdxs_context* ctx, const void* d_x, int64_t x_stride,
+                                  const void* d_residual, int64_t residual_stride, int32_t dtype,
+                                  const void* d_weight, int32_t weight_dtype, int32_t rows,
+                                  int32_t dim, float eps, void* d_out_hidden,
+                                  int64_t hidden_stride, int8_t* d_q, int64_t q_stride,
+                                  float* d_scale, void* stream);
+
+/* Sources of vdxs_i8_prepare. */
+#define VDXS_WEIGHTS_F32   0  /* [out_dim, row_stride] fp32                            */
+#define VDXS_WEIGHTS_BF16  1
+#define VDXS_WEIGHTS_F16   2
+#define VDXS_WEIGHTS_I8    3  /* int8 with d_scales[out_dim]                           */
+#define VDXS_WEIGHTS_Q4_0  4  /* the reference's Q4_0 blocks (row_stride ignored)      */
+typedef struct vdxs_i8_weights vdxs_i8_weights;
+/* Makes the 8-bit weights of an unembedding once, on the context's device: copies int8
+ * rows with their scales, or quantises each row (vocabulary entry) of another type as
+ * vdxs_rms_norm_i8 quantises y. Synchronises `stream`; the source may be freed
+ * afterwards. 1 <= in_dim <= VDXS_I8_MAX_DIM (Q4_0: a multiple of 32). row_stride is in
+ * elements. d_scales is read for VDXS_WEIGHTS_I8 alone. */
+VDXS_API int32_t vdxs_i8_prepare(vdxs_context* ctx, const void* d_weights, int32_t format,
+                                 const float* d_scales, int64_t row_stride, int32_t in_dim,
+                                 int32_t out_dim, void* stream, vdxs_i8_weights** out);
+VDXS_API int32_t vdxs_i8_release(vdxs_i8_weights* w);
+
+/* logits[b][n] = (sum_k q[b][k] * weights[n][k]) * scale[b] * w_scale[n]: exact 32-bit
+ * integer sums, scaled in fp32 and rounded once to `dtype` (VDXS_DTYPE_F32 or _BF16).
+ *   d_q       [batch, q_stride] int8, 16-byte aligned, q_stride a multiple of 16
+ *   d_scale   [batch] fp32
+ *   d_logits  [batch, logits_stride] (logits_stride >= out_dim); what lies between
+ *             out_dim and logits_stride is not written
+ * Uses no workspace and allocates nothing. */
+VDXS_API int32_t vdxs_unembed_i8(vdxs_context* ctx, const vdxs_i8_weights* w, const int8_t* d_q,
+                                 int64_t q_stride, const float* d_scale, int32_t batch,
+                                 void* d_logits, int32_t dtype, int64_t logits_stride,
+                                 void* stream);
+
+/* vdxs_rms_norm_i8 of the last layer's output, vdxs_unembed_i8 into a context-owned fp32
+ * logits buffer, then vdxs_sample on it. d_out_hidden may be NULL. As vdxs_decode_step it
+ * can be captured in a CUDA graph after one warm-up call with the same shapes; the graph
+ * holds the context's buffers, so it must not be replayed after a call on the context that
+ * made them grow (more rows, a larger vocabulary). A call under capture whose own
+ * buffers would have to grow returns VDXS_E_UNSUPPORTED and launches nothing. */
+VDXS_API int32_t vdxs_sample_unembed_i8(vdxs_context* ctx, const vdxs_config* cfg,
+                                        const vdxs_i8_weights* w, const void* d_x, int64_t x_stride,
+                                        const void* d_residual, int64_t residual_stride,
+                                        int32_t dtype, const void* d_norm_weight,
+                                        int32_t weight_dtype, float eps, void* d_out_hidden,
+                                        int64_t hidden_stride, int32_t batch,
+                                        const int32_t* d_history, int64_t history_stride,
+                                        const int32_t* d_history_count, const float* d_uniform,
+                                        int32_t* d_out_tokens, void* stream);
+
+/* ----------------------------------------------------------------------------
+ * Beam search: the selection over beams and vocabulary that stands where the sampler's
+ * draw stands, and the reordering of the search's rows by it. The reference decodes one
+ * sequence and has no search; the repetition penalty and the history ring are those of
+ * TVdxSampler (src/VindexLLM.Sampler.pas:285-303, 530-539).
+ *
+ * Rows are [batch][beams]: prompt g's beam b is row g * beams + b. In one step
+ *   - a live beam (not finished, score > -infinity) offers the tokens of its `beams`
+ *     largest logits (equal logits: the lower token), each with
+ *       score + log softmax(logits)[token]   and   length + 1;
+ *     logits of -infinity are never offered (a mask), and a row that holds a NaN or
+ *     +infinity, or whose logits are all -infinity, offers nothing;
+ *   - a finished beam offers itself, with its score and length, and its logits are not read;
+ *   - the `beams` offers with the highest score / max(length, 1)^length_alpha stay, in that
+ *     order (equal ones: the lower beam, then the beam's own order).
+ * Log-probabilities and the order of the offers are taken in 64 bits; scores are stored in
+ * fp32. A slot that gets no offer has token pad_token, its own slot as the parent, score
+ * -infinity, finished 0, and the length that stood there; it offers nothing in later steps.
+ * ---------------------------------------------------------------------------- */
+#define VDXS_BEAM_MAX_BEAMS 64
+typedef struct vdxs_beam vdxs_beam;
+
+typedef struct vdxs_beam_config {  /* 24 bytes */
+    double  length_alpha;    /* 0 = order by score alone; any finite value             */
+    float   repeat_penalty;  /* 1 = off; as vdxs_config (needs the rings)              */
+    int32_t window;          /* ring length; 0 = no rings                              */
+    int32_t pad_token;       /* token of finished beams and of slots without an offer  */
+    int32_t reserved;        /* 0 */
+} vdxs_beam_config;
+
+/* Device state of the batch * beams rows. hist, hist_pos and hist_count are the rings of
+ * vdxs_device_history_push ([rows][window], [rows], [rows]); they may be NULL when
+ * window is 0. A new search starts with score 0 for beam 0 and -infinity for the others. */
+typedef struct vdxs_beam_rows {
+    float*   scores;
+    int32_t* lengths;
+    int32_t* finished;
+    int32_t* hist;
+    int32_t* hist_pos;
+    int32_t* hist_count;
+} vdxs_beam_rows;
+
+/* A state of the caller that follows its rows (a layer's key or value cache, token lists):
+ * `segments` pieces of segment_bytes in each row, segment_stride bytes apart, rows
+ * row_stride bytes apart. A cache [rows, heads, room, width] of which `used` positions are
+ * filled has heads segments of used * width elements. Row r of dst receives row parent(r)
+ * of src. dst may be src with the same strides (in place: rows that stay are not touched);
+ * otherwise the two do not overlap. Bytes outside the segments are left as they were. */
+typedef struct vdxs_beam_cache {
+    const void* src;
+    void*       dst;
+    int64_t     src_row_stride, src_segment_stride;
+    int64_t     dst_row_stride, dst_segment_stride;
+    int64_t     segment_bytes, segments;
+} vdxs_beam_cache;
+
+/* A search of `batch` prompts with `beams` beams each (1..VDXS_BEAM_MAX_BEAMS; batch *
+ * beams <= 65535) over `vocab` tokens. It owns a fixed workspace, so a step allocates nothing and
+ * may be captured at once; steps of one search that overlap on the GPU race, so give each
+ * stream or graph that runs beside another its own. Destroy it before its context. */
+VDXS_API int32_t vdxs_beam_create(vdxs_context* ctx, int32_t batch, int32_t beams, int32_t vocab,
+                                  vdxs_beam** out);
+VDXS_API int32_t vdxs_beam_destroy(vdxs_beam* beam);
+
+/* One step on `stream`: selects, writes the rows' new scores, lengths and finished flags, moves
+ * the rings and the caches by the parents, and pushes the new tokens of live beams into
+ * the rings (a finished beam's ring is moved as it is). A new token that is in d_stop_ids
+ * finishes its beam.
+ *   d_logits      [batch * beams, row_stride] VDXS_DTYPE_F32 or _BF16
+ *   in, out       the rows before and after; each array of `out` is that of `in` (in
+ *                 place) or overlaps none of them
+ *   d_out_tokens, d_out_parents  [batch * beams] int32; a parent is a beam 0..beams-1 of
+ *                 the same prompt
+ * caches may be NULL when n_caches is 0. */
+VDXS_API int32_t vdxs_beam_step(vdxs_beam* beam, const vdxs_beam_config* cfg, const void* d_logits,
+                                int32_t dtype, int64_t row_stride, const vdxs_beam_rows* in,
+                                const vdxs_beam_rows* out, const int32_t* d_stop_ids, int32_t n_stop,
+                                const vdxs_beam_cache* caches, int32_t n_caches,
+                                int32_t* d_out_tokens, int32_t* d_out_parents, void* stream);
+
+/* Moves more caches by the parents of a step (for a caller that moves a layer's cache just
+ * before it runs the layer). A parent outside 0..beams-1 leaves its row where it is. */
+VDXS_API int32_t vdxs_beam_reorder(vdxs_beam* beam, const int32_t* d_parents,
+                                   const vdxs_beam_cache* caches, int32_t n_caches, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,400 @@
+"""The beam step against a plain 64-bit restatement: the selection over beams and vocabulary,
+its state, the rings and the reordering of caches."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import i8_beam_ref as ref
+from vindexllm_b200 import abi
+
+pytestmark = pytest.mark.gpu
+
+# Scores: an fp32 store (2^-24 of the score) and the error of the log of the sum: the
+# exponentials are off by 2^-22 and 2^-24 for each unit of distance to the maximum (weighted
+# by themselves: below 1), a thread's fp32 sum of n terms by n 2^-24; n <= 64 here: 5e-6.
+ATOL, RTOL = 5e-6, 2.0 ** -23
+
+
+def _state(batch, beams, window, vocab, seed, fresh=False):
+    rng = np.random.default_rng(seed)
+    rows = batch * beams
+    s = dict(scores=(-20 + 3 * rng.standard_normal(rows)).astype(np.float32),
+             lengths=rng.integers(1, 30, rows).astype(np.int32),
+             finished=(rng.random(rows) < 0.2).astype(np.int32))
+    s["scores"][rng.random(rows) < 0.1] = -np.inf
+    if window:
+        s["hist"] = rng.integers(-2, vocab + 2, (rows, window)).astype(np.int32)
+        s["count"] = rng.integers(0, window + 1, rows).astype(np.int32)
+        s["pos"] = (s["count"] % window).astype(np.int32)
+    return s
+
+
+def _device(s, batch, beams, window):
+    import torch
+    from vindexllm_b200.sampler import BeamState
+    t = {k: torch.as_tensor(v.copy(), device="cuda") for k, v in s.items()}
+    return BeamState(batch, beams, window, **t)
+
+
+def _check(got, want, batch, beams, exact=True):
+    """got: (tokens, parents, BeamState); a pick may differ from the restatement's only where the
+    two offers' ranks are nearer than the tolerance."""
+    tokens, parents, state = got
+    wt, wp, ws, ranks, offers = want
+    t, p = tokens.cpu().numpy(), parents.cpu().numpy()
+    same = (t == wt) & (p == wp)
+    for g, k in zip(*np.nonzero(~same)):
+        rank = offers[g].get((p[g, k], t[g, k]))
+        assert rank is not None, f"prompt {g} slot {k}: ({p[g, k]}, {t[g, k]}) is no offer, want ({wp[g, k]}, {wt[g, k]})"
+        near = 2 * (ATOL + RTOL * abs(rank))
+        assert 0 < abs(rank - ranks[g, k]) <= near, f"prompt {g} slot {k}: rank {rank}, want {ranks[g, k]}"
+    ok = same.reshape(-1)
+    sc = state.scores.cpu().numpy()
+    fin = np.isfinite(ws["scores"]) & ok
+    assert np.array_equal(np.isfinite(sc), np.isfinite(ws["scores"]))
+    assert (np.abs(sc[fin] - ws["scores"][fin]) <= ATOL + RTOL * np.abs(ws["scores"][fin])).all()
+    names = {"lengths": state.lengths, "finished": state.finished}
+    if state.window:
+        names |= {"hist": state.hist, "pos": state.pos, "count": state.count}
+    for name, v in names.items():
+        assert np.array_equal(v.cpu().numpy()[ok], ws[name][ok]), name
+
+
+def _bits(x, dtype):
+    import torch
+    t = torch.as_tensor(x, device="cuda")
+    return t if dtype == "f32" else t.to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 33, 1000, 4096, 4097, 20011, 50257])
+@pytest.mark.parametrize("batch,beams", [(1, 1), (3, 4), (2, 5), (1, 16), (1, 33), (1, 64)])
+def test_step(gpu_ctx, dtype, vocab, batch, beams):
+    """Odd vocabularies (rows off the 16-byte boundary), fewer tokens than beams, ties (values
+    rounded to quarters), masks, finished and dead beams, all combinations of penalty and length."""
+    from vindexllm_b200.sampler import BeamSearch
+    rng = np.random.default_rng(vocab * 100 + beams)
+    rows = batch * beams
+    x = 3 * rng.standard_normal((rows, vocab)).astype(np.float32)
+    x[rng.random(x.shape) < 0.05] = -np.inf
+    x[::2] = np.round(x[::2] * 4) / 4
+    lg = _bits(x, dtype)
+    xf = lg.float().cpu().numpy()
+    search = BeamSearch(gpu_ctx, batch, beams, vocab)
+    for window, penalty, alpha in ((0, 1.0, 0.0), (20, 1.3, 0.6), (1, 0.8, 1.0)):
+        s = _state(batch, beams, window, vocab, vocab + window)
+        stop = np.unique(np.argmax(xf, 1))[:3].astype(np.int32)
+        want = ref.beam_step(xf, batch, beams, s, stop, 9, penalty, alpha)
+        state, out = _device(s, batch, beams, window), _device(s, batch, beams, window)
+        import torch
+        st = torch.as_tensor(stop, device="cuda")
+        kw = dict(stop_ids=st, pad_token=9, repeat_penalty=penalty, length_alpha=alpha)
+        got = search.step(state, lg, out=out, **kw)
+        _check((*got, out), want, batch, beams)
+        again = search.step(state, lg, **kw)  # in place: the same
+        assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
+        for name in ("scores", "lengths", "finished") + (("hist", "pos", "count") if window else ()):
+            assert torch.equal(getattr(state, name), getattr(out, name)), name
+    search.close()
+
+
+@pytest.mark.parametrize("kind", ["rising", "falling", "constant", "two values", "one finite", "all masked", "lowest",
+                                  "nan", "inf", "huge"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_that_go_wrong(gpu_ctx, kind, dtype):
+    """Orders in which every element enters the list, ties everywhere, masks that leave a row one
+    token or none, the type's lowest value as a mask, NaN and infinities."""
+    from vindexllm_b200.sampler import BeamSearch
+    vocab = 30011
+    ramp = np.arange(vocab, dtype=np.float32) * 1e-3
+    for beams in (1, 4, 64):
+        x = np.random.default_rng(beams).standard_normal((2 * beams, vocab)).astype(np.float32)
+        row = {"rising": ramp, "falling": -ramp, "constant": np.full(vocab, 2.5, np.float32),
+               "two values": (np.arange(vocab) % 2).astype(np.float32)}.get(kind, x[0].copy())
+        if kind == "one finite":
+            row[:] = -np.inf
+            row[vocab - 2] = -700.0
+        elif kind == "all masked":
+            row[:] = -np.inf
+        elif kind == "lowest":
+            row[3:] = np.finfo(np.float32).min
+        elif kind == "nan":
+            row[vocab // 2] = np.nan
+        elif kind == "inf":
+            row[vocab - 1] = np.inf
+        elif kind == "huge":
+            row *= 1e30
+        x[0] = row
+        if beams > 1:
+            x[beams] = row
+        lg = _bits(x, dtype)
+        xf = lg.float().cpu().numpy()
+        s = _state(2, beams, 0, vocab, 5)
+        s["scores"][:] = np.linspace(-1, -2, 2 * beams)
+        s["finished"][:] = 0
+        want = ref.beam_step(xf, 2, beams, s)
+        search, out = BeamSearch(gpu_ctx, 2, beams, vocab), _device(s, 2, beams, 0)
+        got = search.step(_device(s, 2, beams, 0), lg, out=out)
+        _check((*got, out), want, 2, beams)
+        search.close()
+
+
+def test_strides_and_offsets(gpu_ctx):
+    """A row stride beyond the vocabulary with NaN between the rows, a base at every element offset."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    batch, beams, vocab = 2, 3, 5000
+    for dtype in (torch.float32, torch.bfloat16):
+        wide = torch.full((batch * beams, vocab + 21), float("nan"), device="cuda", dtype=dtype)
+        for off in range(9):
+            wide.fill_(float("nan"))
+            view = wide[:, off:off + vocab]
+            view.copy_(torch.randn(view.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(off)))
+            s = _state(batch, beams, 0, vocab, off)
+            want = ref.beam_step(view.float().cpu().numpy(), batch, beams, s)
+            search, out = BeamSearch(gpu_ctx, batch, beams, vocab), _device(s, batch, beams, 0)
+            got = search.step(_device(s, batch, beams, 0), view, out=out)
+            _check((*got, out), want, batch, beams)
+            search.close()
+
+
+def test_finished_rows_are_not_read(gpu_ctx):
+    """Logits of finished and dead beams may hold anything."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    s = _state(1, 4, 0, 1000, 1)
+    s["scores"][:] = [-3.0, -np.inf, -1.0, np.nan]
+    s["finished"][:] = [0, 0, 1, 0]
+    x = np.random.default_rng(0).standard_normal((4, 1000)).astype(np.float32)
+    want = ref.beam_step(x, 1, 4, s)
+    x[1:] = np.nan
+    search, out = BeamSearch(gpu_ctx, 1, 4, 1000), _device(s, 1, 4, 0)
+    got = search.step(_device(s, 1, 4, 0), torch.as_tensor(x, device="cuda"), out=out)
+    _check((*got, out), want, 1, 4)
+
+
+def test_full_vocabulary(gpu_ctx):
+    """262144 tokens: many rows with long chunks, few rows with short ones. A thread sums up to
+    1024 terms here: its fp32 sum is off by at most 1024 * 2^-24 = 6e-5 of the sum."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    vocab = 262144
+    for batch, beams, dtype in ((1, 4, torch.bfloat16), (40, 8, torch.float32)):
+        rows = batch * beams
+        x = torch.randn(rows, vocab, device="cuda", generator=torch.Generator("cuda").manual_seed(3)).mul_(3.0).to(dtype)
+        s = _state(batch, beams, 0, vocab, 7)
+        search, out = BeamSearch(gpu_ctx, batch, beams, vocab), _device(s, batch, beams, 0)
+        tokens, parents = search.step(_device(s, batch, beams, 0), x, out=out, length_alpha=0.7)
+        logp = torch.log_softmax(x.double(), 1)
+        top = logp.topk(beams, 1).values.cpu().numpy()
+        t, p, sc = tokens.cpu().numpy(), parents.cpu().numpy(), out.scores.cpu().numpy().reshape(batch, beams)
+        for g in range(batch):
+            r = slice(g * beams, (g + 1) * beams)
+            done, score, length = s["finished"][r], s["scores"][r].astype(np.float64), s["lengths"][r]
+            ranks = np.concatenate([[score[b] / length[b] ** 0.7] if done[b] else
+                                    (score[b] + top[g * beams + b]) / (length[b] + 1) ** 0.7 for b in range(beams)])
+            want = np.sort(ranks[ranks > -np.inf])[::-1][:beams]
+            for k in range(len(want)):
+                b = p[g, k]
+                mine = score[b] if done[b] else score[b] + logp[g * beams + b, t[g, k]].item()
+                assert abs(mine / (length[b] + (not done[b])) ** 0.7 - want[k]) <= 6e-5
+                assert abs(sc[g, k] - mine) <= 6e-5 + RTOL * abs(mine)
+        search.close()
+        del logp
+
+
+def test_search_of_many_steps(gpu_ctx):
+    """A whole search from its start (beam 0 alone is alive), in place, with rings, a token list as
+    a cache, and a stop token: the tokens follow the parents, step by step."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch, BeamState
+    batch, beams, vocab, window, steps = 3, 4, 501, 6, 12
+    rng = np.random.default_rng(11)
+    search = BeamSearch(gpu_ctx, batch, beams, vocab)
+    state = BeamState(batch, beams, window)
+    lists = torch.zeros(batch * beams, steps, dtype=torch.int32, device="cuda")
+    host = dict(scores=state.scores.cpu().numpy(), lengths=np.zeros(batch * beams, np.int32),
+                finished=np.zeros(batch * beams, np.int32), hist=np.zeros((batch * beams, window), np.int32),
+                pos=np.zeros(batch * beams, np.int32), count=np.zeros(batch * beams, np.int32))
+    hl = np.zeros((batch * beams, steps), np.int32)
+    stop = torch.tensor([3, 77], dtype=torch.int32, device="cuda")
+    for i in range(steps):
+        x = 2 * rng.standard_normal((batch * beams, vocab)).astype(np.float32)
+        x[:, 77] += 6
+        want = ref.beam_step(x, batch, beams, host, (3, 77), 0, 1.4, 0.8)
+        tokens, parents = search.step(state, torch.as_tensor(x, device="cuda"), stop_ids=stop, repeat_penalty=1.4,
+                                      length_alpha=0.8, caches=[lists[:, :i]] if i else [])
+        lists[:, i] = tokens.view(-1)
+        _check((tokens, parents, state), want, batch, beams)
+        assert np.array_equal(tokens.cpu().numpy(), want[0]) and np.array_equal(parents.cpu().numpy(), want[1])
+        src = (want[1] + beams * np.arange(batch)[:, None]).reshape(-1)
+        hl[:, :i] = hl[src, :i]
+        hl[:, i] = want[0].reshape(-1)
+        host = want[2]
+        host["scores"] = state.scores.cpu().numpy()  # one step's rounding at a time
+    assert np.array_equal(lists.cpu().numpy(), hl)
+    assert state.finished.any()
+
+
+PARENTS = [[0, 1, 2, 3], [3, 2, 1, 0], [0, 0, 0, 0], [1, 2, 3, 3], [-1, 4, 2, 1 << 30]]
+
+
+@pytest.mark.parametrize("dtype,width", [("uint8", 1), ("uint8", 7), ("int16", 9), ("int32", 5), ("int64", 3),
+                                         ("float16", 8), ("float32", 64), ("float32", 1000)])
+def test_reorder(gpu_ctx, dtype, width):
+    """Words of every size, in place and to another buffer, the filled part of a cache, more
+    caches than one launch takes, parents out of range (their rows stay)."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    batch, beams = len(PARENTS), 4
+    parents = torch.tensor(PARENTS, dtype=torch.int32, device="cuda")
+    src = np.array([[b if 0 <= b < beams else k for k, b in enumerate(p)] for p in PARENTS])
+    rows = torch.as_tensor((src + beams * np.arange(batch)[:, None]).reshape(-1), device="cuda")
+    search = BeamSearch(gpu_ctx, batch, beams, 10)
+    dt = getattr(torch, dtype)
+    make = lambda i: torch.randint(0, 100, (batch * beams, 3, 11, width), device="cuda",  # noqa: E731
+                                   generator=torch.Generator("cuda").manual_seed(i)).to(dt)
+    a = [make(i) for i in range(40)]
+    want, b = [t.clone() for t in a], [make(100 + i) for i in range(40)]
+    left = [t.clone() for t in b]
+    used = [(i % 11) + 1 for i in range(40)]
+    search.reorder(parents, [(x[:, :, :u], y[:, :, :u]) for x, y, u in zip(a, b, used)])
+    for x, y, l, w, u in zip(a, b, left, want, used):
+        assert torch.equal(x, w)
+        assert torch.equal(y[:, :, :u], w[rows, :, :u]) and torch.equal(y[:, :, u:], l[:, :, u:])
+    search.reorder(parents, [x[:, 1:, u - 1:u] for x, u in zip(a, used)])
+    for x, w, u in zip(a, want, used):
+        w2 = w.clone()
+        w2[:, 1:, u - 1:u] = w[rows, 1:, u - 1:u]
+        assert torch.equal(x, w2)
+    # Pieces of different shapes, rows inside the segments' gaps, empty views.
+    e, f = make(7), torch.zeros(3, batch * beams, 11, width, dtype=dt, device="cuda").transpose(0, 1)
+    search.reorder(parents, [(e, f), e[:, :0]])
+    assert torch.equal(f, e[rows])
+    search.reorder(parents, [f])
+    assert torch.equal(f, e[rows][rows])
+    search.close()
+
+
+@pytest.mark.parametrize("beams", [1, 2, 9, 17, 64])
+def test_reorder_other_beam_counts(gpu_ctx, beams):
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    batch = 3
+    g = torch.Generator("cuda").manual_seed(beams)
+    parents = torch.randint(0, beams, (batch, beams), device="cuda", generator=g).int()
+    rows = (parents + beams * torch.arange(batch, device="cuda")[:, None]).view(-1).long()
+    x = torch.randn(batch * beams, 2, 300, 8, device="cuda", generator=g)
+    want = x[rows]
+    search = BeamSearch(gpu_ctx, batch, beams, 10)
+    search.reorder(parents, [x])
+    assert torch.equal(x, want)
+    search.close()
+
+
+def test_graph_and_side_stream(gpu_ctx):
+    """Captured without a warm-up call and replayed: each replay advances the state as an eager step
+    of another search does."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch, BeamState
+    batch, beams, vocab = 2, 4, 3000
+    one, two = BeamSearch(gpu_ctx, batch, beams, vocab), BeamSearch(gpu_ctx, batch, beams, vocab)
+    x = torch.randn(batch * beams, vocab, device="cuda")
+    s1, s2 = BeamState(batch, beams, 4), BeamState(batch, beams, 4)
+    c1 = torch.arange(batch * beams * 20, device="cuda").view(batch * beams, 20)
+    c2 = c1.clone()
+    t1 = torch.empty(batch, beams, dtype=torch.int32, device="cuda")
+    p1 = torch.empty_like(t1)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        one.step(s1, x, repeat_penalty=1.2, caches=[c1], tokens=t1, parents=p1)
+    side = torch.cuda.Stream()
+    for i in range(4):
+        x.normal_()
+        side.wait_stream(torch.cuda.current_stream())
+        t2, p2 = two.step(s2, x, repeat_penalty=1.2, caches=[c2], stream=side)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(t1, t2) and torch.equal(p1, p2) and torch.equal(c1, c2)
+        assert torch.equal(s1.scores, s2.scores) and torch.equal(s1.hist, s2.hist) and torch.equal(s1.count, s2.count)
+
+
+def test_norm_product_beam_run(gpu_ctx):
+    """The tail of a decode step as a search runs it: norm, product and beam step, the step held to the
+    restatement on the logits that the product gave."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch, BeamState, I8Weights
+    batch, beams, vocab, k = 2, 5, 4099, 320
+    gen = torch.Generator("cuda").manual_seed(4)
+    w = I8Weights(gpu_ctx, 0.1 * torch.randn(vocab, k, device="cuda", generator=gen))
+    nw = torch.ones(k, device="cuda")
+    search, state = BeamSearch(gpu_ctx, batch, beams, vocab), BeamState(batch, beams, 8)
+    hidden = torch.randn(batch * beams, k, device="cuda", generator=gen).bfloat16()
+    for i in range(4):
+        x = torch.randn(batch * beams, k, device="cuda", generator=gen).bfloat16()
+        host = {n: getattr(state, n).cpu().numpy().copy() for n in ("scores", "lengths", "finished", "hist", "pos", "count")}
+        q, scale, _ = gpu_ctx.rms_norm_i8(x, nw, residual=hidden, out_hidden=hidden)
+        logits = w.unembed(q, scale, dtype=torch.bfloat16 if i % 2 else torch.float32)
+        before = hidden.clone()
+        tokens, parents = search.step(state, logits, repeat_penalty=1.1, caches=[hidden])
+        want = ref.beam_step(logits.float().cpu().numpy(), batch, beams, host, (), 0, 1.1, 0.0)
+        _check((tokens, parents, state), want, batch, beams)
+        src = (parents + beams * torch.arange(batch, device="cuda")[:, None]).view(-1).long()
+        assert torch.equal(hidden, before[src])
+    w.close()
+    search.close()
+
+
+def test_refusals(gpu_ctx):
+    import torch
+    from vindexllm_b200.sampler import BeamSearch, BeamState
+    lib = gpu_ctx.lib
+    out = C.c_void_p()
+    for b, k, v, code in ((0, 4, 10, abi.E_INVALID_ARG), (1, 0, 10, abi.E_INVALID_ARG), (1, 4, 0, abi.E_INVALID_ARG),
+                          (1, 65, 10, abi.E_UNSUPPORTED), (2000, 64, 10, abi.E_UNSUPPORTED),
+                          (1, 4, 1 << 25, abi.E_UNSUPPORTED)):
+        assert lib.vdxs_beam_create(gpu_ctx.handle, b, k, v, C.byref(out)) == code and not out.value
+    search, state = BeamSearch(gpu_ctx, 2, 3, 100), BeamState(2, 3, 4)
+    x = torch.zeros(6, 100, device="cuda")
+    tok = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+
+    def step(cfg=(0.0, 1.0, 4, 0, 0), xp=p(x), dt=0, stride=100, drop=None, stop=None, n_stop=0, cache=None, n=0,
+             tp=p(tok), rows=state):
+        a = rows.rows()
+        if drop:
+            setattr(a, drop, None)
+        c = abi.VdxsBeamConfig(*cfg)
+        return lib.vdxs_beam_step(search._h, C.byref(c), xp, dt, stride, C.byref(a), C.byref(a), stop, n_stop, cache, n,
+                                  tp, p(tok), None)
+
+    assert step() == abi.OK
+    nan = float("nan")
+    for bad in (dict(xp=None), dict(dt=2), dict(stride=99), dict(tp=None), dict(drop="scores"), dict(drop="finished"),
+                dict(drop="hist"), dict(drop="hist_count"), dict(n_stop=1), dict(n_stop=-1), dict(n=1), dict(n=-1),
+                dict(cfg=(nan, 1.0, 4, 0, 0)), dict(cfg=(0.0, 0.0, 4, 0, 0)), dict(cfg=(0.0, nan, 4, 0, 0)),
+                dict(cfg=(0.0, 1.0, -1, 0, 0)), dict(cfg=(0.0, 1.0, 9000, 0, 0)), dict(cfg=(0.0, 1.0, 4, 0, 1)),
+                dict(xp=C.c_void_p(x.data_ptr() + 2))):
+        assert step(**bad) == abi.E_INVALID_ARG, bad
+    buf = torch.zeros(6, 64, dtype=torch.uint8, device="cuda")
+    at = buf.data_ptr()
+    for c in ((at, at, 64, 0, 32, 0, 16, 1),      # in place with other strides
+              (at, at + 8, 64, 0, 64, 0, 16, 1),  # overlap
+              (at, at, 8, 0, 8, 0, 16, 1),        # rows overlap
+              (at, at, 64, 8, 64, 8, 16, 2),      # segments overlap
+              (at, at, -64, 0, -64, 0, 16, 1), (0, at, 64, 0, 64, 0, 16, 1), (at, at, 64, 0, 64, 0, -1, 1)):
+        one = (abi.VdxsBeamCache * 1)(abi.VdxsBeamCache(*c))
+        assert step(cache=one, n=1) == abi.E_INVALID_ARG, c
+        assert lib.vdxs_beam_reorder(search._h, p(tok), one, 1, None) == abi.E_INVALID_ARG, c
+    with pytest.raises(ValueError):
+        search.step(state, x[:5])
+    with pytest.raises(ValueError):
+        search.step(BeamState(2, 4, 4), x)
+    with pytest.raises(ValueError):
+        search.step(state, x, out=BeamState(2, 3, 5))
+    with pytest.raises(ValueError):
+        search.reorder(tok, [torch.zeros(5, 3, device="cuda")])
+    with pytest.raises(TypeError):
+        search.step(state, x.half())
+    search.close()

@@ -5,7 +5,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 
-from .abi import VdxsConfig
+from .abi import VdxsBeamCache, VdxsBeamConfig, VdxsBeamRows, VdxsConfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libvdxsampler.so")
@@ -64,6 +64,17 @@ SIGNATURES = {
     "vdxs_q4_0_release": (i32, [vp]),
     "vdxs_unembed_q4_0": (i32, [vp, vp, vp, i32, vp, vp]),
     "vdxs_sample_unembed_q4_0": (i32, [vp, P(VdxsConfig), vp, vp, i32, vp, i64, vp, vp, vp, vp]),
+    "vdxs_rms_norm_i8": (i32, [vp, vp, i64, vp, i64, i32, vp, i32, i32, i32, C.c_float, vp, i64, vp, i64, vp, vp]),
+    "vdxs_i8_prepare": (i32, [vp, vp, i32, vp, i64, i32, i32, vp, P(vp)]),
+    "vdxs_i8_release": (i32, [vp]),
+    "vdxs_unembed_i8": (i32, [vp, vp, vp, i64, vp, i32, vp, i32, i64, vp]),
+    "vdxs_sample_unembed_i8": (i32, [vp, P(VdxsConfig), vp, vp, i64, vp, i64, i32, vp, i32, C.c_float, vp, i64, i32,
+                                     vp, i64, vp, vp, vp, vp]),
+    "vdxs_beam_create": (i32, [vp, i32, i32, i32, P(vp)]),
+    "vdxs_beam_destroy": (i32, [vp]),
+    "vdxs_beam_step": (i32, [vp, P(VdxsBeamConfig), vp, i32, i64, P(VdxsBeamRows), P(VdxsBeamRows), vp, i32,
+                             P(VdxsBeamCache), i32, vp, vp, vp]),
+    "vdxs_beam_reorder": (i32, [vp, vp, P(VdxsBeamCache), i32, vp]),
 }
 
 

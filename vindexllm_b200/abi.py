@@ -20,6 +20,16 @@ E_DEVICE_STATE = -7
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_F16 = 2
+
+WEIGHTS_F32 = 0
+WEIGHTS_BF16 = 1
+WEIGHTS_F16 = 2
+WEIGHTS_I8 = 3
+WEIGHTS_Q4_0 = 4
+
+I8_MAX_DIM = 32768
+BEAM_MAX_BEAMS = 64
 
 TIES_FAITHFUL = 0
 TIES_CANONICAL = 1
@@ -78,3 +88,33 @@ def default_config(**overrides) -> VdxsConfig:
              repeat_window=64, seed=0)
     d.update(overrides)
     return VdxsConfig.from_dict(d)
+
+
+class VdxsBeamConfig(C.Structure):
+    _fields_ = [
+        ("length_alpha", C.c_double),
+        ("repeat_penalty", C.c_float),
+        ("window", C.c_int32),
+        ("pad_token", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class VdxsBeamRows(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("scores", "lengths", "finished", "hist", "hist_pos", "hist_count")]
+
+
+class VdxsBeamCache(C.Structure):
+    _fields_ = [
+        ("src", C.c_void_p),
+        ("dst", C.c_void_p),
+        ("src_row_stride", C.c_int64),
+        ("src_segment_stride", C.c_int64),
+        ("dst_row_stride", C.c_int64),
+        ("dst_segment_stride", C.c_int64),
+        ("segment_bytes", C.c_int64),
+        ("segments", C.c_int64),
+    ]
+
+
+assert C.sizeof(VdxsBeamConfig) == 24 and C.sizeof(VdxsBeamRows) == 48 and C.sizeof(VdxsBeamCache) == 64

@@ -17,6 +17,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -1271,6 +1272,475 @@ VDXS_API int32_t vdxs_sample_unembed_q4_0(vdxs_context* ctx, const vdxs_config* 
     return vdxs_sample_ex(ctx, cfg, ctx->ws.unembed_logits, VDXS_DTYPE_F32, batch, w->out_dim, w->out_dim, d_history,
                           history_stride, d_history_count, d_uniform, d_out_tokens, nullptr, nullptr, nullptr, 0,
                           stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------
+// Unembedding in 8-bit integers: norm with an 8-bit output, product, sampler.
+// ---------------------------------------------------------------------------------
+struct vdxs_i8_weights {
+    int device = 0;
+    I8Matrix m;
+};
+
+namespace {
+
+int hidden_size(int32_t dtype) { return dtype == VDXS_DTYPE_F32 ? 4 : 2; }
+bool hidden_dtype(int32_t dtype) {
+    return dtype == VDXS_DTYPE_F32 || dtype == VDXS_DTYPE_BF16 || dtype == VDXS_DTYPE_F16;
+}
+bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// Everything of vdxs_rms_norm_i8 but its 8-bit outputs.
+int32_t check_norm(vdxs_context* ctx, const NormI8Args& a) {
+    if (!a.x || !a.weight) return fail(ctx, VDXS_E_INVALID_ARG, "x or weight pointer is NULL");
+    if (!hidden_dtype(a.dtype)) return fail(ctx, VDXS_E_INVALID_ARG, "dtype %d is not F32, BF16 or F16", a.dtype);
+    if (!hidden_dtype(a.weight_dtype))
+        return fail(ctx, VDXS_E_INVALID_ARG, "weight dtype %d is not F32, BF16 or F16", a.weight_dtype);
+    if (a.rows < 1) return fail(ctx, VDXS_E_INVALID_ARG, "rows must be >= 1 (got %d)", a.rows);
+    if (a.dim < 1) return fail(ctx, VDXS_E_INVALID_ARG, "dim must be >= 1 (got %d)", a.dim);
+    if (a.dim > VDXS_I8_MAX_DIM)
+        return fail(ctx, VDXS_E_UNSUPPORTED, "dim %d exceeds %d", a.dim, VDXS_I8_MAX_DIM);
+    if (!(a.eps >= 0.0f) || a.eps > 3.4e38f)
+        return fail(ctx, VDXS_E_INVALID_ARG, "eps must be finite and not negative");
+    if (a.x_stride < a.dim || (a.residual && a.residual_stride < a.dim) || (a.hidden && a.hidden_stride < a.dim))
+        return fail(ctx, VDXS_E_INVALID_ARG, "a row stride is smaller than dim %d", a.dim);
+    const size_t es = (size_t)hidden_size(a.dtype);
+    if (!aligned(a.x, es) || !aligned(a.residual, es) || !aligned(a.hidden, es) ||
+        !aligned(a.weight, (size_t)hidden_size(a.weight_dtype)))
+        return fail(ctx, VDXS_E_INVALID_ARG, "a pointer is not aligned to its element size");
+    if ((a.hidden == a.x && a.hidden_stride != a.x_stride) ||
+        (a.hidden && a.hidden == a.residual && a.hidden_stride != a.residual_stride))
+        return fail(ctx, VDXS_E_INVALID_ARG, "an output in place needs the input's row stride");
+    return VDXS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+VDXS_API int32_t vdxs_rms_norm_i8(vdxs_context* ctx, const void* d_x, int64_t x_stride, const void* d_residual,
+                                  int64_t residual_stride, int32_t dtype, const void* d_weight, int32_t weight_dtype,
+                                  int32_t rows, int32_t dim, float eps, void* d_out_hidden, int64_t hidden_stride,
+                                  int8_t* d_q, int64_t q_stride, float* d_scale, void* stream) {
+    if (!ctx) return fail(nullptr, VDXS_E_INVALID_ARG, "context is NULL");
+    NormI8Args a;
+    a.x = d_x;
+    a.x_stride = x_stride;
+    a.residual = d_residual;
+    a.residual_stride = residual_stride;
+    a.dtype = dtype;
+    a.weight = d_weight;
+    a.weight_dtype = weight_dtype;
+    a.rows = rows;
+    a.dim = dim;
+    a.eps = eps;
+    a.hidden = d_out_hidden;
+    a.hidden_stride = hidden_stride;
+    a.q = d_q;
+    a.q_stride = q_stride;
+    a.scale = d_scale;
+    const int32_t rc = check_norm(ctx, a);
+    if (rc != VDXS_OK) return rc;
+    if (!d_q || !d_scale) return fail(ctx, VDXS_E_INVALID_ARG, "q or scale pointer is NULL");
+    if (q_stride < dim) return fail(ctx, VDXS_E_INVALID_ARG, "q_stride is smaller than dim %d", dim);
+    if (!aligned(d_scale, 4)) return fail(ctx, VDXS_E_INVALID_ARG, "the scale pointer is not aligned to 4 bytes");
+    DeviceGuard g(ctx->device);
+    const cudaError_t e = rms_norm_i8(a, (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "norm launch");
+    ctx->launches += 1;
+    ok(ctx);
+    return VDXS_OK;
+}
+
+VDXS_API int32_t vdxs_i8_prepare(vdxs_context* ctx, const void* d_weights, int32_t format, const float* d_scales,
+                                 int64_t row_stride, int32_t in_dim, int32_t out_dim, void* stream,
+                                 vdxs_i8_weights** out) {
+    if (!ctx) return fail(nullptr, VDXS_E_INVALID_ARG, "context is NULL");
+    if (!out) return fail(ctx, VDXS_E_INVALID_ARG, "output pointer is NULL");
+    *out = nullptr;
+    if (!d_weights) return fail(ctx, VDXS_E_INVALID_ARG, "weights pointer is NULL");
+    if (format < VDXS_WEIGHTS_F32 || format > VDXS_WEIGHTS_Q4_0)
+        return fail(ctx, VDXS_E_INVALID_ARG, "unknown weight format %d", format);
+    if (format == VDXS_WEIGHTS_I8 && !d_scales)
+        return fail(ctx, VDXS_E_INVALID_ARG, "int8 weights need their scales");
+    if (in_dim < 1 || out_dim < 1)
+        return fail(ctx, VDXS_E_INVALID_ARG, "in_dim and out_dim must be >= 1 (got %d, %d)", in_dim, out_dim);
+    if (in_dim > VDXS_I8_MAX_DIM)
+        return fail(ctx, VDXS_E_UNSUPPORTED, "in_dim %d exceeds %d", in_dim, VDXS_I8_MAX_DIM);
+    if (format == VDXS_WEIGHTS_Q4_0 && in_dim % 32 != 0)
+        return fail(ctx, VDXS_E_INVALID_ARG, "in_dim %d is not a multiple of 32 (Q4_0 blocks)", in_dim);
+    if (format != VDXS_WEIGHTS_Q4_0 && row_stride < in_dim)
+        return fail(ctx, VDXS_E_INVALID_ARG, "row_stride %lld is smaller than in_dim %d", (long long)row_stride, in_dim);
+    const size_t es = format == VDXS_WEIGHTS_F32 ? 4 : format == VDXS_WEIGHTS_BF16 || format == VDXS_WEIGHTS_F16 ? 2 : 1;
+    if (!aligned(d_weights, es) || !aligned(d_scales, 4))
+        return fail(ctx, VDXS_E_INVALID_ARG, "a pointer is not aligned to its element size");
+    DeviceGuard g(ctx->device);
+    const cudaStream_t st = (cudaStream_t)stream;
+    auto* w = new (std::nothrow) vdxs_i8_weights();
+    if (!w) return fail(ctx, VDXS_E_NO_MEMORY, "out of host memory");
+    w->device = ctx->device;
+    I8Matrix& m = w->m;
+    m.in_dim = in_dim;
+    m.out_dim = out_dim;
+    m.pitch = ((int64_t)in_dim + 15) / 16 * 16;
+    cudaError_t e = cudaMalloc((void**)&m.q, (size_t)out_dim * (size_t)m.pitch);
+    if (e == cudaSuccess) e = cudaMalloc((void**)&m.scale, (size_t)out_dim * sizeof(float));
+    if (e == cudaSuccess) {
+        if (format == VDXS_WEIGHTS_I8) {
+            e = cudaMemcpy2DAsync(m.q, (size_t)m.pitch, d_weights, (size_t)row_stride, (size_t)in_dim, (size_t)out_dim,
+                                  cudaMemcpyDeviceToDevice, st);
+            if (e == cudaSuccess)
+                e = cudaMemcpyAsync(m.scale, d_scales, (size_t)out_dim * sizeof(float), cudaMemcpyDeviceToDevice, st);
+        } else {
+            e = quantise_rows_i8(d_weights, format, row_stride, m, st);
+            if (e == cudaSuccess) ctx->launches += 1;
+        }
+    }
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess) {
+        cudaFree(m.q);
+        cudaFree(m.scale);
+        delete w;
+        return e == cudaErrorMemoryAllocation ? fail(ctx, VDXS_E_NO_MEMORY, "8-bit weight allocation failed")
+                                              : cuda_fail(ctx, e, "8-bit weights");
+    }
+    *out = w;
+    ok(ctx);
+    return VDXS_OK;
+}
+
+VDXS_API int32_t vdxs_i8_release(vdxs_i8_weights* w) {
+    if (!w) return VDXS_OK;
+    DeviceGuard g(w->device);
+    cudaFree(w->m.q);
+    cudaFree(w->m.scale);
+    delete w;
+    return VDXS_OK;
+}
+
+VDXS_API int32_t vdxs_unembed_i8(vdxs_context* ctx, const vdxs_i8_weights* w, const int8_t* d_q, int64_t q_stride,
+                                 const float* d_scale, int32_t batch, void* d_logits, int32_t dtype,
+                                 int64_t logits_stride, void* stream) {
+    if (!ctx) return fail(nullptr, VDXS_E_INVALID_ARG, "context is NULL");
+    if (!w || !d_q || !d_scale || !d_logits)
+        return fail(ctx, VDXS_E_INVALID_ARG, "weights, q, scale or logits pointer is NULL");
+    if (dtype != VDXS_DTYPE_F32 && dtype != VDXS_DTYPE_BF16)
+        return fail(ctx, VDXS_E_INVALID_ARG, "dtype %d is neither VDXS_DTYPE_F32 nor VDXS_DTYPE_BF16", dtype);
+    if (batch < 1) return fail(ctx, VDXS_E_INVALID_ARG, "batch must be >= 1 (got %d)", batch);
+    if (batch > 65535) return fail(ctx, VDXS_E_UNSUPPORTED, "batch %d exceeds 65535", batch);
+    if (w->device != ctx->device)
+        return fail(ctx, VDXS_E_INVALID_ARG, "weights live on device %d, the context on device %d", w->device,
+                    ctx->device);
+    if (q_stride < w->m.in_dim || q_stride % 16 != 0 || !aligned(d_q, 16))
+        return fail(ctx, VDXS_E_INVALID_ARG,
+                    "q needs 16-byte aligned rows: q_stride %lld must be a multiple of 16 and >= in_dim %d",
+                    (long long)q_stride, w->m.in_dim);
+    if (logits_stride < w->m.out_dim)
+        return fail(ctx, VDXS_E_INVALID_ARG, "logits_stride %lld is smaller than out_dim %d", (long long)logits_stride,
+                    w->m.out_dim);
+    if (!aligned(d_scale, 4) || !aligned(d_logits, dtype == VDXS_DTYPE_F32 ? 4 : 2))
+        return fail(ctx, VDXS_E_INVALID_ARG, "a pointer is not aligned to its element size");
+    DeviceGuard g(ctx->device);
+    int launches = 0;
+    const cudaError_t e = unembed_i8(w->m, d_q, q_stride, d_scale, batch, d_logits, dtype, logits_stride,
+                                     (cudaStream_t)stream, &launches);
+    ctx->launches += launches;
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "8-bit unembedding");
+    ok(ctx);
+    return VDXS_OK;
+}
+
+VDXS_API int32_t vdxs_sample_unembed_i8(vdxs_context* ctx, const vdxs_config* cfg, const vdxs_i8_weights* w,
+                                        const void* d_x, int64_t x_stride, const void* d_residual,
+                                        int64_t residual_stride, int32_t dtype, const void* d_norm_weight,
+                                        int32_t weight_dtype, float eps, void* d_out_hidden, int64_t hidden_stride,
+                                        int32_t batch, const int32_t* d_history, int64_t history_stride,
+                                        const int32_t* d_history_count, const float* d_uniform,
+                                        int32_t* d_out_tokens, void* stream) {
+    if (!ctx) return fail(nullptr, VDXS_E_INVALID_ARG, "context is NULL");
+    if (!w) return fail(ctx, VDXS_E_INVALID_ARG, "weights pointer is NULL");
+    if (w->device != ctx->device)
+        return fail(ctx, VDXS_E_INVALID_ARG, "weights live on device %d, the context on device %d", w->device,
+                    ctx->device);
+    const int64_t vocab = w->m.out_dim;
+    // The whole call is checked before anything runs (the logits pointer stands for the buffer).
+    int32_t rc = validate_common(ctx, cfg, w, VDXS_DTYPE_F32, batch, w->m.out_dim, vocab, d_history, history_stride,
+                                 d_history_count, d_out_tokens);
+    if (rc != VDXS_OK) return rc;
+    if (cfg->temperature != 0.0f && !d_uniform)
+        return fail(ctx, VDXS_E_INVALID_ARG, "uniform pointer is NULL but temperature != 0");
+    NormI8Args a;
+    a.x = d_x;
+    a.x_stride = x_stride;
+    a.residual = d_residual;
+    a.residual_stride = residual_stride;
+    a.dtype = dtype;
+    a.weight = d_norm_weight;
+    a.weight_dtype = weight_dtype;
+    a.rows = batch;
+    a.dim = w->m.in_dim;
+    a.eps = eps;
+    a.hidden = d_out_hidden;
+    a.hidden_stride = hidden_stride;
+    if ((rc = check_norm(ctx, a)) != VDXS_OK) return rc;
+    DeviceGuard g(ctx->device);
+    const cudaStream_t st = (cudaStream_t)stream;
+    Workspace& ws = ctx->ws;
+    const size_t q_bytes = (size_t)batch * (size_t)w->m.pitch, n_logits = (size_t)batch * (size_t)vocab;
+    cudaError_t e;
+    if (ws.i8_q_cap < q_bytes || ws.i8_scale_cap < (size_t)batch || ws.unembed_cap < n_logits) {
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        if ((e = cudaStreamIsCapturing(st, &cap)) != cudaSuccess) return cuda_fail(ctx, e, "capture status");
+        if (cap != cudaStreamCaptureStatusNone)
+            return fail(ctx, VDXS_E_UNSUPPORTED, "the buffers would have to grow under stream capture: run one call "
+                                                 "of these shapes before");
+        if ((e = grow_dev(&ws.i8_q, &ws.i8_q_cap, q_bytes, st)) != cudaSuccess ||
+            (e = grow_dev(&ws.i8_scale, &ws.i8_scale_cap, (size_t)batch, st)) != cudaSuccess ||
+            (e = grow_dev(&ws.unembed_logits, &ws.unembed_cap, n_logits, st)) != cudaSuccess)
+            return fail(ctx, VDXS_E_NO_MEMORY, "hidden state or logits buffer allocation failed");
+    }
+    a.q = ws.i8_q;
+    a.q_stride = w->m.pitch;
+    a.scale = ws.i8_scale;
+    if ((e = rms_norm_i8(a, st)) != cudaSuccess) return cuda_fail(ctx, e, "norm launch");
+    ctx->launches += 1;
+    rc = vdxs_unembed_i8(ctx, w, ws.i8_q, w->m.pitch, ws.i8_scale, batch, ws.unembed_logits, VDXS_DTYPE_F32, vocab,
+                         stream);
+    if (rc != VDXS_OK) return rc;
+    return vdxs_sample_ex(ctx, cfg, ws.unembed_logits, VDXS_DTYPE_F32, batch, (int32_t)vocab, vocab, d_history,
+                          history_stride, d_history_count, d_uniform, d_out_tokens, nullptr, nullptr, nullptr, 0,
+                          stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------
+// Beam search.
+// ---------------------------------------------------------------------------------
+struct vdxs_beam {
+    vdxs_context* ctx = nullptr;
+    int batch = 0, beams = 0, vocab = 0, chunks = 0, chunk = 0;
+    BeamWorkspace ws;
+};
+
+namespace {
+
+void free_beam(vdxs_beam* b) {
+    cudaFree(b->ws.cand);
+    cudaFree(b->ws.part);
+    cudaFree(b->ws.best);
+    cudaFree(b->ws.lse);
+    cudaFree(b->ws.row_done);
+    cudaFree(b->ws.prompt_done);
+    cudaFree(b->ws.push);
+    delete b;
+}
+
+// Validates caches and appends them to `out` (room for n).
+int32_t check_caches(vdxs_beam* b, const vdxs_beam_cache* caches, int32_t n, BeamCacheArgs* out) {
+    const int64_t rows = (int64_t)b->batch * b->beams;
+    for (int32_t i = 0; i < n; ++i) {
+        const vdxs_beam_cache& c = caches[i];
+        if (c.segment_bytes < 0 || c.segments < 0)
+            return fail(b->ctx, VDXS_E_INVALID_ARG, "cache %d: negative size", i);
+        out[i] = BeamCacheArgs();
+        if (c.segment_bytes == 0 || c.segments == 0) continue;
+        if (!c.src || !c.dst) return fail(b->ctx, VDXS_E_INVALID_ARG, "cache %d: NULL pointer", i);
+        // Extent of a row and of all rows, in 128 bits: strides are the caller's.
+        __int128 lo[2], hi[2];
+        const unsigned char* base[2] = {(const unsigned char*)c.src, (const unsigned char*)c.dst};
+        const int64_t row[2] = {c.src_row_stride, c.dst_row_stride};
+        const int64_t seg[2] = {c.src_segment_stride, c.dst_segment_stride};
+        for (int s = 0; s < 2; ++s) {
+            if (row[s] < 0 || seg[s] < 0 || (c.segments > 1 && seg[s] < c.segment_bytes))
+                return fail(b->ctx, VDXS_E_INVALID_ARG, "cache %d: a segment stride is smaller than the segment", i);
+            const __int128 one = (__int128)(c.segments - 1) * seg[s] + c.segment_bytes;
+            // Rows lie behind one another, or inside one another's segment gaps.
+            const bool inside = (__int128)row[s] * (rows - 1) + c.segment_bytes <= seg[s] && row[s] >= c.segment_bytes;
+            if (rows > 1 && row[s] < one && !(c.segments > 1 && inside))
+                return fail(b->ctx, VDXS_E_INVALID_ARG, "cache %d: rows overlap one another", i);
+            lo[s] = (__int128)(uintptr_t)base[s];
+            hi[s] = lo[s] + (__int128)(rows - 1) * row[s] + one;
+            if (hi[s] - lo[s] > ((__int128)1 << 50))
+                return fail(b->ctx, VDXS_E_INVALID_ARG, "cache %d: strides reach too far", i);
+        }
+        const bool same = base[0] == base[1];
+        if (same && (row[0] != row[1] || (c.segments > 1 && seg[0] != seg[1])))
+            return fail(b->ctx, VDXS_E_INVALID_ARG, "cache %d: in place needs equal strides", i);
+        if (!same && lo[0] < hi[1] && lo[1] < hi[0])
+            return fail(b->ctx, VDXS_E_INVALID_ARG, "cache %d: source and target overlap", i);
+        out[i].src = base[0];
+        out[i].dst = (unsigned char*)c.dst;
+        out[i].src_row = row[0];
+        out[i].dst_row = row[1];
+        out[i].src_segment = c.segments > 1 ? seg[0] : 0;
+        out[i].dst_segment = c.segments > 1 ? seg[1] : 0;
+        out[i].segment_bytes = c.segment_bytes;
+        out[i].segments = c.segments;
+    }
+    return VDXS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+VDXS_API int32_t vdxs_beam_create(vdxs_context* ctx, int32_t batch, int32_t beams, int32_t vocab, vdxs_beam** out) {
+    if (!ctx) return fail(nullptr, VDXS_E_INVALID_ARG, "context is NULL");
+    if (!out) return fail(ctx, VDXS_E_INVALID_ARG, "output pointer is NULL");
+    *out = nullptr;
+    if (batch < 1) return fail(ctx, VDXS_E_INVALID_ARG, "batch must be >= 1 (got %d)", batch);
+    if (beams < 1) return fail(ctx, VDXS_E_INVALID_ARG, "beams must be >= 1 (got %d)", beams);
+    if (vocab < 1) return fail(ctx, VDXS_E_INVALID_ARG, "vocab must be >= 1 (got %d)", vocab);
+    if (beams > VDXS_BEAM_MAX_BEAMS)
+        return fail(ctx, VDXS_E_UNSUPPORTED, "beams %d exceeds %d", beams, VDXS_BEAM_MAX_BEAMS);
+    if ((int64_t)batch * beams > 65535)
+        return fail(ctx, VDXS_E_UNSUPPORTED, "batch * beams %lld exceeds 65535", (long long)batch * beams);
+    if (vocab > (1 << 24)) return fail(ctx, VDXS_E_UNSUPPORTED, "vocab %d exceeds %d", vocab, 1 << 24);
+    DeviceGuard g(ctx->device);
+    auto* b = new (std::nothrow) vdxs_beam();
+    if (!b) return fail(ctx, VDXS_E_NO_MEMORY, "out of host memory");
+    b->ctx = ctx;
+    b->batch = batch;
+    b->beams = beams;
+    b->vocab = vocab;
+    const size_t rows = (size_t)batch * beams;
+    beam_plan((int)rows, vocab, ctx->sm_count, &b->chunks, &b->chunk);
+    const size_t lists = rows * (size_t)b->chunks;
+    cudaError_t e;
+    if ((e = cudaMalloc((void**)&b->ws.cand, lists * beams * 8)) != cudaSuccess ||
+        (e = cudaMalloc((void**)&b->ws.part, lists * 16)) != cudaSuccess ||
+        (e = cudaMalloc((void**)&b->ws.best, rows * beams * 8)) != cudaSuccess ||
+        (e = cudaMalloc((void**)&b->ws.lse, rows * 8)) != cudaSuccess ||
+        (e = cudaMalloc((void**)&b->ws.row_done, rows * 4)) != cudaSuccess ||
+        (e = cudaMalloc((void**)&b->ws.prompt_done, (size_t)batch * 4)) != cudaSuccess ||
+        (e = cudaMalloc((void**)&b->ws.push, rows * 4)) != cudaSuccess ||
+        (e = cudaMemset(b->ws.row_done, 0, rows * 4)) != cudaSuccess ||
+        (e = cudaMemset(b->ws.prompt_done, 0, (size_t)batch * 4)) != cudaSuccess ||
+        (e = cudaStreamSynchronize(nullptr)) != cudaSuccess) {
+        free_beam(b);
+        return e == cudaErrorMemoryAllocation ? fail(ctx, VDXS_E_NO_MEMORY, "beam search workspace allocation failed")
+                                              : cuda_fail(ctx, e, "beam search workspace");
+    }
+    *out = b;
+    ok(ctx);
+    return VDXS_OK;
+}
+
+VDXS_API int32_t vdxs_beam_destroy(vdxs_beam* b) {
+    if (!b) return VDXS_OK;
+    DeviceGuard g(b->ctx->device);
+    free_beam(b);
+    return VDXS_OK;
+}
+
+VDXS_API int32_t vdxs_beam_step(vdxs_beam* b, const vdxs_beam_config* cfg, const void* d_logits, int32_t dtype,
+                                int64_t row_stride, const vdxs_beam_rows* in, const vdxs_beam_rows* out,
+                                const int32_t* d_stop_ids, int32_t n_stop, const vdxs_beam_cache* caches,
+                                int32_t n_caches, int32_t* d_out_tokens, int32_t* d_out_parents, void* stream) {
+    if (!b) return fail(nullptr, VDXS_E_INVALID_ARG, "beam search is NULL");
+    vdxs_context* ctx = b->ctx;
+    if (!cfg || !d_logits || !in || !out || !d_out_tokens || !d_out_parents)
+        return fail(ctx, VDXS_E_INVALID_ARG, "NULL argument");
+    if (dtype != VDXS_DTYPE_F32 && dtype != VDXS_DTYPE_BF16)
+        return fail(ctx, VDXS_E_INVALID_ARG, "dtype %d is neither VDXS_DTYPE_F32 nor VDXS_DTYPE_BF16", dtype);
+    if (!aligned(d_logits, dtype == VDXS_DTYPE_F32 ? 4 : 2))
+        return fail(ctx, VDXS_E_INVALID_ARG, "the logits pointer is not aligned to its element size");
+    if (row_stride < b->vocab)
+        return fail(ctx, VDXS_E_INVALID_ARG, "row_stride %lld is smaller than vocab %d", (long long)row_stride,
+                    b->vocab);
+    if (cfg->reserved != 0) return fail(ctx, VDXS_E_INVALID_ARG, "reserved must be 0");
+    if (!(cfg->length_alpha >= -1e6 && cfg->length_alpha <= 1e6))
+        return fail(ctx, VDXS_E_INVALID_ARG, "length_alpha must be within +-1e6");
+    if (!(cfg->repeat_penalty > 0.0f) || cfg->repeat_penalty > 3.4e38f)
+        return fail(ctx, VDXS_E_INVALID_ARG, "repeat_penalty must be finite and above 0");
+    if (cfg->window < 0 || cfg->window > kMaxHistory)
+        return fail(ctx, VDXS_E_INVALID_ARG, "window %d out of range [0,%d]", cfg->window, kMaxHistory);
+    if (!in->scores || !in->lengths || !in->finished || !out->scores || !out->lengths || !out->finished)
+        return fail(ctx, VDXS_E_INVALID_ARG, "scores, lengths or finished are NULL");
+    if (cfg->window > 0 && (!in->hist || !in->hist_pos || !in->hist_count || !out->hist || !out->hist_pos ||
+                            !out->hist_count))
+        return fail(ctx, VDXS_E_INVALID_ARG, "history ring buffers are NULL");
+    if (n_stop < 0 || (n_stop > 0 && !d_stop_ids))
+        return fail(ctx, VDXS_E_INVALID_ARG, "stop list: n_stop %d with a NULL buffer", n_stop);
+    if (n_caches < 0 || (n_caches > 0 && !caches))
+        return fail(ctx, VDXS_E_INVALID_ARG, "n_caches %d with a NULL list", n_caches);
+    BeamArgs a;
+    a.logits = d_logits;
+    a.dtype = dtype;
+    a.stride = row_stride;
+    a.batch = b->batch;
+    a.beams = b->beams;
+    a.vocab = b->vocab;
+    a.chunks = b->chunks;
+    a.chunk = b->chunk;
+    a.penalty = cfg->repeat_penalty;
+    a.window = cfg->window;
+    a.alpha = cfg->length_alpha;
+    a.pad = cfg->pad_token;
+    a.scores_in = in->scores;
+    a.lengths_in = in->lengths;
+    a.finished_in = in->finished;
+    a.hist_in = in->hist;
+    a.pos_in = in->hist_pos;
+    a.count_in = in->hist_count;
+    a.scores = out->scores;
+    a.lengths = out->lengths;
+    a.finished = out->finished;
+    a.hist = out->hist;
+    a.pos = out->hist_pos;
+    a.count = out->hist_count;
+    a.stop_ids = d_stop_ids;
+    a.n_stop = n_stop;
+    a.tokens = d_out_tokens;
+    a.parents = d_out_parents;
+    a.ws = b->ws;
+    auto* moved = new (std::nothrow) BeamCacheArgs[(size_t)n_caches + 1];
+    if (!moved) return fail(ctx, VDXS_E_NO_MEMORY, "out of host memory");
+    const int32_t rc = check_caches(b, caches, n_caches, moved);
+    if (rc != VDXS_OK) {
+        delete[] moved;
+        return rc;
+    }
+    DeviceGuard g(ctx->device);
+    const cudaStream_t st = (cudaStream_t)stream;
+    int launches = 1;
+    cudaError_t e = beam_select(a, st);
+    if (e == cudaSuccess) e = beam_reorder(a, a.window > 0, moved, n_caches, st, &launches);
+    delete[] moved;
+    ctx->launches += launches;
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "beam step launch");
+    ok(ctx);
+    return VDXS_OK;
+}
+
+VDXS_API int32_t vdxs_beam_reorder(vdxs_beam* b, const int32_t* d_parents, const vdxs_beam_cache* caches,
+                                   int32_t n_caches, void* stream) {
+    if (!b) return fail(nullptr, VDXS_E_INVALID_ARG, "beam search is NULL");
+    if (!d_parents) return fail(b->ctx, VDXS_E_INVALID_ARG, "parents pointer is NULL");
+    if (n_caches < 0 || (n_caches > 0 && !caches))
+        return fail(b->ctx, VDXS_E_INVALID_ARG, "n_caches %d with a NULL list", n_caches);
+    auto* moved = new (std::nothrow) BeamCacheArgs[(size_t)n_caches + 1];
+    if (!moved) return fail(b->ctx, VDXS_E_NO_MEMORY, "out of host memory");
+    const int32_t rc = check_caches(b, caches, n_caches, moved);
+    if (rc != VDXS_OK) {
+        delete[] moved;
+        return rc;
+    }
+    BeamArgs a;
+    a.batch = b->batch;
+    a.beams = b->beams;
+    a.parents = const_cast<int32_t*>(d_parents);
+    DeviceGuard g(b->ctx->device);
+    int launches = 0;
+    const cudaError_t e = beam_reorder(a, false, moved, n_caches, (cudaStream_t)stream, &launches);
+    delete[] moved;
+    b->ctx->launches += launches;
+    if (e != cudaSuccess) return cuda_fail(b->ctx, e, "beam reorder launch");
+    ok(b->ctx);
+    return VDXS_OK;
 }
 
 }  // extern "C"

@@ -53,6 +53,9 @@ struct Workspace {
     size_t lk_cap = 0;              // 64-bit words
     float* unembed_logits = nullptr;  // vdxs_sample_unembed_q4_0: [rows * vocab] logits
     size_t unembed_cap = 0;
+    int8_t* i8_q = nullptr;           // vdxs_sample_unembed_i8: [rows * pitch] normed hidden states
+    float* i8_scale = nullptr;        // and their scales [rows]; its logits are unembed_logits
+    size_t i8_q_cap = 0, i8_scale_cap = 0;
     int32_t* err = nullptr;         // device error word (0 = ok)
     // host-buffer entry point staging
     void* d_logits = nullptr;
@@ -141,6 +144,75 @@ cudaError_t q4_0_repack(const uint8_t* src, int in_dim, int out_dim, uint32_t* n
                         cudaStream_t stream);
 cudaError_t q4_0_matvec(const uint32_t* nib, const uint16_t* scales, int in_dim, int out_dim, const float* x,
                         int batch, float* out, cudaStream_t stream, int* launches);
+// Norm, residual and 8-bit output, and the 8-bit unembedding (vdxs_i8.cu).
+struct NormI8Args {
+    const void* x = nullptr;
+    int64_t x_stride = 0;
+    const void* residual = nullptr;
+    int64_t residual_stride = 0;
+    int dtype = 0;
+    const void* weight = nullptr;
+    int weight_dtype = 0;
+    int rows = 0, dim = 0;
+    float eps = 0.0f;
+    void* hidden = nullptr;
+    int64_t hidden_stride = 0;
+    int8_t* q = nullptr;
+    int64_t q_stride = 0;
+    float* scale = nullptr;
+};
+struct I8Matrix {            // weights as the product reads them
+    int8_t* q = nullptr;     // [out_dim][pitch], the bytes behind in_dim are not read
+    float* scale = nullptr;  // [out_dim]
+    int in_dim = 0, out_dim = 0;
+    int64_t pitch = 0;       // bytes between rows: in_dim rounded up to 16
+};
+cudaError_t rms_norm_i8(const NormI8Args& a, cudaStream_t stream);
+// Rows of fp32/bf16/fp16 (format 0..2) or Q4_0 blocks (4) to 8 bits with a scale per row.
+cudaError_t quantise_rows_i8(const void* src, int format, int64_t row_stride, const I8Matrix& w, cudaStream_t stream);
+cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, const float* scale, int batch,
+                       void* logits, int dtype, int64_t logits_stride, cudaStream_t stream, int* launches);
+// Beam search (vdxs_beam.cu).
+struct BeamWorkspace {
+    unsigned long long* cand = nullptr;  // [rows][chunks][beams] each chunk's best (key, token), best first
+    double* part = nullptr;              // [rows][chunks][2] each chunk's maximum and sum of exponentials
+    unsigned long long* best = nullptr;  // [rows][beams] each row's best
+    double* lse = nullptr;               // [rows] log of the sum of exponentials
+    uint32_t* row_done = nullptr;        // [rows] chunks done, self-resetting
+    uint32_t* prompt_done = nullptr;     // [batch] rows done, self-resetting
+    int32_t* push = nullptr;             // [rows] 1: the row's ring takes the new token
+};
+struct BeamArgs {
+    const void* logits = nullptr;
+    int dtype = 0;
+    int64_t stride = 0;
+    int batch = 0, beams = 0, vocab = 0, chunks = 0, chunk = 0;
+    float penalty = 1.0f;
+    int window = 0;
+    double alpha = 0.0;
+    int32_t pad = 0;
+    const float* scores_in = nullptr;
+    const int32_t *lengths_in = nullptr, *finished_in = nullptr, *hist_in = nullptr, *pos_in = nullptr,
+                  *count_in = nullptr;
+    float* scores = nullptr;
+    int32_t *lengths = nullptr, *finished = nullptr, *hist = nullptr, *pos = nullptr, *count = nullptr;
+    const int32_t* stop_ids = nullptr;
+    int n_stop = 0;
+    int32_t *tokens = nullptr, *parents = nullptr;
+    BeamWorkspace ws;
+};
+struct BeamCacheArgs {  // vdxs_beam_cache
+    const unsigned char* src = nullptr;
+    unsigned char* dst = nullptr;
+    int64_t src_row = 0, src_segment = 0, dst_row = 0, dst_segment = 0, segment_bytes = 0, segments = 0;
+};
+// Chunks of a row of `vocab` logits (at most kBeamMaxChunks) and their length.
+constexpr int kBeamMaxChunks = 64;
+void beam_plan(int rows, int vocab, int sm_count, int* chunks, int* chunk);
+cudaError_t beam_select(const BeamArgs& a, cudaStream_t stream);
+// Rings (where a.window > 0 and rings is true) and caches by a.parents.
+cudaError_t beam_reorder(const BeamArgs& a, bool rings, const BeamCacheArgs* caches, int n_caches, cudaStream_t stream,
+                         int* launches);
 // Device-resident decode state (one thread per row).
 cudaError_t launch_device_uniforms(uint64_t* prng, int batch, float* out, cudaStream_t stream);
 cudaError_t launch_history_push(int32_t* hist, int32_t* pos, int32_t* count, int window, const int32_t* tokens,

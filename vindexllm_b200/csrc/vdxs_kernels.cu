@@ -3770,6 +3770,8 @@ void free_workspace(Workspace& ws) {
     cudaFree(ws.shard_recv);
     cudaFree(ws.lk_buf);
     cudaFree(ws.unembed_logits);
+    cudaFree(ws.i8_q);
+    cudaFree(ws.i8_scale);
     cudaFree(ws.err);
     cudaFree(ws.d_logits);
     cudaFree(ws.d_hist);

@@ -17,8 +17,8 @@ from . import abi
 from ._lib import load, check, VdxsError
 from .abi import VdxsConfig, default_config
 
-__all__ = ["SamplerContext", "TVdxSampler", "ShardComm", "DeviceDecodeState", "VdxsError", "default_config",
-           "shard_range", "broadcast_unique_id"]
+__all__ = ["SamplerContext", "TVdxSampler", "ShardComm", "DeviceDecodeState", "Q4Weights", "I8Weights", "BeamSearch",
+           "BeamState", "VdxsError", "default_config", "shard_range", "broadcast_unique_id"]
 
 
 def _stream_ptr(stream):
@@ -39,6 +39,46 @@ def _dtype_code(t) -> int:
 
 def _dptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
+
+
+def _hidden_code(t, what: str) -> int:
+    """VDXS_DTYPE_* of a hidden state or norm weight."""
+    import torch
+    codes = {torch.float32: abi.DTYPE_F32, torch.bfloat16: abi.DTYPE_BF16, torch.float16: abi.DTYPE_F16}
+    if t.dtype not in codes:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return codes[t.dtype]
+
+
+def _on(device: int, stream):
+    """(stream, context manager): the stream of a call on `device` (its current one when
+    None), under which the call's outputs are allocated, so that their memory is reused in
+    that stream's order."""
+    import torch
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    return stream, torch.cuda.stream(stream)
+
+
+def _need(t, what: str, device: int, dtype=None, shape=None, rows=False):
+    """Argument check of a device tensor: its device, type and shape; contiguous, or with
+    `rows` a matrix whose rows are contiguous."""
+    if not t.is_cuda or t.device.index != device:
+        raise ValueError(f"{what} must be a tensor on cuda:{device}, got {t.device}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if rows and (t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1)):
+        raise ValueError(f"{what} must be a matrix with contiguous rows")
+    if not rows and not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+    return t
+
+
+def _pitch(t) -> int:
+    """Elements between the rows of a matrix (a lone row's stride says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
 
 
 class SamplerContext:
@@ -117,6 +157,38 @@ class SamplerContext:
         if flags is None:
             return tokens
         return tokens, flags, oi, op
+
+    def rms_norm_i8(self, x, weight, eps: float = 1e-6, residual=None, out_hidden=None, q=None, scale=None,
+                    stream=None):
+        """vdxs_rms_norm_i8: (q, scale, hidden) of the rows of ``x`` [rows, dim]; hidden is
+        x + residual (None without a residual and without ``out_hidden``). ``out_hidden`` may be
+        ``x`` or ``residual`` for an update in place. A ``q`` made here has rows padded to a
+        multiple of 16 bytes, as ``I8Weights.unembed`` takes it."""
+        import torch
+        code = _hidden_code(x, "x")
+        _need(x, "x", self.device, rows=True)
+        rows, dim = x.shape
+        wcode = _hidden_code(weight, "weight")
+        _need(weight, "weight", self.device, shape=(dim,))
+        if residual is not None:
+            _need(residual, "residual", self.device, x.dtype, x.shape, rows=True)
+        stream, on = _on(self.device, stream)
+        with on:
+            if out_hidden is None and residual is not None:
+                out_hidden = torch.empty(rows, dim, dtype=x.dtype, device=x.device)
+            if q is None:
+                q = torch.empty(rows, -(-dim // 16) * 16, dtype=torch.int8, device=x.device)[:, :dim]
+            if scale is None:
+                scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+        if out_hidden is not None:
+            _need(out_hidden, "out_hidden", self.device, x.dtype, x.shape, rows=True)
+        _need(q, "q", self.device, torch.int8, x.shape, rows=True)
+        _need(scale, "scale", self.device, torch.float32, (rows,))
+        check(self.lib.vdxs_rms_norm_i8(self._h, _dptr(x), _pitch(x), _dptr(residual),
+                                        0 if residual is None else _pitch(residual), code, _dptr(weight), wcode, rows,
+                                        dim, eps, _dptr(out_hidden), 0 if out_hidden is None else _pitch(out_hidden),
+                                        _dptr(q), _pitch(q), _dptr(scale), _stream_ptr(stream)), self._h)
+        return q, scale, out_hidden
 
     def sample_host(self, cfg: VdxsConfig, logits: np.ndarray, uniforms=None, history=None,
                     history_count=None, vocab: int | None = None, stream=None, out=None):
@@ -408,3 +480,244 @@ class Q4Weights:
                                                 _dptr(history), hs, _dptr(history_count), _dptr(uniforms),
                                                 _dptr(tokens), _stream_ptr(stream)), self.ctx.handle)
         return tokens
+
+
+class I8Weights:
+    """An unembedding matrix in 8-bit integers with a scale for each vocabulary entry
+    (vdxs_i8_prepare): the final norm, the product on the integer tensor cores and the
+    sampler for every batch size. Stands beside Q4Weights, whose matvec keeps the reference's
+    order of sums and serves small batches."""
+
+    def __init__(self, ctx: SamplerContext, weight, scales=None, stream=None):
+        """``weight`` [out_dim, in_dim]: int8 with ``scales`` [out_dim] float32, or float32,
+        bfloat16 or float16, quantised here row by row."""
+        import torch
+        formats = {torch.float32: abi.WEIGHTS_F32, torch.bfloat16: abi.WEIGHTS_BF16, torch.float16: abi.WEIGHTS_F16,
+                   torch.int8: abi.WEIGHTS_I8}
+        if weight.dtype not in formats:
+            raise TypeError(f"weight must be int8, float32, bfloat16 or float16, got {weight.dtype}")
+        _need(weight, "weight", ctx.device, rows=True)
+        out_dim, in_dim = weight.shape
+        if (weight.dtype == torch.int8) != (scales is not None):
+            raise ValueError("scales go with int8 weights, and with those alone")
+        if scales is not None:
+            _need(scales, "scales", ctx.device, torch.float32, (out_dim,))
+        self._prepare(ctx, weight, formats[weight.dtype], scales, _pitch(weight), in_dim, out_dim, stream)
+
+    @classmethod
+    def from_q4_0(cls, ctx: SamplerContext, q4_0, in_dim: int, out_dim: int, stream=None) -> "I8Weights":
+        """From the reference's Q4_0 blocks (the uint8 tensor that Q4Weights takes)."""
+        import torch
+        _need(q4_0, "q4_0", ctx.device, torch.uint8)
+        if q4_0.numel() != out_dim * (in_dim // 32) * 18:
+            raise ValueError(f"{q4_0.numel()} bytes are not {out_dim} x {in_dim} in Q4_0 blocks")
+        w = cls.__new__(cls)
+        w._prepare(ctx, q4_0, abi.WEIGHTS_Q4_0, None, in_dim, in_dim, out_dim, stream)
+        return w
+
+    def _prepare(self, ctx, weight, fmt, scales, stride, in_dim, out_dim, stream):
+        self.ctx, self.lib = ctx, ctx.lib
+        self.in_dim, self.out_dim = in_dim, out_dim
+        stream, _ = _on(ctx.device, stream)
+        h = C.c_void_p()
+        check(self.lib.vdxs_i8_prepare(ctx.handle, _dptr(weight), fmt, _dptr(scales), stride, in_dim, out_dim,
+                                       _stream_ptr(stream), C.byref(h)), ctx.handle)
+        self._h = h
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self.lib.vdxs_i8_release(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def unembed(self, q, scale, logits=None, dtype=None, stream=None):
+        """logits [batch, out_dim] (float32 or bfloat16) of 8-bit rows ``q`` [batch, in_dim] with
+        ``scale`` [batch], as SamplerContext.rms_norm_i8 returns them."""
+        import torch
+        dev = self.ctx.device
+        _need(q, "q", dev, torch.int8, (q.shape[0], self.in_dim), rows=True)
+        _need(scale, "scale", dev, torch.float32, (q.shape[0],))
+        stream, on = _on(dev, stream)
+        if logits is None:
+            with on:
+                logits = torch.empty(q.shape[0], self.out_dim, dtype=dtype or torch.float32, device=q.device)
+        _need(logits, "logits", dev, dtype, (q.shape[0], self.out_dim), rows=True)
+        pitch = q.stride(0) if q.shape[0] > 1 else -(-self.in_dim // 16) * 16
+        check(self.lib.vdxs_unembed_i8(self.ctx.handle, self._h, _dptr(q), pitch, _dptr(scale), q.shape[0],
+                                       _dptr(logits), _dtype_code(logits), _pitch(logits), _stream_ptr(stream)),
+              self.ctx.handle)
+        return logits
+
+    def sample(self, cfg: VdxsConfig, x, norm_weight, eps: float = 1e-6, residual=None, out_hidden=None, uniforms=None,
+               history=None, history_count=None, tokens=None, stream=None):
+        """vdxs_sample_unembed_i8: norm, unembedding and sampling in one call; returns tokens."""
+        import torch
+        dev = self.ctx.device
+        code, wcode = _hidden_code(x, "x"), _hidden_code(norm_weight, "norm_weight")
+        _need(x, "x", dev, shape=(x.shape[0], self.in_dim), rows=True)
+        _need(norm_weight, "norm_weight", dev, shape=(self.in_dim,))
+        for t, what in ((residual, "residual"), (out_hidden, "out_hidden")):
+            if t is not None:
+                _need(t, what, dev, x.dtype, x.shape, rows=True)
+        B = x.shape[0]
+        stream, on = _on(dev, stream)
+        if tokens is None:
+            with on:
+                tokens = torch.empty(B, dtype=torch.int32, device=x.device)
+        hs = history.shape[1] if history is not None else 1
+        check(self.lib.vdxs_sample_unembed_i8(self.ctx.handle, C.byref(cfg), self._h, _dptr(x), _pitch(x),
+                                              _dptr(residual), 0 if residual is None else _pitch(residual), code,
+                                              _dptr(norm_weight), wcode, eps, _dptr(out_hidden),
+                                              0 if out_hidden is None else _pitch(out_hidden), B, _dptr(history), hs,
+                                              _dptr(history_count), _dptr(uniforms), _dptr(tokens),
+                                              _stream_ptr(stream)), self.ctx.handle)
+        return tokens
+
+
+class BeamState:
+    """Device state of a search's batch * beams rows (vdxs_beam_rows): cumulative scores,
+    lengths, finished flags and, with window > 0, the penalty rings. A new state is that of
+    a search at its start: beam 0 of each prompt has score 0, the others -infinity."""
+
+    def __init__(self, batch: int, beams: int, window: int = 0, device=None, scores=None, lengths=None, finished=None,
+                 hist=None, pos=None, count=None):
+        import torch
+        if device is None:
+            device = scores.device if scores is not None else torch.device("cuda", torch.cuda.current_device())
+        rows = batch * beams
+        self.batch, self.beams, self.window = batch, beams, window
+
+        def own(t, dtype, *shape):
+            if t is None:
+                return torch.zeros(shape, dtype=dtype, device=device)
+            return _need(t, "state", t.device.index if t.is_cuda else -1, dtype, shape)
+
+        if scores is None:
+            scores = torch.full((batch, beams), -float("inf"), dtype=torch.float32, device=device)
+            scores[:, 0] = 0.0
+            scores = scores.view(-1)
+        self.scores = own(scores, torch.float32, rows)
+        self.lengths = own(lengths, torch.int32, rows)
+        self.finished = own(finished, torch.int32, rows)
+        self.hist = own(hist, torch.int32, rows, window) if window else None
+        self.pos = own(pos, torch.int32, rows) if window else None
+        self.count = own(count, torch.int32, rows) if window else None
+
+    def rows(self) -> abi.VdxsBeamRows:
+        def p(t):
+            return None if t is None else t.data_ptr()
+        return abi.VdxsBeamRows(p(self.scores), p(self.lengths), p(self.finished), p(self.hist), p(self.pos),
+                                p(self.count))
+
+
+def _cache_pieces(t, what: str, most: int | None = None):
+    """(row stride, segment stride, segment bytes, segments) of a tensor [rows, ...] whose rows are
+    one contiguous piece, or equal pieces (of at most `most` bytes) at one distance."""
+    size, inner = t.element_size(), 1
+    dims = [(n, s) for n, s in zip(t.shape[1:], t.stride()[1:]) if n != 1]
+    while dims and dims[-1][1] == inner and (most is None or inner * size < most):
+        inner *= dims.pop()[0]
+    count, step = 1, inner
+    while dims:
+        n, s = dims.pop()
+        if count == 1:
+            step = s
+        elif s != step * count:
+            raise ValueError(f"{what}: the rows of strides {t.stride()} are not equal pieces at one distance")
+        count *= n
+    row = t.stride(0) if t.shape[0] > 1 else step * count
+    return row * size, step * size, inner * size, count
+
+
+class BeamSearch:
+    """A beam search of ``batch`` prompts with ``beams`` beams each over ``vocab`` tokens
+    (vdxs_beam): the selection over beams and vocabulary, with the reordering of the rows.
+    The reference decodes one sequence and has no counterpart."""
+
+    def __init__(self, ctx: SamplerContext, batch: int, beams: int, vocab: int):
+        self.ctx, self.lib = ctx, ctx.lib
+        self.batch, self.beams, self.vocab = batch, beams, vocab
+        h = C.c_void_p()
+        check(self.lib.vdxs_beam_create(ctx.handle, batch, beams, vocab, C.byref(h)), ctx.handle)
+        self._h = h
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self.lib.vdxs_beam_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _caches(self, caches):
+        """A cache is a tensor [rows, ...] (in place) or a pair (source, target) of them; a view
+        of the filled part moves that part alone."""
+        n = len(caches)
+        out = (abi.VdxsBeamCache * max(n, 1))()
+        for i, c in enumerate(caches):
+            src, dst = c if isinstance(c, (tuple, list)) else (c, c)
+            for t in (src, dst):
+                if not t.is_cuda or t.device.index != self.ctx.device:
+                    raise ValueError(f"cache {i} must be on cuda:{self.ctx.device}, got {t.device}")
+                if t.dim() < 1 or t.shape[0] != self.batch * self.beams:
+                    raise ValueError(f"cache {i} must have {self.batch * self.beams} rows, got shape {tuple(t.shape)}")
+            if src.shape != dst.shape or src.dtype != dst.dtype:
+                raise ValueError(f"cache {i}: source and target differ in shape or type")
+            if src.numel() == 0:
+                continue  # a zeroed entry has no bytes to move
+            a, b = _cache_pieces(src, f"cache {i}"), _cache_pieces(dst, f"cache {i}")
+            if a[2] != b[2]:  # the smaller pieces of the two
+                a, b = (_cache_pieces(t, f"cache {i}", min(a[2], b[2])) for t in (src, dst))
+            if a[2:] != b[2:]:
+                raise ValueError(f"cache {i}: source and target are laid out in different pieces")
+            out[i] = abi.VdxsBeamCache(src.data_ptr(), dst.data_ptr(), a[0], a[1], b[0], b[1], a[2], a[3])
+        return out, n
+
+    def step(self, state: BeamState, logits, out: BeamState | None = None, stop_ids=None, pad_token: int = 0,
+             repeat_penalty: float = 1.0, length_alpha: float = 0.0, caches=(), tokens=None, parents=None, stream=None):
+        """One step (vdxs_beam_step): (tokens, parents) as int32 [batch, beams]. ``out`` receives the
+        rows after it (``state`` itself, in place, when None)."""
+        import torch
+        dev, rows = self.ctx.device, self.batch * self.beams
+        out = state if out is None else out
+        _need(logits, "logits", dev, shape=(rows, self.vocab), rows=True)
+        for s in (state, out):
+            if (s.batch, s.beams, s.window) != (self.batch, self.beams, state.window):
+                raise ValueError(f"a state of {s.batch} x {s.beams}, window {s.window}, for a search of {self.batch} x "
+                                 f"{self.beams}, window {state.window}")
+            if s.scores.device.index != dev:
+                raise ValueError(f"the state is on {s.scores.device}, the search on cuda:{dev}")
+        if stop_ids is not None:
+            _need(stop_ids, "stop_ids", dev, torch.int32)
+        stream, on = _on(dev, stream)
+        with on:
+            if tokens is None:
+                tokens = torch.empty(self.batch, self.beams, dtype=torch.int32, device=logits.device)
+            if parents is None:
+                parents = torch.empty(self.batch, self.beams, dtype=torch.int32, device=logits.device)
+        _need(tokens, "tokens", dev, torch.int32, (self.batch, self.beams))
+        _need(parents, "parents", dev, torch.int32, (self.batch, self.beams))
+        cfg = abi.VdxsBeamConfig(length_alpha, repeat_penalty, state.window, pad_token, 0)
+        a, b = state.rows(), out.rows()
+        moved, n = self._caches(caches)
+        check(self.lib.vdxs_beam_step(self._h, C.byref(cfg), _dptr(logits), _dtype_code(logits), _pitch(logits),
+                                      C.byref(a), C.byref(b), _dptr(stop_ids),
+                                      0 if stop_ids is None else int(stop_ids.numel()), moved, n, _dptr(tokens),
+                                      _dptr(parents), _stream_ptr(stream)), self.ctx.handle)
+        return tokens, parents
+
+    def reorder(self, parents, caches, stream=None):
+        """Moves caches by a step's parents (vdxs_beam_reorder)."""
+        import torch
+        _need(parents, "parents", self.ctx.device, torch.int32, (self.batch, self.beams))
+        stream, _ = _on(self.ctx.device, stream)
+        moved, n = self._caches(caches)
+        check(self.lib.vdxs_beam_reorder(self._h, _dptr(parents), moved, n, _stream_ptr(stream)), self.ctx.handle)
