@@ -214,6 +214,14 @@ VDXS_API int32_t vdxs_create(int32_t device, vdxs_context** out) {
         return fail(nullptr, VDXS_E_UNSUPPORTED, "device %d is compute capability %d.x; this library is built for sm_100a",
                     device, major);
     }
+    // The error word that kernels set instead of trapping.
+    if ((e = cudaMalloc((void**)&ctx->ws.err, sizeof(int32_t))) != cudaSuccess ||
+        (e = cudaMemset(ctx->ws.err, 0, sizeof(int32_t))) != cudaSuccess ||
+        (e = cudaStreamSynchronize(nullptr)) != cudaSuccess) {
+        cudaFree(ctx->ws.err);
+        delete ctx;
+        return cuda_fail(nullptr, e, "error word");
+    }
     *out = ctx;
     ok(ctx);
     return VDXS_OK;
@@ -1445,7 +1453,7 @@ VDXS_API int32_t vdxs_unembed_i8(vdxs_context* ctx, const vdxs_i8_weights* w, co
     DeviceGuard g(ctx->device);
     int launches = 0;
     const cudaError_t e = unembed_i8(w->m, d_q, q_stride, d_scale, batch, d_logits, dtype, logits_stride,
-                                     (cudaStream_t)stream, &launches);
+                                     ctx->ws.err, ctx->sm_count, (cudaStream_t)stream, &launches);
     ctx->launches += launches;
     if (e != cudaSuccess) return cuda_fail(ctx, e, "8-bit unembedding");
     ok(ctx);

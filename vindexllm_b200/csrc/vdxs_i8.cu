@@ -1,7 +1,7 @@
-// vdxs_i8.cu - the 8-bit unembedding: the final norm with an 8-bit output (residual's
-// addition, root-mean-square norm, a scale per token) and the product with 8-bit weights
-// that have a scale per vocabulary entry. It stands where TVdxModel.UnembedToLogits
-// (src/VindexLLM.Model.pas:1258-1271) runs the norm and the tied-embedding product.
+// vdxs_i8.cu - the operands of the 8-bit unembedding: the final norm with an 8-bit output
+// (residual's addition, root-mean-square norm, a scale per token), and the weights with a
+// scale per vocabulary entry. The norm stands where TVdxModel.UnembedToLogits
+// (src/VindexLLM.Model.pas:1258-1271) runs it; the product is in vdxs_i8_product.cu.
 #include "vdxs_internal.h"
 #include "../../include/vdx_sampler.h"
 
@@ -128,30 +128,6 @@ __global__ void __launch_bounds__(kNormThreads) quantise_rows_kernel(S src, I8Ma
             bad || top == 0.0 || i >= w.in_dim ? 0 : (int8_t)quantum((double)src.at(row, i), top);
 }
 
-template <typename O>
-__device__ __forceinline__ O scaled(int acc, float ws, float xs) {
-    return from_f32<O>(__fmul_rn(__fmul_rn((float)acc, ws), xs));
-}
-
-// One vocabulary entry per warp, four-byte words across the lanes.
-template <typename O>
-__global__ void __launch_bounds__(256) unembed_i8_kernel(I8Matrix w, const int8_t* q, int64_t q_stride,
-                                                         const float* scale, int batch, O* logits, int64_t stride) {
-    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (n >= w.out_dim) return;
-    const int lane = threadIdx.x & 31, words = w.in_dim >> 2;
-    const int8_t* wr = w.q + n * w.pitch;
-    for (int64_t b = blockIdx.y; b < batch; b += gridDim.y) {
-        const int8_t* xr = q + b * q_stride;
-        int acc = 0;
-        for (int i = lane; i < words; i += 32)
-            acc = __dp4a(reinterpret_cast<const int*>(wr)[i], reinterpret_cast<const int*>(xr)[i], acc);
-        for (int i = 4 * words + lane; i < w.in_dim; i += 32) acc += (int)wr[i] * (int)xr[i];
-        for (int s = 16; s > 0; s >>= 1) acc += __shfl_xor_sync(FULLMASK, acc, s);
-        if (lane == 0) logits[b * stride + n] = scaled<O>(acc, w.scale[n], scale[b]);
-    }
-}
-
 template <typename T, typename W>
 cudaError_t launch_norm(const NormI8Args& a, cudaStream_t stream) {
     const size_t smem = (size_t)a.dim * sizeof(T);
@@ -192,17 +168,6 @@ cudaError_t quantise_rows_i8(const void* src, int format, int64_t row_stride, co
         default:
             quantise_rows_kernel<<<grid, kNormThreads, 0, stream>>>(Q40Rows{(const uint8_t*)src, w.in_dim / 32}, w);
     }
-    return cudaGetLastError();
-}
-
-cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, const float* scale, int batch,
-                       void* logits, int dtype, int64_t logits_stride, cudaStream_t stream, int* launches) {
-    const dim3 grid((unsigned)((w.out_dim + 7) / 8), (unsigned)std::min(batch, 64));
-    if (dtype == VDXS_DTYPE_BF16)
-        unembed_i8_kernel<<<grid, 256, 0, stream>>>(w, q, q_stride, scale, batch, (__nv_bfloat16*)logits, logits_stride);
-    else
-        unembed_i8_kernel<<<grid, 256, 0, stream>>>(w, q, q_stride, scale, batch, (float*)logits, logits_stride);
-    ++*launches;
     return cudaGetLastError();
 }
 

@@ -1,0 +1,314 @@
+// vdxs_i8_product.cu - the 8-bit unembedding product on the integer tensor cores:
+//   logits[b][n] = scale[b] * w_scale[n] * sum_k q[b][k] * w[n][k].
+//
+// The vocabulary is the accumulator's row axis (128 rows a tile) and the batch its column
+// axis (16..256 columns): a decode batch of any size then reads the weights once, as the
+// A operand, and a tile's column leaves tensor memory with the 32 lanes of a warp on 32
+// neighbouring vocabulary entries, so the logits go out as whole 128-byte lines without a
+// stop in shared memory.
+//
+// One persistent CTA per SM, six warps: warp 0 copies 128-byte wide tiles of both operands
+// into a ring of stages (TMA, 128-byte swizzle), warp 1 issues the products, warps 2 to 5
+// scale and store one accumulator while the next tile is summed in the other one. Sums are
+// exact 32-bit integers; the two scales are applied in fp32.
+#include "vdxs_internal.h"
+#include "../../include/vdx_sampler.h"
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+namespace vdxs {
+namespace {
+
+constexpr int kThreadsP = 192;
+constexpr int kTileM = 128;          // vocabulary entries of a tile
+constexpr int kChunkK = 128;         // bytes of a row in a stage: one swizzle span
+constexpr int kMaxN = 256;           // batch columns of a tile
+constexpr int kMaxStages = 12;
+constexpr int kStageBytesA = kTileM * kChunkK;
+constexpr int kSmemBudget = 220 * 1024;
+constexpr int32_t kErrTimeout = 3;   // the context's device error word: a bounded wait gave up
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void bar_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done)
+                 : "r"(smem_addr(bar)), "r"(parity)
+                 : "memory");
+    return done != 0u;
+}
+// Waits for a phase, at most about two seconds (false: gave up).
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity) {
+    if (bar_try(bar, parity)) return true;
+    uint64_t t0, t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+    for (;;) {
+        for (int i = 0; i < 64; ++i)
+            if (bar_try(bar, parity)) return true;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+        if (t - t0 > 2000000000ull) return false;
+    }
+}
+
+__device__ __forceinline__ void copy_tile(const CUtensorMap* map, void* dst, int x, int y, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
+        : "memory");
+}
+
+// Shared-memory operand: rows of 128 bytes, 128-byte swizzle, 8 rows (1024 bytes) to a group.
+__device__ __forceinline__ uint64_t operand(const void* p) {
+    return (uint64_t)((smem_addr(p) & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void load16(uint32_t addr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr));
+}
+// The registers of a load pass through the wait, so that no use of them moves before it.
+__device__ __forceinline__ void wait16(uint32_t* v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::
+                     "memory");
+}
+
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+struct ProductParams {
+    int in_dim, out_dim, batch, n, n_tiles, stages, columns;
+    int64_t tiles;  // vocabulary tiles * n_tiles
+    const float *w_scale, *scale;
+    void* logits;
+    int64_t stride;
+    int32_t* err;
+};
+
+template <typename O>
+__global__ void __launch_bounds__(kThreadsP, 1)
+    unembed_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q,
+                      const ProductParams p) {
+    extern __shared__ unsigned char raw[];
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_base;
+    unsigned char* stages = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int stage_bytes = kStageBytesA + p.n * kChunkK;
+    const int chunks = (p.in_dim + kChunkK - 1) / kChunkK;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) bar_init(&full[i], 1), bar_init(&empty[i], 1);
+        for (int i = 0; i < 2; ++i) bar_init(&acc_full[i], 1), bar_init(&acc_empty[i], 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                     "r"(p.columns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_base;
+
+    bool good = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 0;
+            int issued = 0;  // stages with a copy that nobody has waited for, should a wait give up
+            for (int64_t t = blockIdx.x; good && t < p.tiles; t += gridDim.x) {
+                const int m = (int)(t / p.n_tiles), n = (int)(t - (int64_t)m * p.n_tiles);
+                for (int c = 0; c < chunks; ++c) {
+                    if (!(good = bar_wait(&empty[s], phase ^ 1))) break;
+                    unsigned char* a = stages + s * stage_bytes;
+                    bar_expect(&full[s], stage_bytes);
+                    copy_tile(&map_w, a, c * kChunkK, m * kTileM, &full[s]);
+                    copy_tile(&map_q, a + kStageBytesA, c * kChunkK, n * p.n, &full[s]);
+                    issued = min(issued + 1, p.stages);
+                    if (++s == p.stages) s = 0, phase ^= 1;
+                }
+            }
+            // The copies in flight land before the CTA may end.
+            if (!good)
+                for (; issued > 0; --issued) {
+                    if (--s < 0) s = p.stages - 1, phase ^= 1;
+                    bar_wait(&full[s], phase);
+                }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // D: 32-bit integers; A, B: signed 8 bits, K-major.
+            const uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(p.n >> 3) << 17 | (uint32_t)(kTileM >> 4) << 24;
+            int s = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            for (int64_t t = blockIdx.x; good && t < p.tiles; t += gridDim.x) {
+                if (!(good = bar_wait(&acc_empty[acc], acc_phase ^ 1))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t d = tmem + acc * (p.columns >> 1);
+                for (int c = 0; c < chunks; ++c) {
+                    if (!(good = bar_wait(&full[s], phase))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t a = operand(stages + s * stage_bytes);
+                    const uint64_t b = operand(stages + s * stage_bytes + kStageBytesA);
+                    // What lies behind in_dim is zero in shared memory; whole steps of it are left out.
+                    const int steps = min(4, (p.in_dim - c * kChunkK + 31) / 32);
+                    for (int k = 0; k < steps; ++k) mma_i8(d, a + 2 * k, b + 2 * k, idesc, c > 0 || k > 0);
+                    mma_commit(&empty[s]);
+                    if (++s == p.stages) s = 0, phase ^= 1;
+                }
+                if (!good) break;
+                mma_commit(&acc_full[acc]);
+                if (++acc == 2) acc = 0, acc_phase ^= 1;
+            }
+        }
+    } else {
+        const int quad = warp & 3;  // the tensor memory lanes that this warp may read
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
+            const int m = (int)(t / p.n_tiles), n = (int)(t - (int64_t)m * p.n_tiles);
+            const int64_t row = (int64_t)m * kTileM + quad * 32 + lane;
+            const bool have = row < p.out_dim;
+            const float ws = have ? __ldg(p.w_scale + row) : 0.0f;
+            if (!(good = __all_sync(0xFFFFFFFFu, bar_wait(&acc_full[acc], acc_phase)))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t src = tmem + acc * (p.columns >> 1) + ((uint32_t)quad * 32 << 16);
+            const int b0 = n * p.n;
+            O* out = static_cast<O*>(p.logits) + row;
+            for (int c = 0; c < p.n && b0 + c < p.batch; c += 16) {
+                uint32_t v[16];
+                load16(src + c, v);
+                const int bl = b0 + c + (lane & 15);
+                const float xs = bl < p.batch ? __ldg(p.scale + bl) : 0.0f;
+                wait16(v);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float x = __shfl_sync(0xFFFFFFFFu, xs, j);
+                    const int b = b0 + c + j;
+                    if (have && b < p.batch)
+                        put(out + b * p.stride, __fmul_rn(__fmul_rn((float)(int)v[j], ws), x));
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (lane == 0) bar_arrive(&acc_empty[acc]);
+            if (++acc == 2) acc = 0, acc_phase ^= 1;
+        }
+    }
+    if (!good) *p.err = kErrTimeout;
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 2)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.columns));
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return (EncodeTiled)p;
+    }();
+    return fn;
+}
+
+// Bytes [rows][pitch] of which `width` are used; boxes of 128 bytes by `box_rows` rows.
+cudaError_t make_map(CUtensorMap* map, const void* base, int width, int rows, int64_t pitch, int box_rows) {
+    const EncodeTiled encode = encoder();
+    if (!encode) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)pitch};
+    const cuuint32_t box[2] = {kChunkK, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, const float* scale, int batch,
+                       void* logits, int dtype, int64_t logits_stride, int32_t* err, int sm_count, cudaStream_t stream,
+                       int* launches) {
+    ProductParams p{};
+    p.in_dim = w.in_dim;
+    p.out_dim = w.out_dim;
+    p.batch = batch;
+    // Equal column tiles of at most 256, a multiple of 16 wide.
+    p.n_tiles = (batch + kMaxN - 1) / kMaxN;
+    p.n = ((batch + p.n_tiles - 1) / p.n_tiles + 15) / 16 * 16;
+    p.columns = 32;
+    while (p.columns < 2 * p.n) p.columns *= 2;
+    const int stage_bytes = kStageBytesA + p.n * kChunkK;
+    p.stages = std::min(kMaxStages, (kSmemBudget - 1024) / stage_bytes);
+    p.tiles = (int64_t)((w.out_dim + kTileM - 1) / kTileM) * p.n_tiles;
+    p.w_scale = w.scale;
+    p.scale = scale;
+    p.logits = logits;
+    p.stride = logits_stride;
+    p.err = err;
+    CUtensorMap map_w, map_q;
+    cudaError_t e;
+    if ((e = make_map(&map_w, w.q, w.in_dim, w.out_dim, w.pitch, kTileM)) != cudaSuccess ||
+        (e = make_map(&map_q, q, w.in_dim, batch, q_stride, p.n)) != cudaSuccess)
+        return e;
+    const int smem = p.stages * stage_bytes + 1024;
+    const int grid = (int)std::min<int64_t>(p.tiles, sm_count);
+    if (dtype == VDXS_DTYPE_BF16) {
+        if ((e = cudaFuncSetAttribute(unembed_i8_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      kSmemBudget)) != cudaSuccess)
+            return e;
+        unembed_i8_kernel<__nv_bfloat16><<<grid, kThreadsP, smem, stream>>>(map_w, map_q, p);
+    } else {
+        if ((e = cudaFuncSetAttribute(unembed_i8_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      kSmemBudget)) != cudaSuccess)
+            return e;
+        unembed_i8_kernel<float><<<grid, kThreadsP, smem, stream>>>(map_w, map_q, p);
+    }
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    ++*launches;
+    return cudaSuccess;
+}
+
+}  // namespace vdxs

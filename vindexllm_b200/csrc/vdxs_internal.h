@@ -144,7 +144,7 @@ cudaError_t q4_0_repack(const uint8_t* src, int in_dim, int out_dim, uint32_t* n
                         cudaStream_t stream);
 cudaError_t q4_0_matvec(const uint32_t* nib, const uint16_t* scales, int in_dim, int out_dim, const float* x,
                         int batch, float* out, cudaStream_t stream, int* launches);
-// Norm, residual and 8-bit output, and the 8-bit unembedding (vdxs_i8.cu).
+// Norm, residual and 8-bit output, and the 8-bit unembedding (vdxs_i8.cu, vdxs_i8_product.cu).
 struct NormI8Args {
     const void* x = nullptr;
     int64_t x_stride = 0;
@@ -171,7 +171,8 @@ cudaError_t rms_norm_i8(const NormI8Args& a, cudaStream_t stream);
 // Rows of fp32/bf16/fp16 (format 0..2) or Q4_0 blocks (4) to 8 bits with a scale per row.
 cudaError_t quantise_rows_i8(const void* src, int format, int64_t row_stride, const I8Matrix& w, cudaStream_t stream);
 cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, const float* scale, int batch,
-                       void* logits, int dtype, int64_t logits_stride, cudaStream_t stream, int* launches);
+                       void* logits, int dtype, int64_t logits_stride, int32_t* err, int sm_count, cudaStream_t stream,
+                       int* launches);
 // Beam search (vdxs_beam.cu).
 struct BeamWorkspace {
     unsigned long long* cand = nullptr;  // [rows][chunks][beams] each chunk's best (key, token), best first
