@@ -1395,6 +1395,7 @@ VDXS_API int32_t vdxs_i8_prepare(vdxs_context* ctx, const void* d_weights, int32
     m.pitch = ((int64_t)in_dim + 15) / 16 * 16;
     cudaError_t e = cudaMalloc((void**)&m.q, (size_t)out_dim * (size_t)m.pitch);
     if (e == cudaSuccess) e = cudaMalloc((void**)&m.scale, (size_t)out_dim * sizeof(float));
+    if (e == cudaSuccess) e = map_weights_i8(m);
     if (e == cudaSuccess) {
         if (format == VDXS_WEIGHTS_I8) {
             e = cudaMemcpy2DAsync(m.q, (size_t)m.pitch, d_weights, (size_t)row_stride, (size_t)in_dim, (size_t)out_dim,

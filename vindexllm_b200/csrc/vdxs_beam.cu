@@ -483,7 +483,8 @@ cudaError_t beam_select(const BeamArgs& a, cudaStream_t stream) {
     const int grid = a.batch * a.beams * a.chunks;
     void (*kern)(BeamArgs) =
         a.dtype == VDXS_DTYPE_BF16 ? beam_select_kernel<__nv_bfloat16> : beam_select_kernel<float>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemLimit limit[2];
+    cudaError_t e = limit[a.dtype == VDXS_DTYPE_BF16].raise(kern, smem);
     if (e != cudaSuccess) return e;
     kern<<<grid, kBThreads, smem, stream>>>(a);
     return cudaGetLastError();
@@ -492,8 +493,8 @@ cudaError_t beam_select(const BeamArgs& a, cudaStream_t stream) {
 cudaError_t beam_reorder(const BeamArgs& a, bool rings, const BeamCacheArgs* caches, int n_caches, cudaStream_t stream,
                          int* launches) {
     const size_t smem = (size_t)a.beams * kRThreads * 16;
-    cudaError_t e =
-        cudaFuncSetAttribute(beam_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static SmemLimit limit;
+    cudaError_t e = limit.raise(beam_reorder_kernel, smem);
     if (e != cudaSuccess) return e;
     int at = 0;
     while (rings || at < n_caches) {

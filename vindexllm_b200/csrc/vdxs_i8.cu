@@ -131,8 +131,8 @@ __global__ void __launch_bounds__(kNormThreads) quantise_rows_kernel(S src, I8Ma
 template <typename T, typename W>
 cudaError_t launch_norm(const NormI8Args& a, cudaStream_t stream) {
     const size_t smem = (size_t)a.dim * sizeof(T);
-    cudaError_t e = cudaFuncSetAttribute(rms_norm_i8_kernel<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
+    static SmemLimit limit;
+    cudaError_t e = limit.raise(rms_norm_i8_kernel<T, W>, smem);
     if (e != cudaSuccess) return e;
     rms_norm_i8_kernel<T, W><<<a.rows, kNormThreads, smem, stream>>>(a);
     return cudaGetLastError();

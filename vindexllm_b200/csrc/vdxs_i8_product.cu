@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstring>
 
 namespace vdxs {
 namespace {
@@ -289,26 +290,30 @@ cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, con
     p.stride = logits_stride;
     p.err = err;
     CUtensorMap map_w, map_q;
-    cudaError_t e;
-    if ((e = make_map(&map_w, w.q, w.in_dim, w.out_dim, w.pitch, kTileM)) != cudaSuccess ||
-        (e = make_map(&map_q, q, w.in_dim, batch, q_stride, p.n)) != cudaSuccess)
-        return e;
+    static_assert(sizeof(map_w) == sizeof(w.map), "tensor map size");
+    memcpy(&map_w, w.map, sizeof(map_w));
+    cudaError_t e = make_map(&map_q, q, w.in_dim, batch, q_stride, p.n);
+    if (e != cudaSuccess) return e;
     const int smem = p.stages * stage_bytes + 1024;
     const int grid = (int)std::min<int64_t>(p.tiles, sm_count);
+    static SmemLimit limit[2];
     if (dtype == VDXS_DTYPE_BF16) {
-        if ((e = cudaFuncSetAttribute(unembed_i8_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      kSmemBudget)) != cudaSuccess)
-            return e;
+        if ((e = limit[0].raise(unembed_i8_kernel<__nv_bfloat16>, kSmemBudget)) != cudaSuccess) return e;
         unembed_i8_kernel<__nv_bfloat16><<<grid, kThreadsP, smem, stream>>>(map_w, map_q, p);
     } else {
-        if ((e = cudaFuncSetAttribute(unembed_i8_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      kSmemBudget)) != cudaSuccess)
-            return e;
+        if ((e = limit[1].raise(unembed_i8_kernel<float>, kSmemBudget)) != cudaSuccess) return e;
         unembed_i8_kernel<float><<<grid, kThreadsP, smem, stream>>>(map_w, map_q, p);
     }
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     ++*launches;
     return cudaSuccess;
+}
+
+cudaError_t map_weights_i8(I8Matrix& w) {
+    CUtensorMap map;
+    const cudaError_t e = make_map(&map, w.q, w.in_dim, w.out_dim, w.pitch, kTileM);
+    if (e == cudaSuccess) memcpy(w.map, &map, sizeof(map));
+    return e;
 }
 
 }  // namespace vdxs

@@ -2,6 +2,7 @@
 // sm_100a kernels (vdxs_kernels.cu). Not part of the public ABI.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -166,6 +167,24 @@ struct I8Matrix {            // weights as the product reads them
     float* scale = nullptr;  // [out_dim]
     int in_dim = 0, out_dim = 0;
     int64_t pitch = 0;       // bytes between rows: in_dim rounded up to 16
+    alignas(64) unsigned char map[128] = {};  // tensor map of q (map_weights_i8)
+};
+// Makes w.map, once the other members are set.
+cudaError_t map_weights_i8(I8Matrix& w);
+// cudaFuncAttributeMaxDynamicSharedMemorySize of a kernel, raised once for each device.
+struct SmemLimit {
+    std::atomic<int> have[64] = {};
+    template <typename F>
+    cudaError_t raise(F* kernel, size_t bytes) {
+        if (bytes <= 48 * 1024) return cudaSuccess;
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev < 64 && have[dev].load(std::memory_order_relaxed) >= (int)bytes) return cudaSuccess;
+        e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess && dev < 64) have[dev].store((int)bytes, std::memory_order_relaxed);
+        return e;
+    }
 };
 cudaError_t rms_norm_i8(const NormI8Args& a, cudaStream_t stream);
 // Rows of fp32/bf16/fp16 (format 0..2) or Q4_0 blocks (4) to 8 bits with a scale per row.

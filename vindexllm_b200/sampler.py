@@ -41,44 +41,65 @@ def _dptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
+def _ptr(t):
+    """Address of a tensor, as ctypes takes it for a pointer argument (0 is NULL)."""
+    return 0 if t is None else t.data_ptr()
+
+
+_HIDDEN_CODES: dict = {}
+
+
 def _hidden_code(t, what: str) -> int:
     """VDXS_DTYPE_* of a hidden state or norm weight."""
-    import torch
-    codes = {torch.float32: abi.DTYPE_F32, torch.bfloat16: abi.DTYPE_BF16, torch.float16: abi.DTYPE_F16}
-    if t.dtype not in codes:
+    if not _HIDDEN_CODES:
+        import torch
+        _HIDDEN_CODES.update({torch.float32: abi.DTYPE_F32, torch.bfloat16: abi.DTYPE_BF16,
+                              torch.float16: abi.DTYPE_F16})
+    code = _HIDDEN_CODES.get(t.dtype)
+    if code is None:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
-    return codes[t.dtype]
+    return code
 
 
-def _on(device: int, stream):
-    """(stream, context manager): the stream of a call on `device` (its current one when
-    None), under which the call's outputs are allocated, so that their memory is reused in
-    that stream's order."""
+def _stream_on(device: int, stream) -> int:
+    """The stream of a call on `device`: the given one, or the device's current one."""
+    import torch
+    return (torch.cuda.current_stream(device) if stream is None else stream).cuda_stream
+
+
+def _empty(shape, dtype, device, stream):
+    """An output. With a stream of the caller's it is allocated under that one, so that its memory
+    is reused in that stream's order."""
     import torch
     if stream is None:
-        stream = torch.cuda.current_stream(device)
-    return stream, torch.cuda.stream(stream)
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _need(t, what: str, device: int, dtype=None, shape=None, rows=False):
     """Argument check of a device tensor: its device, type and shape; contiguous, or with
     `rows` a matrix whose rows are contiguous."""
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         raise ValueError(f"{what} must be a tensor on cuda:{device}, got {t.device}")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if rows and (t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1)):
+    if not t.is_contiguous():
+        if not rows:
+            raise ValueError(f"{what} must be contiguous")
+        if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+            raise ValueError(f"{what} must be a matrix with contiguous rows")
+    elif rows and t.dim() != 2:
         raise ValueError(f"{what} must be a matrix with contiguous rows")
-    if not rows and not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous")
     return t
 
 
 def _pitch(t) -> int:
     """Elements between the rows of a matrix (a lone row's stride says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    rows, width = t.shape
+    return t.stride(0) if rows > 1 else max(t.stride(0), width)
 
 
 class SamplerContext:
@@ -165,29 +186,34 @@ class SamplerContext:
         ``x`` or ``residual`` for an update in place. A ``q`` made here has rows padded to a
         multiple of 16 bytes, as ``I8Weights.unembed`` takes it."""
         import torch
-        code = _hidden_code(x, "x")
-        _need(x, "x", self.device, rows=True)
-        rows, dim = x.shape
-        wcode = _hidden_code(weight, "weight")
-        _need(weight, "weight", self.device, shape=(dim,))
+        dev, code, wcode = self.device, _hidden_code(x, "x"), _hidden_code(weight, "weight")
+        _need(x, "x", dev, rows=True)
+        shape = x.shape
+        rows, dim = shape
+        _need(weight, "weight", dev, None, (dim,))
         if residual is not None:
-            _need(residual, "residual", self.device, x.dtype, x.shape, rows=True)
-        stream, on = _on(self.device, stream)
-        with on:
-            if out_hidden is None and residual is not None:
-                out_hidden = torch.empty(rows, dim, dtype=x.dtype, device=x.device)
-            if q is None:
-                q = torch.empty(rows, -(-dim // 16) * 16, dtype=torch.int8, device=x.device)[:, :dim]
-            if scale is None:
-                scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+            _need(residual, "residual", dev, x.dtype, shape, True)
+            if out_hidden is None:
+                out_hidden = _empty(shape, x.dtype, x.device, stream)
         if out_hidden is not None:
-            _need(out_hidden, "out_hidden", self.device, x.dtype, x.shape, rows=True)
-        _need(q, "q", self.device, torch.int8, x.shape, rows=True)
-        _need(scale, "scale", self.device, torch.float32, (rows,))
-        check(self.lib.vdxs_rms_norm_i8(self._h, _dptr(x), _pitch(x), _dptr(residual),
-                                        0 if residual is None else _pitch(residual), code, _dptr(weight), wcode, rows,
-                                        dim, eps, _dptr(out_hidden), 0 if out_hidden is None else _pitch(out_hidden),
-                                        _dptr(q), _pitch(q), _dptr(scale), _stream_ptr(stream)), self._h)
+            _need(out_hidden, "out_hidden", dev, x.dtype, shape, True)
+        if q is None:
+            room = -(-dim // 16) * 16
+            q = _empty((rows, room), torch.int8, x.device, stream)
+            if room != dim:
+                q = q[:, :dim]
+        else:
+            _need(q, "q", dev, torch.int8, shape, True)
+        if scale is None:
+            scale = _empty(rows, torch.float32, x.device, stream)
+        else:
+            _need(scale, "scale", dev, torch.float32, (rows,))
+        rc = self.lib.vdxs_rms_norm_i8(self._h, _ptr(x), _pitch(x), _ptr(residual),
+                                       0 if residual is None else _pitch(residual), code, _ptr(weight), wcode, rows, dim,
+                                       eps, _ptr(out_hidden), 0 if out_hidden is None else _pitch(out_hidden), _ptr(q),
+                                       _pitch(q), _ptr(scale), _stream_on(dev, stream))
+        if rc:
+            check(rc, self._h)
         return q, scale, out_hidden
 
     def sample_host(self, cfg: VdxsConfig, logits: np.ndarray, uniforms=None, history=None,
@@ -518,10 +544,9 @@ class I8Weights:
     def _prepare(self, ctx, weight, fmt, scales, stride, in_dim, out_dim, stream):
         self.ctx, self.lib = ctx, ctx.lib
         self.in_dim, self.out_dim = in_dim, out_dim
-        stream, _ = _on(ctx.device, stream)
         h = C.c_void_p()
-        check(self.lib.vdxs_i8_prepare(ctx.handle, _dptr(weight), fmt, _dptr(scales), stride, in_dim, out_dim,
-                                       _stream_ptr(stream), C.byref(h)), ctx.handle)
+        check(self.lib.vdxs_i8_prepare(ctx.handle, _ptr(weight), fmt, _ptr(scales), stride, in_dim, out_dim,
+                                       _stream_on(ctx.device, stream), C.byref(h)), ctx.handle)
         self._h = h
 
     def close(self):
@@ -540,17 +565,22 @@ class I8Weights:
         ``scale`` [batch], as SamplerContext.rms_norm_i8 returns them."""
         import torch
         dev = self.ctx.device
-        _need(q, "q", dev, torch.int8, (q.shape[0], self.in_dim), rows=True)
-        _need(scale, "scale", dev, torch.float32, (q.shape[0],))
-        stream, on = _on(dev, stream)
+        _need(q, "q", dev, torch.int8, None, True)
+        batch, width = q.shape
+        if width != self.in_dim:
+            raise ValueError(f"q must have {self.in_dim} columns, got {width}")
+        _need(scale, "scale", dev, torch.float32, (batch,))
         if logits is None:
-            with on:
-                logits = torch.empty(q.shape[0], self.out_dim, dtype=dtype or torch.float32, device=q.device)
-        _need(logits, "logits", dev, dtype, (q.shape[0], self.out_dim), rows=True)
-        pitch = q.stride(0) if q.shape[0] > 1 else -(-self.in_dim // 16) * 16
-        check(self.lib.vdxs_unembed_i8(self.ctx.handle, self._h, _dptr(q), pitch, _dptr(scale), q.shape[0],
-                                       _dptr(logits), _dtype_code(logits), _pitch(logits), _stream_ptr(stream)),
-              self.ctx.handle)
+            logits = _empty((batch, self.out_dim), dtype or torch.float32, q.device, stream)
+            pitch = self.out_dim
+        else:
+            _need(logits, "logits", dev, dtype, (batch, self.out_dim), True)
+            pitch = _pitch(logits)
+        rc = self.lib.vdxs_unembed_i8(self.ctx._h, self._h, _ptr(q),
+                                      q.stride(0) if batch > 1 else -(-width // 16) * 16, _ptr(scale), batch,
+                                      _ptr(logits), _dtype_code(logits), pitch, _stream_on(dev, stream))
+        if rc:
+            check(rc, self.ctx._h)
         return logits
 
     def sample(self, cfg: VdxsConfig, x, norm_weight, eps: float = 1e-6, residual=None, out_hidden=None, uniforms=None,
@@ -559,23 +589,29 @@ class I8Weights:
         import torch
         dev = self.ctx.device
         code, wcode = _hidden_code(x, "x"), _hidden_code(norm_weight, "norm_weight")
-        _need(x, "x", dev, shape=(x.shape[0], self.in_dim), rows=True)
-        _need(norm_weight, "norm_weight", dev, shape=(self.in_dim,))
+        _need(x, "x", dev, None, (x.shape[0], self.in_dim), True)
+        _need(norm_weight, "norm_weight", dev, None, (self.in_dim,))
         for t, what in ((residual, "residual"), (out_hidden, "out_hidden")):
             if t is not None:
-                _need(t, what, dev, x.dtype, x.shape, rows=True)
-        B = x.shape[0]
-        stream, on = _on(dev, stream)
+                _need(t, what, dev, x.dtype, x.shape, True)
+        batch = x.shape[0]
         if tokens is None:
-            with on:
-                tokens = torch.empty(B, dtype=torch.int32, device=x.device)
-        hs = history.shape[1] if history is not None else 1
-        check(self.lib.vdxs_sample_unembed_i8(self.ctx.handle, C.byref(cfg), self._h, _dptr(x), _pitch(x),
-                                              _dptr(residual), 0 if residual is None else _pitch(residual), code,
-                                              _dptr(norm_weight), wcode, eps, _dptr(out_hidden),
-                                              0 if out_hidden is None else _pitch(out_hidden), B, _dptr(history), hs,
-                                              _dptr(history_count), _dptr(uniforms), _dptr(tokens),
-                                              _stream_ptr(stream)), self.ctx.handle)
+            tokens = _empty(batch, torch.int32, x.device, stream)
+        for t, what, dtype, shape in ((uniforms, "uniforms", torch.float32, (batch,)),
+                                      (history_count, "history_count", torch.int32, (batch,)),
+                                      (tokens, "tokens", torch.int32, (batch,))):
+            if t is not None:
+                _need(t, what, dev, dtype, shape)
+        hs = 1
+        if history is not None:
+            _need(history, "history", dev, torch.int32, (batch, history.shape[1]))
+            hs = history.shape[1]
+        check(self.lib.vdxs_sample_unembed_i8(self.ctx._h, C.byref(cfg), self._h, _ptr(x), _pitch(x), _ptr(residual),
+                                              0 if residual is None else _pitch(residual), code, _ptr(norm_weight),
+                                              wcode, eps, _ptr(out_hidden),
+                                              0 if out_hidden is None else _pitch(out_hidden), batch, _ptr(history), hs,
+                                              _ptr(history_count), _ptr(uniforms), _ptr(tokens),
+                                              _stream_on(dev, stream)), self.ctx._h)
         return tokens
 
 
@@ -588,14 +624,17 @@ class BeamState:
                  hist=None, pos=None, count=None):
         import torch
         if device is None:
-            device = scores.device if scores is not None else torch.device("cuda", torch.cuda.current_device())
+            device = scores.device if scores is not None else torch.cuda.current_device()
+        device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         rows = batch * beams
         self.batch, self.beams, self.window = batch, beams, window
 
         def own(t, dtype, *shape):
             if t is None:
                 return torch.zeros(shape, dtype=dtype, device=device)
-            return _need(t, "state", t.device.index if t.is_cuda else -1, dtype, shape)
+            return _need(t, "state", device.index, dtype, shape)
 
         if scores is None:
             scores = torch.full((batch, beams), -float("inf"), dtype=torch.float32, device=device)
@@ -609,28 +648,33 @@ class BeamState:
         self.count = own(count, torch.int32, rows) if window else None
 
     def rows(self) -> abi.VdxsBeamRows:
-        def p(t):
-            return None if t is None else t.data_ptr()
-        return abi.VdxsBeamRows(p(self.scores), p(self.lengths), p(self.finished), p(self.hist), p(self.pos),
-                                p(self.count))
+        if not self.window:
+            return abi.VdxsBeamRows(self.scores.data_ptr(), self.lengths.data_ptr(), self.finished.data_ptr())
+        return abi.VdxsBeamRows(self.scores.data_ptr(), self.lengths.data_ptr(), self.finished.data_ptr(),
+                                self.hist.data_ptr(), self.pos.data_ptr(), self.count.data_ptr())
 
 
 def _cache_pieces(t, what: str, most: int | None = None):
     """(row stride, segment stride, segment bytes, segments) of a tensor [rows, ...] whose rows are
     one contiguous piece, or equal pieces (of at most `most` bytes) at one distance."""
-    size, inner = t.element_size(), 1
-    dims = [(n, s) for n, s in zip(t.shape[1:], t.stride()[1:]) if n != 1]
-    while dims and dims[-1][1] == inner and (most is None or inner * size < most):
-        inner *= dims.pop()[0]
-    count, step = 1, inner
-    while dims:
-        n, s = dims.pop()
+    size, shape, stride = t.element_size(), t.shape, t.stride()
+    inner = count = 1
+    d = len(shape) - 1
+    while d > 0 and (shape[d] == 1 or (stride[d] == inner and (most is None or inner * size < most))):
+        inner *= shape[d]
+        d -= 1
+    step = inner
+    while d > 0:
+        n, s = shape[d], stride[d]
+        d -= 1
+        if n == 1:
+            continue
         if count == 1:
             step = s
         elif s != step * count:
-            raise ValueError(f"{what}: the rows of strides {t.stride()} are not equal pieces at one distance")
+            raise ValueError(f"{what}: the rows of strides {stride} are not equal pieces at one distance")
         count *= n
-    row = t.stride(0) if t.shape[0] > 1 else step * count
+    row = stride[0] if shape[0] > 1 else step * count
     return row * size, step * size, inner * size, count
 
 
@@ -661,19 +705,24 @@ class BeamSearch:
         """A cache is a tensor [rows, ...] (in place) or a pair (source, target) of them; a view
         of the filled part moves that part alone."""
         n = len(caches)
-        out = (abi.VdxsBeamCache * max(n, 1))()
+        if not n:
+            return None, 0
+        out = (abi.VdxsBeamCache * n)()
+        dev, rows = self.ctx.device, self.batch * self.beams
         for i, c in enumerate(caches):
             src, dst = c if isinstance(c, (tuple, list)) else (c, c)
             for t in (src, dst):
-                if not t.is_cuda or t.device.index != self.ctx.device:
-                    raise ValueError(f"cache {i} must be on cuda:{self.ctx.device}, got {t.device}")
-                if t.dim() < 1 or t.shape[0] != self.batch * self.beams:
-                    raise ValueError(f"cache {i} must have {self.batch * self.beams} rows, got shape {tuple(t.shape)}")
-            if src.shape != dst.shape or src.dtype != dst.dtype:
+                if t.get_device() != dev:
+                    raise ValueError(f"cache {i} must be on cuda:{dev}, got {t.device}")
+                if t.dim() < 1 or t.shape[0] != rows:
+                    raise ValueError(f"cache {i} must have {rows} rows, got shape {tuple(t.shape)}")
+            if src is not dst and (src.shape != dst.shape or src.dtype != dst.dtype):
                 raise ValueError(f"cache {i}: source and target differ in shape or type")
             if src.numel() == 0:
                 continue  # a zeroed entry has no bytes to move
-            a, b = _cache_pieces(src, f"cache {i}"), _cache_pieces(dst, f"cache {i}")
+            a = b = _cache_pieces(src, f"cache {i}")
+            if src is not dst:
+                b = _cache_pieces(dst, f"cache {i}")
             if a[2] != b[2]:  # the smaller pieces of the two
                 a, b = (_cache_pieces(t, f"cache {i}", min(a[2], b[2])) for t in (src, dst))
             if a[2:] != b[2:]:
@@ -686,38 +735,42 @@ class BeamSearch:
         """One step (vdxs_beam_step): (tokens, parents) as int32 [batch, beams]. ``out`` receives the
         rows after it (``state`` itself, in place, when None)."""
         import torch
-        dev, rows = self.ctx.device, self.batch * self.beams
+        dev, rows, shape = self.ctx.device, self.batch * self.beams, (self.batch, self.beams)
         out = state if out is None else out
-        _need(logits, "logits", dev, shape=(rows, self.vocab), rows=True)
+        _need(logits, "logits", dev, None, (rows, self.vocab), True)
         for s in (state, out):
-            if (s.batch, s.beams, s.window) != (self.batch, self.beams, state.window):
+            if s.batch != self.batch or s.beams != self.beams or s.window != state.window:
                 raise ValueError(f"a state of {s.batch} x {s.beams}, window {s.window}, for a search of {self.batch} x "
                                  f"{self.beams}, window {state.window}")
-            if s.scores.device.index != dev:
+            if s.scores.get_device() != dev:
                 raise ValueError(f"the state is on {s.scores.device}, the search on cuda:{dev}")
+        n_stop = 0
         if stop_ids is not None:
             _need(stop_ids, "stop_ids", dev, torch.int32)
-        stream, on = _on(dev, stream)
-        with on:
-            if tokens is None:
-                tokens = torch.empty(self.batch, self.beams, dtype=torch.int32, device=logits.device)
-            if parents is None:
-                parents = torch.empty(self.batch, self.beams, dtype=torch.int32, device=logits.device)
-        _need(tokens, "tokens", dev, torch.int32, (self.batch, self.beams))
-        _need(parents, "parents", dev, torch.int32, (self.batch, self.beams))
+            n_stop = stop_ids.numel()
+        if tokens is None:
+            tokens = _empty(shape, torch.int32, logits.device, stream)
+        else:
+            _need(tokens, "tokens", dev, torch.int32, shape)
+        if parents is None:
+            parents = _empty(shape, torch.int32, logits.device, stream)
+        else:
+            _need(parents, "parents", dev, torch.int32, shape)
         cfg = abi.VdxsBeamConfig(length_alpha, repeat_penalty, state.window, pad_token, 0)
-        a, b = state.rows(), out.rows()
+        a = state.rows()
+        b = a if out is state else out.rows()
         moved, n = self._caches(caches)
-        check(self.lib.vdxs_beam_step(self._h, C.byref(cfg), _dptr(logits), _dtype_code(logits), _pitch(logits),
-                                      C.byref(a), C.byref(b), _dptr(stop_ids),
-                                      0 if stop_ids is None else int(stop_ids.numel()), moved, n, _dptr(tokens),
-                                      _dptr(parents), _stream_ptr(stream)), self.ctx.handle)
+        rc = self.lib.vdxs_beam_step(self._h, C.byref(cfg), _ptr(logits), _dtype_code(logits), _pitch(logits), C.byref(a),
+                                     C.byref(b), _ptr(stop_ids), n_stop, moved, n, _ptr(tokens), _ptr(parents),
+                                     _stream_on(dev, stream))
+        if rc:
+            check(rc, self.ctx._h)
         return tokens, parents
 
     def reorder(self, parents, caches, stream=None):
         """Moves caches by a step's parents (vdxs_beam_reorder)."""
         import torch
         _need(parents, "parents", self.ctx.device, torch.int32, (self.batch, self.beams))
-        stream, _ = _on(self.ctx.device, stream)
         moved, n = self._caches(caches)
-        check(self.lib.vdxs_beam_reorder(self._h, _dptr(parents), moved, n, _stream_ptr(stream)), self.ctx.handle)
+        check(self.lib.vdxs_beam_reorder(self._h, _ptr(parents), moved, n, _stream_on(self.ctx.device, stream)),
+              self.ctx._h)
