@@ -528,7 +528,7 @@ typedef struct vdxs_beam_cache {
 } vdxs_beam_cache;
 
 /* A search of `batch` prompts with `beams` beams each (1..VDXS_BEAM_MAX_BEAMS; batch *
- * beams <= 65535) over `vocab` tokens. It owns a fixed workspace, so a step allocates nothing and
+ * beams <= 65535) over `vocab` tokens (at most 8000000). It owns a fixed workspace, so a step allocates nothing and
  * may be captured at once; steps of one search that overlap on the GPU race, so give each
  * stream or graph that runs beside another its own. Destroy it before its context. */
 VDXS_API int32_t vdxs_beam_create(vdxs_context* ctx, int32_t batch, int32_t beams, int32_t vocab,

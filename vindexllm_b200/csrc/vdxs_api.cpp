@@ -1607,7 +1607,8 @@ VDXS_API int32_t vdxs_beam_create(vdxs_context* ctx, int32_t batch, int32_t beam
         return fail(ctx, VDXS_E_UNSUPPORTED, "beams %d exceeds %d", beams, VDXS_BEAM_MAX_BEAMS);
     if ((int64_t)batch * beams > 65535)
         return fail(ctx, VDXS_E_UNSUPPORTED, "batch * beams %lld exceeds 65535", (long long)batch * beams);
-    if (vocab > (1 << 24)) return fail(ctx, VDXS_E_UNSUPPORTED, "vocab %d exceeds %d", vocab, 1 << 24);
+    if (vocab > kBeamMaxVocab)
+        return fail(ctx, VDXS_E_UNSUPPORTED, "vocab %d exceeds %d", vocab, kBeamMaxVocab);
     DeviceGuard g(ctx->device);
     auto* b = new (std::nothrow) vdxs_beam();
     if (!b) return fail(ctx, VDXS_E_NO_MEMORY, "out of host memory");
@@ -1717,7 +1718,7 @@ VDXS_API int32_t vdxs_beam_step(vdxs_beam* b, const vdxs_beam_config* cfg, const
     const cudaStream_t st = (cudaStream_t)stream;
     int launches = 1;
     cudaError_t e = beam_select(a, st);
-    if (e == cudaSuccess) e = beam_reorder(a, a.window > 0, moved, n_caches, st, &launches);
+    if (e == cudaSuccess) e = beam_reorder(a, true, moved, n_caches, st, &launches);
     delete[] moved;
     ctx->launches += launches;
     if (e != cudaSuccess) return cuda_fail(ctx, e, "beam step launch");

@@ -2,12 +2,12 @@
 // the search's rows by the selected parents (rings and the caller's caches).
 //
 // One pass over the logits. A row is cut into chunks, a CTA takes one: each thread keeps a
-// running maximum and a sum of exponentials relative to it, and the CTA keeps a list of the
-// elements that can still be among its K = beams largest. The K-th largest of the threads'
-// maxima over the chunk's first tile is a lower bound of the chunk's K-th largest element,
-// so from then on only elements above it enter the list. The last CTA of a row merges the
-// row's lists and sums, the last row of a prompt merges the beams' offers; both are found
-// by counters that reset themselves.
+// running maximum with a sum of exponentials relative to it, and notes the maximum of its 16
+// elements of every tile. The K-th largest of disjoint groups' maxima is a lower bound of the
+// chunk's K-th largest element (K = beams), and only the groups whose maximum reaches the
+// bound, hardly more than K of them, are read again for their elements. The last CTA of a row
+// merges the row's lists and sums, the last row of a prompt merges the beams' offers; both are
+// found by counters that reset themselves.
 #include "vdxs_internal.h"
 #include "../../include/vdx_sampler.h"
 
@@ -23,10 +23,15 @@ namespace {
 
 constexpr unsigned FULLMASK = 0xFFFFFFFFu;
 constexpr int kBThreads = 256;
-constexpr int kPer = 16;                    // elements of a tile per thread
-constexpr int kTile = kBThreads * kPer;     // 4096
-constexpr int kListLimit = 512;             // entries before a list is cut back to K
+constexpr int kBWarps = kBThreads / 32;
+constexpr int kPer = 16;                      // elements of a tile per thread
+constexpr int kTile = kBThreads * kPer;       // 4096
+constexpr int kVecs = 4;                      // 16-byte loads per thread that are in flight together
+constexpr int kListLimit = 512;               // entries before a list is cut back to K
 constexpr int kListCap = kTile + kListLimit;  // a tile may add every element it has
+constexpr int kMaxTiles = 32;                 // tiles of a chunk
+constexpr int kGroups = kBThreads;            // groups that may be read again
+constexpr int kStopsKept = 64;                // stop ids in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 typedef unsigned long long u64;
 
@@ -41,6 +46,11 @@ __device__ __forceinline__ float key_value(u64 k) {
     return __uint_as_float((u >> 31) ? u ^ 0x80000000u : ~u);
 }
 __device__ __forceinline__ int key_token(u64 k) { return (int)~(uint32_t)k; }
+// The order of doubles without NaN as that of whole numbers.
+__device__ __forceinline__ u64 order_of(double v) {
+    const u64 u = (u64)__double_as_longlong(v + 0.0);
+    return u ^ ((u >> 63) ? ~0ull : 1ull << 63);
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -53,37 +63,56 @@ struct SelectShared {
     u64 best[VDXS_BEAM_MAX_BEAMS];
     u64 maxima[kBThreads];
     u64 bound;
-    int count;
+    int count, extra;
     int flag;
-    float wm[kBThreads / 32];
-    double ws[kBThreads / 32];
+    float fbound;
+    float wm[kBWarps];
+    double ws[kBWarps];
+    // The prompt's rows before the step, and what becomes of them.
+    float score[VDXS_BEAM_MAX_BEAMS];
+    int done[VDXS_BEAM_MAX_BEAMS], old[VDXS_BEAM_MAX_BEAMS];
+    int stop[kStopsKept];
+    double lse[VDXS_BEAM_MAX_BEAMS], size[VDXS_BEAM_MAX_BEAMS];
+    int parent[VDXS_BEAM_MAX_BEAMS], place[VDXS_BEAM_MAX_BEAMS];
+    unsigned short group[kGroups];
 };
+static_assert(kMaxTiles * kBThreads * sizeof(float) <= sizeof(u64) * kListCap, "the groups' maxima lie in the list");
+static_assert(kGroups * kPer <= kListCap, "a list holds the groups' elements");
 
-// The K-th largest of one value per thread (ties by thread), in sh.bound.
-__device__ __forceinline__ void block_bound(SelectShared& sh, u64 mine, int K) {
-    const int tid = threadIdx.x;
-    sh.maxima[tid] = mine;
-    __syncthreads();
+// How many of the n (a multiple of 4) values at p are above mine, or equal to it at a lower
+// place.
+__device__ __forceinline__ int count_above(const float* p, int n, float mine, int place) {
     int above = 0;
-    for (int j = 0; j < kBThreads; ++j) {
-        const u64 o = sh.maxima[j];
-        above += o > mine || (o == mine && j < tid);
+#pragma unroll 4
+    for (int j = 0; j < n; j += 4) {
+        const float4 o = *reinterpret_cast<const float4*>(p + j);
+        above += (o.x > mine || (o.x == mine && j < place)) + (o.y > mine || (o.y == mine && j + 1 < place)) +
+                 (o.z > mine || (o.z == mine && j + 2 < place)) + (o.w > mine || (o.w == mine && j + 3 < place));
     }
-    if (above == K - 1) sh.bound = mine;
-    __syncthreads();
+    return above;
 }
 
 // Cuts list[0..count) to its K largest, in order, in best[]; the rest of best is 0.
 // While the list is long, each thread takes the maximum of its share: the K-th largest of
 // those is a lower bound of the K-th largest entry, and at most a quarter plus K remain.
-__device__ void block_select(SelectShared& sh, int K) {
+// Then every entry counts the ones above it.
+__device__ __noinline__ void block_select(SelectShared& sh, int K) {
     const int tid = threadIdx.x;
     __syncthreads();
     int n = sh.count;
     while (n > kListLimit) {
         u64 mx = 0;
         for (int i = tid; i < n; i += kBThreads) mx = max(mx, sh.list[i]);
-        block_bound(sh, mx, K);
+        sh.maxima[tid] = mx;
+        __syncthreads();
+        int above = 0;
+#pragma unroll 8
+        for (int j = 0; j < kBThreads; ++j) {
+            const u64 o = sh.maxima[j];
+            above += o > mx || (o == mx && j < tid);
+        }
+        if (above == K - 1) sh.bound = mx;
+        __syncthreads();
         const u64 bound = sh.bound;
         u64 mine[kListCap / kBThreads];
         int m = 0;
@@ -103,11 +132,16 @@ __device__ void block_select(SelectShared& sh, int K) {
         n = sh.count;
     }
     if (tid < K) sh.best[tid] = 0;
+    if (tid == 0) sh.list[n] = 0;  // an even number of entries
     __syncthreads();
     for (int i = tid; i < n; i += kBThreads) {
         const u64 mine = sh.list[i];
         int above = 0;
-        for (int j = 0; j < n; ++j) above += sh.list[j] > mine;
+#pragma unroll 4
+        for (int j = 0; j < n; j += 2) {
+            const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(sh.list + j);
+            above += (o.x > mine) + (o.y > mine);
+        }
         if (above < K) sh.best[above] = mine;
     }
     __syncthreads();
@@ -118,259 +152,410 @@ struct Vec;  // 16 bytes of logits
 template <>
 struct Vec<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ void load(const float* p, float* v) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(p));
-        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-    }
+    static constexpr uint32_t kLowest = 0xFF800000u;  // -infinity
     static __device__ __forceinline__ float one(const float* p) { return __ldg(p); }
+    static __device__ __forceinline__ float at(const uint4* v, int i) {
+        const uint4 w = v[i / 4];
+        return __uint_as_float(i % 4 == 0 ? w.x : i % 4 == 1 ? w.y : i % 4 == 2 ? w.z : w.w);
+    }
+    // A vector of which only the elements [lo, hi) may be read.
+    static __device__ uint4 edge(const float* p, int e, int lo, int hi) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = e + i >= lo && e + i < hi ? __float_as_uint(__ldg(p + e + i)) : kLowest;
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
 };
 template <>
 struct Vec<__nv_bfloat16> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void load(const __nv_bfloat16* p, float* v) {
-        const uint4 f = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+    static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ float at(const uint4* v, int i) {
+        const uint4 q = v[i / 8];
+        const int j = (i % 8) / 2;
+        const uint32_t w = j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w;
+        return __uint_as_float(i % 2 ? w & 0xFFFF0000u : w << 16);
+    }
+    static __device__ uint4 edge(const __nv_bfloat16* p, int e, int lo, int hi) {
+        const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+        uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            const int a = e + 2 * i;
+            const uint32_t x = a >= lo && a < hi ? __ldg(s + a) : 0xFF80u;
+            const uint32_t y = a + 1 >= lo && a + 1 < hi ? __ldg(s + a + 1) : 0xFF80u;
+            w[i] = x | y << 16;
         }
+        return make_uint4(w[0], w[1], w[2], w[3]);
     }
-    static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 };
 
-// x > 0: x / p, else x * p, once for every time the ring holds the token (Sampler.pas:285-303).
-__device__ float penalised(float x, int token, const int32_t* ring, int n, float p) {
-    for (int i = 0; i < n; ++i)
-        if (ring[i] == token) x = x > 0.0f ? __fdiv_rn(x, p) : __fmul_rn(x, p);
-    return x;
+// Two fp32 values in one register pair, for the packed operations of sm_100.
+__device__ __forceinline__ u64 pack2(float lo, float hi) {
+    u64 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void unpack2(u64 v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+    u64 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+    u64 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 
-// The prompt's offers: each row's best[] is in order, so K times the best head is taken.
-// Lane l holds the heads of beams l and l + 32. One warp.
-__device__ void select_prompt(const BeamArgs& p, int prompt) {
-    __shared__ double s_score[VDXS_BEAM_MAX_BEAMS], s_size[VDXS_BEAM_MAX_BEAMS];
-    __shared__ int s_len[VDXS_BEAM_MAX_BEAMS], s_done[VDXS_BEAM_MAX_BEAMS], s_old[VDXS_BEAM_MAX_BEAMS];
-    __shared__ double o_score[VDXS_BEAM_MAX_BEAMS];
-    __shared__ int o_token[VDXS_BEAM_MAX_BEAMS], o_parent[VDXS_BEAM_MAX_BEAMS];
-    const int lane = threadIdx.x & 31, K = p.beams;
-    const int64_t row0 = (int64_t)prompt * K;
-    for (int b = lane; b < K; b += 32) {
-        const int64_t r = row0 + b;
-        const int done = p.finished_in[r] != 0, len = p.lengths_in[r];
-        s_score[b] = p.scores_in[r];
-        s_done[b] = done;
-        s_old[b] = len;
-        s_len[b] = done ? len : len + 1;
-        s_size[b] = pow((double)max(s_len[b], 1), p.alpha);
+// One vector of a chunk; what lies outside [lo, hi) is -infinity.
+template <typename T>
+__device__ __forceinline__ uint4 load_vector(const T* base, int e, int lo, int hi) {
+    return e >= lo && e + Vec<T>::N <= hi ? __ldg(reinterpret_cast<const uint4*>(base + e))
+                                          : Vec<T>::edge(base, e, lo, hi);
+}
+
+// The elements of a vector that can be among the K largest enter the list.
+template <typename T>
+__device__ __forceinline__ void enter(SelectShared& sh, const T* base, const uint32_t* marks, int e, int lo, int hi,
+                                      float tau, bool equal, int shift) {
+    const uint4 raw = load_vector(base, e, lo, hi);
+    const uint32_t out = marks && e < hi ? marks[e >> 5] >> (e & 31) : 0u;
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) {
+        const float v = Vec<T>::at(&raw, i);
+        if ((equal ? v >= tau : v > tau) && v > -INFINITY && !(out >> i & 1))
+            sh.list[atomicAdd(&sh.count, 1)] = make_key(v, e + i + shift);
     }
-    __syncwarp();
-    int at[2] = {0, 0};
-    double score[2], rank[2];
-    int token[2];
-    auto head = [&](int j) {
-        const int b = lane + 32 * j;
-        rank[j] = -INFINITY;
-        if (b >= K || at[j] >= K) return;
-        const double before = s_score[b];
-        if (s_done[b]) {
-            if (at[j] > 0) return;
-            score[j] = before;
-            token[j] = p.pad;
+}
+
+// Where many groups reach the bound (equal logits): the chunk tile by tile, the list cut to
+// its K largest whenever it is long. From the first cut on the K entries have lower
+// tokens than what follows, so an element equal to the K-th stays out.
+template <typename T>
+__device__ __noinline__ void select_slow(SelectShared& sh, const T* base, const uint32_t* marks, int lo, int hi,
+                                         float tau, int shift, int K) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    bool equal = true;
+    __syncthreads();
+    for (int t0 = 0; t0 < hi; t0 += kTile) {
+        for (int u = 0; u < kPer / Vec<T>::N; ++u)
+            enter<T>(sh, base, marks, t0 + (u * kBThreads + tid) * Vec<T>::N, lo, hi, tau, equal, shift);
+        __syncthreads();
+        if (sh.count > kListLimit) {
+            block_select(sh, K);
+            if (tid < K) sh.list[tid] = sh.best[tid];
+            if (tid == 0) sh.count = K;
+            tau = key_value(sh.best[K - 1]);
+            equal = false;
+        }
+        __syncthreads();
+    }
+}
+
+// The prompt's offers: ranks of all of them in shared memory, each beam's in order, so K
+// times the best head of a beam is taken. Lane l holds the heads of beams l and l + 32.
+__device__ __noinline__ void select_prompt(SelectShared& sh, const BeamArgs& p, int prompt) {
+    const int tid = threadIdx.x, lane = tid & 31, K = p.beams;
+    const int64_t row0 = (int64_t)prompt * K;
+    u64* ranks = sh.list;           // [beams][K] order_of(rank); 0: none
+    u64* keys = sh.list + K * K;    // the offers' keys, where there is room for them
+    const bool kept = 2 * K * K <= kListCap;
+    if (tid < K) {
+        sh.lse[tid] = sh.done[tid] ? 0.0 : __ldcg(p.ws.lse + row0 + tid);
+        const int n = max(sh.done[tid] ? sh.old[tid] : sh.old[tid] + 1, 1);
+        sh.size[tid] = p.alpha == 0.0 ? 1.0 : pow((double)n, p.alpha);
+    } else if (tid >= kBThreads - kStopsKept && tid - (kBThreads - kStopsKept) < p.n_stop) {
+        sh.stop[tid - (kBThreads - kStopsKept)] = p.stop_ids[tid - (kBThreads - kStopsKept)];
+    }
+    __syncthreads();
+    auto offer = [&](int b, u64 key) { return (double)sh.score[b] + ((double)key_value(key) - sh.lse[b]); };
+    for (int e = tid; e < K * K; e += kBThreads) {
+        const int b = e / K, i = e - b * K;
+        double score = -INFINITY;
+        if (sh.done[b]) {
+            if (i == 0) score = sh.score[b];
         } else {
-            const u64 k = __ldcg(p.ws.best + (row0 + b) * K + at[j]);
-            if (k == 0) return;
-            score[j] = before + ((double)key_value(k) - __ldcg(p.ws.lse + row0 + b));
-            token[j] = key_token(k);
+            const u64 k = __ldcg(p.ws.best + row0 * K + e);
+            if (kept) keys[e] = k;
+            if (k) score = offer(b, k);
         }
-        if (score[j] > -INFINITY) rank[j] = score[j] / s_size[b];
-    };
-    head(0);
-    head(1);
+        ranks[e] = score > -INFINITY ? order_of(score / sh.size[b]) : 0;
+    }
+    __syncthreads();
+    if (tid >= 32) return;
+    const u64 none = order_of(-INFINITY);
+    int at0 = 0, at1 = 0;
+    u64 h0 = lane < K ? ranks[lane * K] : 0, h1 = lane + 32 < K ? ranks[(lane + 32) * K] : 0;
     for (int k = 0; k < K; ++k) {
-        double best = rank[0];
-        int from = lane;
-        if (rank[1] > best) best = rank[1], from = lane + 32;
-        for (int s = 16; s > 0; s >>= 1) {
-            const double o = __shfl_xor_sync(FULLMASK, best, s);
-            const int f = __shfl_xor_sync(FULLMASK, from, s);
-            if (o > best || (o == best && f < from)) best = o, from = f;
-        }
-        if (!(best > -INFINITY)) {
-            if (lane == 0) o_parent[k] = -1;
-            continue;
-        }
-        if ((from & 31) == lane) {
-            const int j = from >> 5;
-            o_parent[k] = from;
-            o_token[k] = j ? token[1] : token[0];
-            o_score[k] = j ? score[1] : score[0];
-            if (j) ++at[1], head(1);
-            else ++at[0], head(0);
+        const bool second = h1 > h0;
+        const u64 h = second ? h1 : h0;
+        const uint32_t hi = __reduce_max_sync(FULLMASK, (uint32_t)(h >> 32));
+        const uint32_t lo = __reduce_max_sync(FULLMASK, (uint32_t)(h >> 32) == hi ? (uint32_t)h : 0u);
+        const u64 top = (u64)hi << 32 | lo;
+        const int from = (int)__reduce_min_sync(FULLMASK, h == top ? (uint32_t)(second ? lane + 32 : lane) : 64u);
+        if (top <= none) {
+            if (lane == 0) sh.parent[k] = -1;
+        } else if ((from & 31) == lane) {
+            sh.parent[k] = from;
+            if (from >= 32) {
+                sh.place[k] = at1;
+                h1 = ++at1 < K ? ranks[from * K + at1] : 0;
+            } else {
+                sh.place[k] = at0;
+                h0 = ++at0 < K ? ranks[from * K + at0] : 0;
+            }
         }
     }
     __syncwarp();
     for (int k = lane; k < K; k += 32) {
         const int64_t r = row0 + k;
-        const int b = o_parent[k];
-        const bool none = b < 0, fresh = !none && !s_done[b];
-        const int tok = none ? p.pad : o_token[k];
+        const int b = sh.parent[k];
+        const bool nothing = b < 0, fresh = !nothing && !sh.done[b];
+        u64 key = 0;
+        if (fresh) key = kept ? keys[b * K + sh.place[k]] : __ldcg(p.ws.best + (row0 + b) * K + sh.place[k]);
+        const int token = fresh ? key_token(key) : p.pad;
         bool stop = false;
-        if (fresh)
-            for (int i = 0; i < p.n_stop; ++i) stop |= p.stop_ids[i] == tok;
-        p.tokens[r] = tok;
-        p.parents[r] = none ? k : b;
-        p.scores[r] = none ? -INFINITY : (float)o_score[k];
-        p.lengths[r] = none ? s_old[k] : s_len[b];
-        p.finished[r] = none ? 0 : fresh ? stop : 1;
+        if (fresh) {
+            for (int i = 0; i < min(p.n_stop, kStopsKept); ++i) stop |= sh.stop[i] == token;
+            for (int i = kStopsKept; i < p.n_stop; ++i) stop |= p.stop_ids[i] == token;
+        }
+        p.tokens[r] = token;
+        p.parents[r] = nothing ? k : b;
+        p.scores[r] = nothing ? -INFINITY : fresh ? (float)offer(b, key) : sh.score[b];
+        p.lengths[r] = nothing ? sh.old[k] : sh.old[b] + fresh;
+        p.finished[r] = nothing ? 0 : fresh ? stop : 1;
         p.ws.push[r] = fresh;
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kBThreads) beam_select_kernel(BeamArgs p) {
+template <typename T, bool PEN>
+__global__ void __launch_bounds__(kBThreads, 3) beam_select_kernel(const __grid_constant__ BeamArgs p) {
     extern __shared__ __align__(16) unsigned char smem[];
     SelectShared& sh = *reinterpret_cast<SelectShared*>(smem);
-    uint32_t* marks = reinterpret_cast<uint32_t*>(smem + sizeof(SelectShared));
+    uint32_t* marks = reinterpret_cast<uint32_t*>(smem + sizeof(SelectShared));  // PEN: a bit for each position
+    u64* extra = reinterpret_cast<u64*>(smem + sizeof(SelectShared) + p.chunk / 8);  // PEN: the ring's tokens
     constexpr int VN = Vec<T>::N;
+    constexpr int kUnit = kBThreads * kVecs * VN;  // elements that are loaded together: one tile, two of bf16
+    asm volatile("griddepcontrol.launch_dependents;");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = p.beams;
     const int row = blockIdx.x / p.chunks, c = blockIdx.x - row * p.chunks;
+    const int prompt = row / K;
     const bool live = p.finished_in[row] == 0 && p.scores_in[row] > -INFINITY;
+    if (tid < K) {
+        // The prompt's rows, for its last CTA: nothing is written before that one.
+        const int64_t r = (int64_t)prompt * K + tid;
+        sh.score[tid] = p.scores_in[r];
+        sh.done[tid] = p.finished_in[r] != 0;
+        sh.old[tid] = p.lengths_in[r];
+    }
     if (live) {
-        // Positions count from the 16-byte boundary at or below the row's first element.
+        // Positions count from the 16-byte boundary at or below the row's first element, and
+        // within the chunk: [lo, hi) hold logits, position e is token e + shift.
         const T* x = static_cast<const T*>(p.logits) + (int64_t)row * p.stride;
         const int off = (int)(((uintptr_t)x & 15) / sizeof(T));
-        const T* base = x - off;
-        const int64_t lo = off, hi = (int64_t)p.vocab + off;
-        const int64_t c0 = (int64_t)c * p.chunk, c1 = min(c0 + p.chunk, hi);
-        const bool pen = p.window > 0 && p.penalty != 1.0f;
-        const int32_t* ring = pen ? p.hist_in + (int64_t)row * p.window : nullptr;
-        const int held = pen ? min(max(p.count_in[row], 0), p.window) : 0;
-        if (pen) {
+        const int64_t c0 = (int64_t)c * p.chunk;
+        const T* base = x - off + c0;
+        const int lo = c == 0 ? off : 0, hi = (int)min((int64_t)p.chunk, p.vocab + off - c0);
+        const int shift = (int)(c0 - off);
+        auto load = [&](int u0, uint4* v) {
+#pragma unroll
+            for (int u = 0; u < kVecs; ++u) v[u] = load_vector<T>(base, u0 + (u * kBThreads + tid) * VN, lo, hi);
+        };
+        uint4 next[kVecs];
+        load(0, next);
+        float m = -FLT_MAX, s = 0.0f;
+        if (PEN) {
+            // The chunk's tokens that the ring holds leave the stream (their marks) and enter here,
+            // with x / p for x > 0, else x * p, once for each time that the ring holds them
+            // (Sampler.pas:285-303). The entry whose thread sets the mark stands for the token.
+            const int32_t* ring = p.hist_in + (int64_t)row * p.window;
+            const int held = min(max(p.count_in[row], 0), p.window);
+            int* tokens = reinterpret_cast<int*>(sh.list);
             for (int i = tid; i < p.chunk / 32; i += kBThreads) marks[i] = 0;
+            if (tid == 0) sh.count = 0, sh.extra = 0;
             __syncthreads();
             for (int i = tid; i < held; i += kBThreads) {
-                const int64_t v = (int64_t)ring[i] + off;
-                if (ring[i] >= 0 && ring[i] < p.vocab && v >= c0 && v < c1)
-                    atomicOr(&marks[(v - c0) >> 5], 1u << ((v - c0) & 31));
-            }
-        }
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        float m = -FLT_MAX, s = 0.0f, tau = -INFINITY;
-        bool first = true;
-        for (int64_t t0 = c0; t0 < c1; t0 += kTile) {
-            float v[kPer];
-#pragma unroll
-            for (int u = 0; u < kPer / VN; ++u) {
-                const int64_t e = t0 + (int64_t)(u * kBThreads + tid) * VN;
-                if (e >= lo && e + VN <= c1) {
-                    Vec<T>::load(base + e, v + u * VN);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < VN; ++i)
-                        v[u * VN + i] = e + i >= lo && e + i < c1 ? Vec<T>::one(base + e + i) : -INFINITY;
-                }
-                if (pen && e < c1) {
-                    const uint32_t w = (marks[(e - c0) >> 5] >> ((e - c0) & 31)) & ((1u << VN) - 1);
-                    if (w) {
-#pragma unroll
-                        for (int i = 0; i < VN; ++i)
-                            if (w >> i & 1)
-                                v[u * VN + i] = penalised(v[u * VN + i], (int)(e + i - off), ring, held, p.penalty);
-                    }
+                const int token = ring[i];
+                const int64_t e = (int64_t)token - shift;
+                if (token >= 0 && token < p.vocab && e >= lo && e < hi) {
+                    const uint32_t bit = 1u << (e & 31);
+                    const uint32_t before = atomicOr(&marks[e >> 5], bit);
+                    tokens[atomicAdd(&sh.count, 1)] = before & bit ? ~token : token;
                 }
             }
-            float top = v[0];
-#pragma unroll
-            for (int i = 1; i < kPer; ++i) top = fmaxf(top, v[i]);
-            if (top > m) {
-                s *= ex2((m - top) * kLog2e);
-                m = top;
-            }
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) s += ex2((v[i] - m) * kLog2e);
-            if (first) {
-                block_bound(sh, make_key(top, tid), K);
-                tau = key_value(sh.bound);
-            }
-            if (first ? top >= tau : top > tau) {
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) {
-                    if ((first ? v[i] >= tau : v[i] > tau) && v[i] > -INFINITY) {
-                        const int64_t e = t0 + (int64_t)((i / VN) * kBThreads + tid) * VN + i % VN;
-                        sh.list[atomicAdd(&sh.count, 1)] = make_key(v[i], (int)(e - off));
-                    }
-                }
-            }
-            first = false;
             __syncthreads();
-            if (sh.count > kListLimit && t0 + kTile < c1) {
-                block_select(sh, K);
-                if (tid < K) sh.list[tid] = sh.best[tid];
-                if (tid == 0) sh.count = K;
-                tau = key_value(sh.best[K - 1]);
+            const int n = sh.count;
+            for (int i = tid; i < n; i += kBThreads) {
+                const int token = tokens[i];
+                if (token < 0) continue;
+                float v = Vec<T>::one(base + (token - shift));
+                for (int j = 0; j < n; ++j)
+                    if (tokens[j] == token || ~tokens[j] == token)
+                        v = v > 0.0f ? __fdiv_rn(v, p.penalty) : __fmul_rn(v, p.penalty);
+                if (v > m) s *= ex2((m - v) * kLog2e), m = v;
+                s += ex2((v - m) * kLog2e);
+                // Kept beside the list: a ring is at most kMaxHistory entries long.
+                if (v > -INFINITY) extra[atomicAdd(&sh.extra, 1)] = make_key(v, token);
             }
             __syncthreads();
         }
-        block_select(sh, K);
-        const int64_t slot = (int64_t)row * p.chunks + c;
-        if (tid < K) p.ws.cand[slot * K + tid] = sh.best[tid];
+        float* tops = reinterpret_cast<float*>(sh.list);  // [tiles][threads]
+        float most = -INFINITY;
+        int tiles = 0;
+        for (int u0 = 0; u0 < hi; u0 += kUnit) {
+            uint4 raw[kVecs];
+#pragma unroll
+            for (int u = 0; u < kVecs; ++u) raw[u] = next[u];
+            if (u0 + kUnit < hi) load(u0 + kUnit, next);
+#pragma unroll
+            for (int part = 0; part < kVecs * VN / kPer; ++part) {
+                float v[kPer];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) v[i] = Vec<T>::at(raw, part * kPer + i);
+                if (PEN) {
+#pragma unroll
+                    for (int u = 0; u < kPer / VN; ++u) {
+                        const int e = u0 + part * kTile + (u * kBThreads + tid) * VN;
+                        const uint32_t w = e < hi ? (marks[e >> 5] >> (e & 31)) & ((1u << VN) - 1) : 0u;
+                        if (w) {
+#pragma unroll
+                            for (int i = 0; i < VN; ++i)
+                                if (w >> i & 1) v[u * VN + i] = -INFINITY;
+                        }
+                    }
+                }
+                float top = v[0];
+#pragma unroll
+                for (int i = 1; i < kPer; ++i) top = fmaxf(top, v[i]);
+                tops[tiles++ * kBThreads + tid] = top;
+                most = fmaxf(most, top);
+                if (top > m) {
+                    s *= ex2((m - top) * kLog2e);
+                    m = top;
+                }
+                u64 sum = 0;
+                const u64 minus = pack2(-m, -m), scale = pack2(kLog2e, kLog2e);
+#pragma unroll
+                for (int i = 0; i < kPer; i += 2) {
+                    float y0, y1;
+                    unpack2(mul2(add2(pack2(v[i], v[i + 1]), minus), scale), y0, y1);
+                    sum = add2(sum, pack2(ex2(y0), ex2(y1)));
+                }
+                float sum0, sum1;
+                unpack2(sum, sum0, sum1);
+                s += sum0 + sum1;
+            }
+        }
+        // The bound: the K-th largest of 64 (128) disjoint groups' maxima.
+        float* groups = reinterpret_cast<float*>(sh.maxima);
+        const int share = K <= 16 ? 4 : 2;
+        float g = fmaxf(most, __shfl_xor_sync(FULLMASK, most, 1));
+        if (share == 4) g = fmaxf(g, __shfl_xor_sync(FULLMASK, g, 2));
+        if (tid % share == 0) groups[tid / share] = g;
         float wm = m;
         for (int d = 16; d > 0; d >>= 1) wm = fmaxf(wm, __shfl_xor_sync(FULLMASK, wm, d));
         double ws = (double)s * ex2((m - wm) * kLog2e);
         for (int d = 16; d > 0; d >>= 1) ws += __shfl_xor_sync(FULLMASK, ws, d);
         if (lane == 0) sh.wm[warp] = wm, sh.ws[warp] = ws;
+        if (tid == 0) sh.count = 0;
         __syncthreads();
+        const int n = kBThreads / share;
+        if (tid < n && count_above(groups, n, groups[tid], tid) == K - 1) sh.fbound = groups[tid];
+        __syncthreads();
+        const float tau = sh.fbound;
+        if (most >= tau) {
+            for (int t = 0; t < tiles; ++t) {
+                const float top = tops[t * kBThreads + tid];
+                if (top >= tau && top > -INFINITY) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < kGroups) sh.group[at] = (unsigned short)(t * kBThreads + tid);
+                }
+            }
+        }
+        __syncthreads();
+        const int reach = sh.count;
+        const uint32_t* out = PEN ? marks : nullptr;
+        if (reach <= kGroups) {
+            __syncthreads();
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+            for (int q = tid; q < reach * (kPer / VN); q += kBThreads) {
+                const int at = sh.group[q / (kPer / VN)], u = q % (kPer / VN);
+                enter<T>(sh, base, out, at / kBThreads * kTile + (u * kBThreads + at % kBThreads) * VN, lo, hi, tau, true,
+                         shift);
+            }
+        } else {
+            select_slow<T>(sh, base, out, lo, hi, tau, shift, K);
+        }
+        if (PEN) {
+            // The ring's tokens join the rest, which is cut to K first.
+            const int more = sh.extra;
+            for (int i0 = 0; i0 < more; i0 += kTile) {
+                block_select(sh, K);
+                const int now = min(kTile, more - i0);
+                if (tid < K) sh.list[tid] = sh.best[tid];
+                for (int i = tid; i < now; i += kBThreads) sh.list[K + i] = extra[i0 + i];
+                if (tid == 0) sh.count = K + now;
+            }
+        }
+        block_select(sh, K);
+        const int64_t slot = (int64_t)row * p.chunks + c;
+        if (tid < K) p.ws.cand[slot * K + tid] = sh.best[tid];
         if (tid == 0) {
             float M = sh.wm[0];
-            for (int w = 1; w < kBThreads / 32; ++w) M = fmaxf(M, sh.wm[w]);
+            for (int w = 1; w < kBWarps; ++w) M = fmaxf(M, sh.wm[w]);
             double S = 0.0;
-            for (int w = 0; w < kBThreads / 32; ++w) S += sh.ws[w] * ex2((sh.wm[w] - M) * kLog2e);
+            for (int w = 0; w < kBWarps; ++w) S += sh.ws[w] * ex2((sh.wm[w] - M) * kLog2e);
             p.ws.part[2 * slot] = M;
             p.ws.part[2 * slot + 1] = S;
         }
     }
-    // The row's last CTA merges its chunks.
-    __threadfence();
+    // The row's last CTA merges its chunks. The barrier orders the CTA's writes before the fence
+    // of the thread that counts.
     __syncthreads();
-    if (tid == 0) sh.flag = atomicAdd(&p.ws.row_done[row], 1u) == (uint32_t)p.chunks - 1;
+    if (tid == 0) {
+        __threadfence();
+        sh.flag = atomicAdd(&p.ws.row_done[row], 1u) == (uint32_t)p.chunks - 1;
+        __threadfence();
+    }
     __syncthreads();
     if (!sh.flag) return;
-    __threadfence();
     if (live) {
         const int n = p.chunks * K;
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += kBThreads) {
-            const u64 k = __ldcg(p.ws.cand + (int64_t)row * n + i);
-            if (k) sh.list[atomicAdd(&sh.count, 1)] = k;
-        }
-        block_select(sh, K);
-        if (warp == 0) {
-            double M = -INFINITY, S = 0.0;
-            const double* part = p.ws.part + (int64_t)row * p.chunks * 2;
-            for (int i = lane; i < p.chunks; i += 32) M = fmax(M, __ldcg(part + 2 * i));
-            for (int d = 16; d > 0; d >>= 1) M = fmax(M, __shfl_xor_sync(FULLMASK, M, d));
-            for (int i = lane; i < p.chunks; i += 32) S += __ldcg(part + 2 * i + 1) * exp(__ldcg(part + 2 * i) - M);
+        if (tid == 0) sh.count = n;
+        if (warp == kBWarps - 1) {
+            const double2* part = reinterpret_cast<const double2*>(p.ws.part) + (int64_t)row * p.chunks;
+            const double2 zero = make_double2(-INFINITY, 0.0);
+            const double2 a = lane < p.chunks ? __ldcg(part + lane) : zero;
+            const double2 b = lane + 32 < p.chunks ? __ldcg(part + lane + 32) : zero;
+            float M = (float)fmax(a.x, b.x);  // maxima of fp32 values
+            for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(FULLMASK, M, d));
+            double S = a.y * ex2(((float)a.x - M) * kLog2e) + b.y * ex2(((float)b.x - M) * kLog2e);
             for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(FULLMASK, S, d);
-            if (lane == 0) p.ws.lse[row] = M + log(S);
-            // A NaN sum (a NaN or +infinity in the row) offers nothing.
-            for (int k = lane; k < K; k += 32) p.ws.best[(int64_t)row * K + k] = S > 0.0 ? sh.best[k] : 0;
+            // A NaN sum (a NaN or +infinity in the row), or none, offers nothing.
+            if (lane == 0) p.ws.lse[row] = M + log(S), sh.ws[0] = S;
         }
+        // Empty places have key 0 and stay below every entry.
+        for (int i = tid; i < n; i += kBThreads) sh.list[i] = __ldcg(p.ws.cand + (int64_t)row * n + i);
+        block_select(sh, K);
+        if (tid < K) p.ws.best[(int64_t)row * K + tid] = sh.ws[0] > 0.0 ? sh.best[tid] : 0;
     }
-    __threadfence();
     __syncthreads();
-    const int prompt = row / K;
     if (tid == 0) {
         p.ws.row_done[row] = 0;
+        __threadfence();
         sh.flag = atomicAdd(&p.ws.prompt_done[prompt], 1u) == (uint32_t)K - 1;
+        __threadfence();
     }
     __syncthreads();
-    if (!sh.flag || warp != 0) return;
-    __threadfence();
-    select_prompt(p, prompt);
-    if (lane == 0) p.ws.prompt_done[prompt] = 0;
+    if (!sh.flag) return;
+    select_prompt(sh, p, prompt);
+    if (tid == 0) p.ws.prompt_done[prompt] = 0;
 }
 
 constexpr int kRThreads = 128;
@@ -410,6 +595,9 @@ __device__ void move_words(const ReorderParams& p, int i, int prompt, int64_t fi
 __global__ void __launch_bounds__(kRThreads) beam_reorder_kernel(const __grid_constant__ ReorderParams p) {
     extern __shared__ __align__(16) unsigned char stage[];  // [beams][kRThreads] words
     __shared__ int parent[VDXS_BEAM_MAX_BEAMS], pos[VDXS_BEAM_MAX_BEAMS], count[VDXS_BEAM_MAX_BEAMS];
+    __shared__ int token[VDXS_BEAM_MAX_BEAMS], slot[VDXS_BEAM_MAX_BEAMS];
+    // A step's reordering is launched while its selection still runs, and waits here for its end.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int K = p.beams;
     int64_t block = blockIdx.x;
     const bool ring = block < p.ring_blocks;
@@ -448,16 +636,18 @@ __global__ void __launch_bounds__(kRThreads) beam_reorder_kernel(const __grid_co
         int at = p.pos_in[row0 + parent[k]] % W;
         pos[k] = at < 0 ? at + W : at;
         count[k] = p.count_in[row0 + parent[k]];
+        token[k] = p.tokens[row0 + k];
+        slot[k] = p.push[row0 + k] ? pos[k] : -1;
     }
     __syncthreads();
     int32_t* mine = reinterpret_cast<int32_t*>(stage) + threadIdx.x;
     for (int j = threadIdx.x; j < W; j += kRThreads) {
+#pragma unroll 8
         for (int k = 0; k < K; ++k) mine[k * kRThreads] = p.hist_in[(row0 + parent[k]) * W + j];
-        for (int k = 0; k < K; ++k)
-            p.hist[(row0 + k) * W + j] = p.push[row0 + k] && pos[k] == j ? p.tokens[row0 + k] : mine[k * kRThreads];
+        for (int k = 0; k < K; ++k) p.hist[(row0 + k) * W + j] = slot[k] == j ? token[k] : mine[k * kRThreads];
     }
     for (int k = threadIdx.x; k < K; k += kRThreads) {
-        const bool push = p.push[row0 + k] != 0;
+        const bool push = slot[k] >= 0;
         p.pos[row0 + k] = push ? (pos[k] + 1) % W : pos[k];
         p.count[row0 + k] = push && count[k] < W ? max(count[k], 0) + 1 : count[k];
     }
@@ -469,9 +659,10 @@ void beam_plan(int rows, int vocab, int sm_count, int* chunks, int* chunk) {
     // A position is counted from a 16-byte boundary, so up to 7 lie before the row.
     const int64_t span = (int64_t)vocab + 7;
     const int64_t tiles = (span + kTile - 1) / kTile;
-    // Two CTAs for each SM's four places at least, and at most kBeamMaxChunks lists to merge.
-    int64_t want = std::min<int64_t>(kBeamMaxChunks, std::max<int64_t>(1, ((int64_t)sm_count * 8 + rows - 1) / rows));
-    want = std::min(want, tiles);
+    // Every CTA place once (three for each SM), at most kBeamMaxChunks lists to merge, and at
+    // most kMaxTiles tiles to a chunk.
+    int64_t want = std::min<int64_t>(kBeamMaxChunks, std::max<int64_t>(1, (int64_t)sm_count * 3 / rows));
+    want = std::min(std::max(want, (tiles + kMaxTiles - 1) / kMaxTiles), tiles);
     const int64_t per = (tiles + want - 1) / want;
     *chunk = (int)(per * kTile);
     *chunks = (int)((tiles + per - 1) / per);
@@ -479,19 +670,21 @@ void beam_plan(int rows, int vocab, int sm_count, int* chunks, int* chunk) {
 
 cudaError_t beam_select(const BeamArgs& a, cudaStream_t stream) {
     const bool pen = a.window > 0 && a.penalty != 1.0f;
-    const size_t smem = sizeof(SelectShared) + (pen ? (size_t)a.chunk / 8 : 0);
+    const size_t smem = sizeof(SelectShared) + (pen ? (size_t)a.chunk / 8 + (size_t)std::min(a.window, a.chunk) * 8 : 0);
     const int grid = a.batch * a.beams * a.chunks;
-    void (*kern)(BeamArgs) =
-        a.dtype == VDXS_DTYPE_BF16 ? beam_select_kernel<__nv_bfloat16> : beam_select_kernel<float>;
-    static SmemLimit limit[2];
-    cudaError_t e = limit[a.dtype == VDXS_DTYPE_BF16].raise(kern, smem);
+    const bool half = a.dtype == VDXS_DTYPE_BF16;
+    void (*kern)(BeamArgs) = half ? (pen ? beam_select_kernel<__nv_bfloat16, true> : beam_select_kernel<__nv_bfloat16, false>)
+                                  : (pen ? beam_select_kernel<float, true> : beam_select_kernel<float, false>);
+    static SmemLimit limit[4];
+    cudaError_t e = limit[2 * half + pen].raise(kern, smem);
     if (e != cudaSuccess) return e;
     kern<<<grid, kBThreads, smem, stream>>>(a);
     return cudaGetLastError();
 }
 
-cudaError_t beam_reorder(const BeamArgs& a, bool rings, const BeamCacheArgs* caches, int n_caches, cudaStream_t stream,
-                         int* launches) {
+cudaError_t beam_reorder(const BeamArgs& a, bool behind_select, const BeamCacheArgs* caches, int n_caches,
+                         cudaStream_t stream, int* launches) {
+    bool rings = behind_select && a.window > 0;
     const size_t smem = (size_t)a.beams * kRThreads * 16;
     static SmemLimit limit;
     cudaError_t e = limit.raise(beam_reorder_kernel, smem);
@@ -532,8 +725,18 @@ cudaError_t beam_reorder(const BeamArgs& a, bool rings, const BeamCacheArgs* cac
         const int64_t grid = p.ring_blocks + end;
         if (grid == 0) continue;
         if (grid > INT32_MAX) return cudaErrorInvalidValue;
-        beam_reorder_kernel<<<(unsigned)grid, kRThreads, smem, stream>>>(p);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        cudaLaunchAttribute early{};
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3(kRThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cfg.attrs = &early;
+        cfg.numAttrs = behind_select ? 1 : 0;
+        behind_select = false;
+        if ((e = cudaLaunchKernelEx(&cfg, beam_reorder_kernel, p)) != cudaSuccess) return e;
         ++*launches;
     }
     return cudaSuccess;

@@ -228,11 +228,12 @@ struct BeamCacheArgs {  // vdxs_beam_cache
 };
 // Chunks of a row of `vocab` logits (at most kBeamMaxChunks) and their length.
 constexpr int kBeamMaxChunks = 64;
+constexpr int kBeamMaxVocab = 8000000;  // kBeamMaxChunks chunks of the longest kind
 void beam_plan(int rows, int vocab, int sm_count, int* chunks, int* chunk);
 cudaError_t beam_select(const BeamArgs& a, cudaStream_t stream);
-// Rings (where a.window > 0 and rings is true) and caches by a.parents.
-cudaError_t beam_reorder(const BeamArgs& a, bool rings, const BeamCacheArgs* caches, int n_caches, cudaStream_t stream,
-                         int* launches);
+// Caches by a.parents; behind a beam_select on the same stream also the rings (a.window > 0).
+cudaError_t beam_reorder(const BeamArgs& a, bool behind_select, const BeamCacheArgs* caches, int n_caches,
+                         cudaStream_t stream, int* launches);
 // Device-resident decode state (one thread per row).
 cudaError_t launch_device_uniforms(uint64_t* prng, int batch, float* out, cudaStream_t stream);
 cudaError_t launch_history_push(int32_t* hist, int32_t* pos, int32_t* count, int window, const int32_t* tokens,
