@@ -28,9 +28,11 @@ constexpr int kPer = 16;                      // elements of a tile per thread
 constexpr int kTile = kBThreads * kPer;       // 4096
 constexpr int kVecs = 4;                      // 16-byte loads per thread that are in flight together
 constexpr int kListLimit = 512;               // entries before a list is cut back to K
+constexpr int kListShort = 96;                // entries that are ranked without a bound
 constexpr int kListCap = kTile + kListLimit;  // a tile may add every element it has
 constexpr int kMaxTiles = 32;                 // tiles of a chunk
 constexpr int kGroups = kBThreads;            // groups that may be read again
+constexpr int kValues = (kListCap * 8 - kMaxHistory * 4) / 4;  // penalised logits kept in the list's room
 constexpr int kStopsKept = 64;                // stop ids in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 typedef unsigned long long u64;
@@ -58,12 +60,21 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Counts one more of a group of CTAs, and orders what the CTA wrote before (its barrier) and what
+// it reads behind the count.
+__device__ __forceinline__ uint32_t count_in(uint32_t* counter) {
+    uint32_t before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    return before;
+}
+
 struct SelectShared {
     u64 list[kListCap];
     u64 best[VDXS_BEAM_MAX_BEAMS];
     u64 maxima[kBThreads];
     u64 bound;
-    int count, extra;
+    int count, extra, reach;
+    uint32_t marked;  // tiles with marks
     int flag;
     float fbound;
     float wm[kBWarps];
@@ -92,52 +103,77 @@ __device__ __forceinline__ int count_above(const float* p, int n, float mine, in
     return above;
 }
 
+// The K-th largest of 64 (K <= 16) or 128 disjoint groups' maxima, of one value per thread: a
+// lower bound of the K-th largest of what the values are the maxima of. In sh.fbound.
+__device__ __forceinline__ void block_bound(SelectShared& sh, float v, int K) {
+    float* groups = reinterpret_cast<float*>(sh.maxima);
+    const int tid = threadIdx.x, share = K <= 16 ? 4 : 2, n = kBThreads / share;
+    v = fmaxf(v, __shfl_xor_sync(FULLMASK, v, 1));
+    if (share == 4) v = fmaxf(v, __shfl_xor_sync(FULLMASK, v, 2));
+    if (tid % share == 0) groups[tid / share] = v;
+    __syncthreads();
+    if (tid < n && count_above(groups, n, groups[tid], tid) == K - 1) sh.fbound = groups[tid];
+    __syncthreads();
+}
+
+// Keeps list[0..n) entries that are at least `bound`; their number in sh.count.
+__device__ __forceinline__ void block_keep(SelectShared& sh, int n, u64 bound) {
+    const int tid = threadIdx.x;
+    u64 mine[kListCap / kBThreads];
+    int m = 0;
+#pragma unroll
+    for (int j = 0; j < kListCap / kBThreads; ++j) {
+        const int i = tid + j * kBThreads;
+        mine[j] = i < n && sh.list[i] >= bound ? sh.list[i] : 0;
+        m += mine[j] != 0;
+    }
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    int at = m ? atomicAdd(&sh.count, m) : 0;
+#pragma unroll
+    for (int j = 0; j < kListCap / kBThreads; ++j)
+        if (mine[j]) sh.list[at++] = mine[j];
+    __syncthreads();
+}
+
 // Cuts list[0..count) to its K largest, in order, in best[]; the rest of best is 0.
-// While the list is long, each thread takes the maximum of its share: the K-th largest of
-// those is a lower bound of the K-th largest entry, and at most a quarter plus K remain.
-// Then every entry counts the ones above it.
+// Of a longer list first those that reach a bound stay. Equal values get past that: while the
+// list is still long, each thread takes the largest key of its share, the K-th largest of
+// those (keys are all different) is a bound again, and at most a quarter plus K remain. Then
+// every entry counts the ones above it.
 __device__ __noinline__ void block_select(SelectShared& sh, int K) {
     const int tid = threadIdx.x;
     __syncthreads();
     int n = sh.count;
+    if (tid < K) sh.best[tid] = 0;
+    if (n > kListShort) {
+        u64 mx = 0;
+        for (int i = tid; i < n; i += kBThreads) mx = max(mx, sh.list[i]);
+        block_bound(sh, mx ? key_value(mx) : -INFINITY, K);
+        block_keep(sh, n, (make_key(sh.fbound, -1) >> 32) << 32);
+        n = sh.count;
+    }
     while (n > kListLimit) {
         u64 mx = 0;
         for (int i = tid; i < n; i += kBThreads) mx = max(mx, sh.list[i]);
         sh.maxima[tid] = mx;
         __syncthreads();
         int above = 0;
-#pragma unroll 8
         for (int j = 0; j < kBThreads; ++j) {
             const u64 o = sh.maxima[j];
             above += o > mx || (o == mx && j < tid);
         }
         if (above == K - 1) sh.bound = mx;
         __syncthreads();
-        const u64 bound = sh.bound;
-        u64 mine[kListCap / kBThreads];
-        int m = 0;
-#pragma unroll
-        for (int j = 0; j < kListCap / kBThreads; ++j) {
-            const int i = tid + j * kBThreads;
-            mine[j] = i < n && sh.list[i] >= bound ? sh.list[i] : 0;
-            m += mine[j] != 0;
-        }
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        int at = m ? atomicAdd(&sh.count, m) : 0;
-#pragma unroll
-        for (int j = 0; j < kListCap / kBThreads; ++j)
-            if (mine[j]) sh.list[at++] = mine[j];
-        __syncthreads();
+        block_keep(sh, n, sh.bound);
         n = sh.count;
     }
-    if (tid < K) sh.best[tid] = 0;
     if (tid == 0) sh.list[n] = 0;  // an even number of entries
     __syncthreads();
     for (int i = tid; i < n; i += kBThreads) {
         const u64 mine = sh.list[i];
         int above = 0;
-#pragma unroll 4
+#pragma unroll 2
         for (int j = 0; j < n; j += 2) {
             const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(sh.list + j);
             above += (o.x > mine) + (o.y > mine);
@@ -265,49 +301,54 @@ __device__ __noinline__ void select_prompt(SelectShared& sh, const BeamArgs& p, 
     u64* ranks = sh.list;           // [beams][K] order_of(rank); 0: none
     u64* keys = sh.list + K * K;    // the offers' keys, where there is room for them
     const bool kept = 2 * K * K <= kListCap;
-    if (tid < K) {
-        sh.lse[tid] = sh.done[tid] ? 0.0 : __ldcg(p.ws.lse + row0 + tid);
-        const int n = max(sh.done[tid] ? sh.old[tid] : sh.old[tid] + 1, 1);
-        sh.size[tid] = p.alpha == 0.0 ? 1.0 : pow((double)n, p.alpha);
-    } else if (tid >= kBThreads - kStopsKept && tid - (kBThreads - kStopsKept) < p.n_stop) {
-        sh.stop[tid - (kBThreads - kStopsKept)] = p.stop_ids[tid - (kBThreads - kStopsKept)];
+    if (tid < min(p.n_stop, kStopsKept)) sh.stop[tid] = p.stop_ids[tid];
+    if (tid >= 64 && tid < 64 + K) {
+        const int b = tid - 64;
+        sh.lse[b] = sh.done[b] ? 0.0 : __ldcg(p.ws.lse + row0 + b);
+        if (p.alpha != 0.0) sh.size[b] = pow((double)max(sh.done[b] ? sh.old[b] : sh.old[b] + 1, 1), p.alpha);
     }
-    __syncthreads();
     auto offer = [&](int b, u64 key) { return (double)sh.score[b] + ((double)key_value(key) - sh.lse[b]); };
-    for (int e = tid; e < K * K; e += kBThreads) {
-        const int b = e / K, i = e - b * K;
+    for (int e0 = 0; e0 < K * K; e0 += kBThreads) {
+        const int e = e0 + tid, b = e / K, i = e - b * K;
+        const bool mine = e < K * K;
+        const u64 k = mine && !sh.done[b] ? __ldcg(p.ws.best + row0 * K + e) : 0;
+        if (e0 == 0) __syncthreads();
+        if (!mine) break;
+        if (kept) keys[e] = k;
         double score = -INFINITY;
-        if (sh.done[b]) {
-            if (i == 0) score = sh.score[b];
-        } else {
-            const u64 k = __ldcg(p.ws.best + row0 * K + e);
-            if (kept) keys[e] = k;
-            if (k) score = offer(b, k);
-        }
-        ranks[e] = score > -INFINITY ? order_of(score / sh.size[b]) : 0;
+        if (k) score = offer(b, k);
+        else if (i == 0 && sh.done[b]) score = sh.score[b];
+        if (p.alpha != 0.0) score /= sh.size[b];
+        ranks[e] = score > -INFINITY ? order_of(score) : 0;
     }
     __syncthreads();
     if (tid >= 32) return;
-    const u64 none = order_of(-INFINITY);
     int at0 = 0, at1 = 0;
     u64 h0 = lane < K ? ranks[lane * K] : 0, h1 = lane + 32 < K ? ranks[(lane + 32) * K] : 0;
     for (int k = 0; k < K; ++k) {
         const bool second = h1 > h0;
-        const u64 h = second ? h1 : h0;
+        u64 h = second ? h1 : h0;
+        // The highest rank: by its upper half, where that is not enough by the lower, and among
+        // equals the lowest beam.
         const uint32_t hi = __reduce_max_sync(FULLMASK, (uint32_t)(h >> 32));
-        const uint32_t lo = __reduce_max_sync(FULLMASK, (uint32_t)(h >> 32) == hi ? (uint32_t)h : 0u);
-        const u64 top = (u64)hi << 32 | lo;
-        const int from = (int)__reduce_min_sync(FULLMASK, h == top ? (uint32_t)(second ? lane + 32 : lane) : 64u);
-        if (top <= none) {
+        bool top = (uint32_t)(h >> 32) == hi;
+        uint32_t who = __ballot_sync(FULLMASK, top);
+        if (who & (who - 1)) {
+            const uint32_t lo = __reduce_max_sync(FULLMASK, top ? (uint32_t)h : 0u);
+            top = top && (uint32_t)h == lo;
+            const uint32_t first = __reduce_min_sync(FULLMASK, top ? (uint32_t)(second ? lane + 32 : lane) : 64u);
+            who = 1u << (first & 31);
+        }
+        if (hi == 0) {  // no offer is left (a rank's upper half is never 0)
             if (lane == 0) sh.parent[k] = -1;
-        } else if ((from & 31) == lane) {
-            sh.parent[k] = from;
-            if (from >= 32) {
+        } else if (who >> lane & 1) {
+            sh.parent[k] = second ? lane + 32 : lane;
+            if (second) {
                 sh.place[k] = at1;
-                h1 = ++at1 < K ? ranks[from * K + at1] : 0;
+                h1 = ++at1 < K ? ranks[(lane + 32) * K + at1] : 0;
             } else {
                 sh.place[k] = at0;
-                h0 = ++at0 < K ? ranks[from * K + at0] : 0;
+                h0 = ++at0 < K ? ranks[lane * K + at0] : 0;
             }
         }
     }
@@ -374,18 +415,24 @@ __global__ void __launch_bounds__(kBThreads, 3) beam_select_kernel(const __grid_
             // with x / p for x > 0, else x * p, once for each time that the ring holds them
             // (Sampler.pas:285-303). The entry whose thread sets the mark stands for the token.
             const int32_t* ring = p.hist_in + (int64_t)row * p.window;
-            const int held = min(max(p.count_in[row], 0), p.window);
+            const int count = p.count_in[row];
             int* tokens = reinterpret_cast<int*>(sh.list);
+            float* values = reinterpret_cast<float*>(tokens + kMaxHistory);
+            if (tid == 0) sh.count = 0, sh.extra = 0, sh.marked = 0;
             for (int i = tid; i < p.chunk / 32; i += kBThreads) marks[i] = 0;
-            if (tid == 0) sh.count = 0, sh.extra = 0;
-            __syncthreads();
-            for (int i = tid; i < held; i += kBThreads) {
-                const int token = ring[i];
+            for (int i0 = 0; i0 < p.window; i0 += kBThreads) {
+                const int i = i0 + tid, token = i < p.window ? ring[i] : -1;
                 const int64_t e = (int64_t)token - shift;
-                if (token >= 0 && token < p.vocab && e >= lo && e < hi) {
+                const bool in = i < count && token >= 0 && token < p.vocab && e >= lo && e < hi;
+                const float v = in ? Vec<T>::one(base + e) : 0.0f;
+                if (i0 == 0) __syncthreads();
+                if (in) {
                     const uint32_t bit = 1u << (e & 31);
                     const uint32_t before = atomicOr(&marks[e >> 5], bit);
-                    tokens[atomicAdd(&sh.count, 1)] = before & bit ? ~token : token;
+                    atomicOr(&sh.marked, 1u << (e / kTile));
+                    const int at = atomicAdd(&sh.count, 1);
+                    tokens[at] = before & bit ? ~token : token;
+                    if (at < kValues) values[at] = v;
                 }
             }
             __syncthreads();
@@ -393,7 +440,7 @@ __global__ void __launch_bounds__(kBThreads, 3) beam_select_kernel(const __grid_
             for (int i = tid; i < n; i += kBThreads) {
                 const int token = tokens[i];
                 if (token < 0) continue;
-                float v = Vec<T>::one(base + (token - shift));
+                float v = i < kValues ? values[i] : Vec<T>::one(base + (token - shift));
                 for (int j = 0; j < n; ++j)
                     if (tokens[j] == token || ~tokens[j] == token)
                         v = v > 0.0f ? __fdiv_rn(v, p.penalty) : __fmul_rn(v, p.penalty);
@@ -404,6 +451,7 @@ __global__ void __launch_bounds__(kBThreads, 3) beam_select_kernel(const __grid_
             }
             __syncthreads();
         }
+        const uint32_t marked = PEN ? sh.marked : 0u;
         float* tops = reinterpret_cast<float*>(sh.list);  // [tiles][threads]
         float most = -INFINITY;
         int tiles = 0;
@@ -417,7 +465,7 @@ __global__ void __launch_bounds__(kBThreads, 3) beam_select_kernel(const __grid_
                 float v[kPer];
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) v[i] = Vec<T>::at(raw, part * kPer + i);
-                if (PEN) {
+                if (PEN && (marked >> tiles & 1)) {
 #pragma unroll
                     for (int u = 0; u < kPer / VN; ++u) {
                         const int e = u0 + part * kTile + (u * kBThreads + tid) * VN;
@@ -451,43 +499,35 @@ __global__ void __launch_bounds__(kBThreads, 3) beam_select_kernel(const __grid_
                 s += sum0 + sum1;
             }
         }
-        // The bound: the K-th largest of 64 (128) disjoint groups' maxima.
-        float* groups = reinterpret_cast<float*>(sh.maxima);
-        const int share = K <= 16 ? 4 : 2;
-        float g = fmaxf(most, __shfl_xor_sync(FULLMASK, most, 1));
-        if (share == 4) g = fmaxf(g, __shfl_xor_sync(FULLMASK, g, 2));
-        if (tid % share == 0) groups[tid / share] = g;
         float wm = m;
         for (int d = 16; d > 0; d >>= 1) wm = fmaxf(wm, __shfl_xor_sync(FULLMASK, wm, d));
         double ws = (double)s * ex2((m - wm) * kLog2e);
         for (int d = 16; d > 0; d >>= 1) ws += __shfl_xor_sync(FULLMASK, ws, d);
         if (lane == 0) sh.wm[warp] = wm, sh.ws[warp] = ws;
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        const int n = kBThreads / share;
-        if (tid < n && count_above(groups, n, groups[tid], tid) == K - 1) sh.fbound = groups[tid];
-        __syncthreads();
+        if (tid == 0) sh.count = 0, sh.reach = 0;
+        block_bound(sh, most, K);
         const float tau = sh.fbound;
         if (most >= tau) {
             for (int t = 0; t < tiles; ++t) {
                 const float top = tops[t * kBThreads + tid];
                 if (top >= tau && top > -INFINITY) {
-                    const int at = atomicAdd(&sh.count, 1);
+                    const int at = atomicAdd(&sh.reach, 1);
                     if (at < kGroups) sh.group[at] = (unsigned short)(t * kBThreads + tid);
                 }
             }
         }
         __syncthreads();
-        const int reach = sh.count;
+        const int reach = sh.reach;
         const uint32_t* out = PEN ? marks : nullptr;
         if (reach <= kGroups) {
-            __syncthreads();
-            if (tid == 0) sh.count = 0;
-            __syncthreads();
-            for (int q = tid; q < reach * (kPer / VN); q += kBThreads) {
-                const int at = sh.group[q / (kPer / VN)], u = q % (kPer / VN);
-                enter<T>(sh, base, out, at / kBThreads * kTile + (u * kBThreads + at % kBThreads) * VN, lo, hi, tau, true,
-                         shift);
+            // One element for each thread.
+            for (int q = tid; q < reach * kPer; q += kBThreads) {
+                const int at = sh.group[q / kPer], i = q % kPer;
+                const int e = at / kBThreads * kTile + (i / VN * kBThreads + at % kBThreads) * VN + i % VN;
+                if (e < lo || e >= hi) continue;
+                const float v = Vec<T>::one(base + e);
+                if (v >= tau && v > -INFINITY && !(PEN && (marks[e >> 5] >> (e & 31) & 1)))
+                    sh.list[atomicAdd(&sh.count, 1)] = make_key(v, e + shift);
             }
         } else {
             select_slow<T>(sh, base, out, lo, hi, tau, shift, K);
@@ -515,14 +555,9 @@ __global__ void __launch_bounds__(kBThreads, 3) beam_select_kernel(const __grid_
             p.ws.part[2 * slot + 1] = S;
         }
     }
-    // The row's last CTA merges its chunks. The barrier orders the CTA's writes before the fence
-    // of the thread that counts.
+    // The row's last CTA merges its chunks.
     __syncthreads();
-    if (tid == 0) {
-        __threadfence();
-        sh.flag = atomicAdd(&p.ws.row_done[row], 1u) == (uint32_t)p.chunks - 1;
-        __threadfence();
-    }
+    if (tid == 0) sh.flag = count_in(&p.ws.row_done[row]) == (uint32_t)p.chunks - 1;
     __syncthreads();
     if (!sh.flag) return;
     if (live) {
@@ -548,9 +583,7 @@ __global__ void __launch_bounds__(kBThreads, 3) beam_select_kernel(const __grid_
     __syncthreads();
     if (tid == 0) {
         p.ws.row_done[row] = 0;
-        __threadfence();
-        sh.flag = atomicAdd(&p.ws.prompt_done[prompt], 1u) == (uint32_t)K - 1;
-        __threadfence();
+        sh.flag = count_in(&p.ws.prompt_done[prompt]) == (uint32_t)K - 1;
     }
     __syncthreads();
     if (!sh.flag) return;
