@@ -31,42 +31,49 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
 // Sum of `a` and maximum of `b` over the block, in every thread.
-__device__ __forceinline__ void block_sum_max(double& a, double& b) {
-    __shared__ double sa[kNormThreads / 32], sb[kNormThreads / 32];
+template <typename B>
+__device__ __forceinline__ void block_sum_max(double& a, B& b) {
+    __shared__ double sa[32];
+    __shared__ B sb[32];
     for (int s = 16; s > 0; s >>= 1) {
         a += __shfl_xor_sync(FULLMASK, a, s);
-        b = fmax(b, __shfl_xor_sync(FULLMASK, b, s));
+        b = max(b, __shfl_xor_sync(FULLMASK, b, s));
     }
-    const int warp = threadIdx.x >> 5;
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (warps == 1) return;
     if ((threadIdx.x & 31) == 0) sa[warp] = a, sb[warp] = b;
     __syncthreads();
     a = sa[0];
     b = sb[0];
-    for (int w = 1; w < kNormThreads / 32; ++w) a += sa[w], b = fmax(b, sb[w]);
+    for (int w = 1; w < warps; ++w) a += sa[w], b = max(b, sb[w]);
 }
 
 // q = t / (top / 127) to the nearest even integer, in 64 bits: t * 127 is rounded once and
 // the quotient once, so a value on a border falls as the exact quotient does.
 __device__ __forceinline__ int quantum(double t, double top) { return (int)rint(t * 127.0 / top); }
 
-// One row per CTA. The row's h stays in shared memory between the sums and the rounding,
-// so an output in place of an input is safe.
+// The same from fp32 where that decides: t32, f = 127 / top and their product are rounded once
+// each (2^-24 relative), so v is off by at most 127 * 3 * 2^-24 = 2.3e-5; a v that is 1e-4 from
+// a border rounds as the exact quotient does. Else (one value in 5000) false.
+__device__ __forceinline__ bool quick_quantum(float t32, float f, int* q) {
+    const float v = t32 * f, r = rintf(v);
+    *q = (int)r;
+    return fabsf(v - r) <= 0.4999f;
+}
+
+// A row in 64 bits throughout. `done`: h is in p.hidden (or is x itself) already.
 template <typename T, typename W>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_i8_kernel(NormI8Args p) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    T* keep = reinterpret_cast<T*>(smem);
-    const int64_t row = blockIdx.x;
+__device__ __noinline__ void norm_row(const NormI8Args& p, int64_t row, bool done) {
     const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
     const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_stride : nullptr;
-    T* h = p.hidden ? static_cast<T*>(p.hidden) + row * p.hidden_stride : nullptr;
+    T* hidden = p.hidden ? static_cast<T*>(p.hidden) + row * p.hidden_stride : nullptr;
     const W* w = static_cast<const W*>(p.weight);
+    auto sum_of = [&](int i) { return r ? from_f32<T>(to_f32(x[i]) + to_f32(r[i])) : x[i]; };
     double sum = 0.0, top = 0.0;
     bool bad = false;
-    for (int i = threadIdx.x; i < p.dim; i += kNormThreads) {
-        T v = x[i];
-        if (r) v = from_f32<T>(to_f32(v) + to_f32(r[i]));
-        if (h) h[i] = v;
-        keep[i] = v;
+    for (int i = threadIdx.x; i < p.dim; i += blockDim.x) {
+        const T v = done && hidden ? hidden[i] : sum_of(i);
+        if (!done && hidden) hidden[i] = v;
         const double d = to_f32(v), t = d * (double)to_f32(w[i]);
         bad |= !(fabs(t) <= DBL_MAX) || !(fabs(d) <= DBL_MAX);
         sum += d * d;
@@ -74,11 +81,209 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_i8_kernel(NormI8Args p)
     }
     block_sum_max(sum, top);
     bad = __syncthreads_or(bad);
-    const double inv = 1.0 / sqrt(sum / p.dim + (double)p.eps);
-    if (threadIdx.x == 0) p.scale[row] = bad ? nanf("") : (float)(top / 127.0 * inv);
+    if (threadIdx.x == 0)
+        p.scale[row] = bad ? nanf("") : (float)(top / 127.0 * (1.0 / sqrt(sum / p.dim + (double)p.eps)));
     int8_t* q = p.q + row * p.q_stride;
-    for (int i = threadIdx.x; i < p.dim; i += kNormThreads)
-        q[i] = bad || top == 0.0 ? 0 : (int8_t)quantum((double)to_f32(keep[i]) * (double)to_f32(w[i]), top);
+    const float f = (float)(127.0 / top);
+    for (int i = threadIdx.x; i < p.dim; i += blockDim.x) {
+        // A thread reads what it wrote itself; without p.hidden the inputs are as they were.
+        const double t = (double)to_f32(hidden ? hidden[i] : sum_of(i)) * (double)to_f32(w[i]);
+        int v = 0;
+        if (!bad && top > 0.0 && !(f < 1e30f && quick_quantum((float)t, f, &v))) v = quantum(t, top);
+        q[i] = (int8_t)v;
+    }
+}
+
+// Rows of any alignment, one per CTA.
+template <typename T, typename W>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_i8_kernel(const __grid_constant__ NormI8Args p) {
+    norm_row<T, W>(p, blockIdx.x, false);
+}
+
+template <typename T>
+struct Pack;  // 16 bytes of a row
+template <>
+struct Pack<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void get(const uint4& v, float* f) {
+        f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ uint4 put(const float* f) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+};
+template <typename T2>
+__device__ __forceinline__ uint32_t bits_of(T2 v) {
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+template <>
+struct Pack<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(const uint4& v, float* f) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+    static __device__ __forceinline__ uint4 put(const float* f) {
+        return make_uint4(bits_of(__floats2bfloat162_rn(f[0], f[1])), bits_of(__floats2bfloat162_rn(f[2], f[3])),
+                          bits_of(__floats2bfloat162_rn(f[4], f[5])), bits_of(__floats2bfloat162_rn(f[6], f[7])));
+    }
+};
+template <>
+struct Pack<__half> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(const uint4& v, float* f) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = g.x, f[2 * i + 1] = g.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 put(const float* f) {
+        return make_uint4(bits_of(__floats2half2_rn(f[0], f[1])), bits_of(__floats2half2_rn(f[2], f[3])),
+                          bits_of(__floats2half2_rn(f[4], f[5])), bits_of(__floats2half2_rn(f[6], f[7])));
+    }
+};
+// N weights from an address that is a multiple of 16 bytes (8 for four 16-bit ones).
+template <typename W, int N>
+__device__ __forceinline__ void get_weights(const W* p, float* f) {
+    if constexpr (sizeof(W) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) Pack<float>::get(__ldg(reinterpret_cast<const uint4*>(p + i)), f + i);
+    } else if constexpr (N == 8) {
+        Pack<W>::get(__ldg(reinterpret_cast<const uint4*>(p)), f);
+    } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        float g[8];
+        Pack<W>::get(make_uint4(v.x, v.y, 0u, 0u), g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = g[i];
+    }
+}
+
+// Rows whose 16-byte vectors are whole and aligned, one per CTA, kept in registers (NV vectors
+// per thread), so that every byte crosses memory once. The squares are added in 64 bits. The
+// maximum is found in fp32, its exact value among the few products that are within rounding
+// of it, and q from fp32 except next to a border. A row whose fp32 maximum says nothing
+// (NaN, overflow, subnormal) is done again in 64 bits.
+template <typename T, typename W, int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT) rms_norm_i8_rows_kernel(const __grid_constant__ NormI8Args p) {
+    constexpr int N = Pack<T>::N;
+    __shared__ unsigned long long s_top;
+    const int64_t row = blockIdx.x;
+    const int nv = p.dim / N;
+    const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + row * p.x_stride);
+    const W* w = static_cast<const W*>(p.weight);
+    uint4 h[NV];
+    float t[NV][N];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int v = threadIdx.x + j * blockDim.x;
+        h[j] = v < nv ? x[v] : make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (p.residual) {
+        const uint4* r = reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + row * p.residual_stride);
+        uint4 add[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int v = threadIdx.x + j * blockDim.x;
+            add[j] = v < nv ? r[v] : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float a[N], b[N];
+            Pack<T>::get(h[j], a);
+            Pack<T>::get(add[j], b);
+#pragma unroll
+            for (int i = 0; i < N; ++i) a[i] += b[i];
+            h[j] = Pack<T>::put(a);
+        }
+    }
+    if (p.hidden) {
+        uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.hidden) + row * p.hidden_stride);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int v = threadIdx.x + j * blockDim.x;
+            if (v < nv) out[v] = h[j];
+        }
+    }
+    double sum = 0.0;
+    float most = 0.0f, check = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int v = threadIdx.x + j * blockDim.x;
+        float a[N], b[N];
+        Pack<T>::get(h[j], a);
+#pragma unroll
+        for (int i = 0; i < N; ++i) b[i] = 0.0f;
+        if (v < nv) get_weights<W, N>(w + v * N, b);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            t[j][i] = a[i] * b[i];
+            most = fmaxf(most, fabsf(t[j][i]));
+            check += t[j][i] * 0.0f;  // NaN where a product is NaN or infinite
+            sum += (double)a[i] * (double)a[i];
+        }
+    }
+    if (!(check == 0.0f)) most = INFINITY;
+    if (threadIdx.x == 0) s_top = 0ull;
+    block_sum_max(sum, most);
+    if (!(most >= 1e-30f && most < 1e38f && sum < DBL_MAX)) {
+        // (The block is of one mind here.) h is in p.hidden, or the inputs are as they were.
+        __syncthreads();
+        norm_row<T, W>(p, row, p.hidden != nullptr);
+        return;
+    }
+    if (blockDim.x == 32) __syncwarp();
+    // The exact maximum: a product is off by 2^-24 relative in fp32.
+    const float near = most * 0.9999996f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(t[j][i]));
+        if (m >= near) {
+            float a[N], b[N];
+            Pack<T>::get(h[j], a);
+            get_weights<W, N>(w + (threadIdx.x + j * blockDim.x) * N, b);
+            double d = 0.0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) d = fmax(d, fabs((double)a[i] * (double)b[i]));
+            atomicMax(&s_top, (unsigned long long)__double_as_longlong(d));
+        }
+    }
+    __syncthreads();
+    const double top = __longlong_as_double((long long)s_top);
+    if (threadIdx.x == 0) p.scale[row] = (float)(top / 127.0 * (1.0 / sqrt(sum / p.dim + (double)p.eps)));
+    const float f = (float)(127.0 / top);
+    int8_t* q = p.q + row * p.q_stride;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int v = threadIdx.x + j * blockDim.x;
+        if (v >= nv) break;
+        uint32_t word[N / 4];
+        bool sure = true;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            int k;
+            sure &= quick_quantum(t[j][i], f, &k);
+            if (i % 4 == 0) word[i / 4] = 0u;
+            word[i / 4] |= (uint32_t)(k & 0xFF) << (8 * (i % 4));
+        }
+        if (!sure) {
+            float a[N], b[N];
+            Pack<T>::get(h[j], a);
+            get_weights<W, N>(w + v * N, b);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const uint32_t k = (uint32_t)(quantum((double)a[i] * (double)b[i], top) & 0xFF);
+                word[i / 4] = (word[i / 4] & ~(0xFFu << (8 * (i % 4)))) | k << (8 * (i % 4));
+            }
+        }
+        if constexpr (N == 8) reinterpret_cast<uint2*>(q)[v] = make_uint2(word[0], word[1]);
+        else reinterpret_cast<uint32_t*>(q)[v] = word[0];
+    }
 }
 
 struct F32Rows {
@@ -130,11 +335,29 @@ __global__ void __launch_bounds__(kNormThreads) quantise_rows_kernel(S src, I8Ma
 
 template <typename T, typename W>
 cudaError_t launch_norm(const NormI8Args& a, cudaStream_t stream) {
-    const size_t smem = (size_t)a.dim * sizeof(T);
-    static SmemLimit limit;
-    cudaError_t e = limit.raise(rms_norm_i8_kernel<T, W>, smem);
-    if (e != cudaSuccess) return e;
-    rms_norm_i8_kernel<T, W><<<a.rows, kNormThreads, smem, stream>>>(a);
+    constexpr int N = Pack<T>::N;
+    auto whole = [](const void* p, int64_t stride, size_t size, size_t to) {
+        return (uintptr_t)p % to == 0 && (uint64_t)stride * size % to == 0;
+    };
+    // Whole aligned vectors of every row; a lone row needs its base alone.
+    const int64_t one = a.rows > 1;
+    const bool rows = a.dim % N == 0 && whole(a.x, one * a.x_stride, sizeof(T), 16) &&
+                      whole(a.residual, one * a.residual_stride, sizeof(T), 16) &&
+                      whole(a.hidden, one * a.hidden_stride, sizeof(T), 16) && whole(a.q, one * a.q_stride, 1, N) &&
+                      (uintptr_t)a.weight % 16 == 0;
+    if (!rows) {
+        rms_norm_i8_kernel<T, W><<<a.rows, kNormThreads, 0, stream>>>(a);
+        return cudaGetLastError();
+    }
+    // Many rows: 32 elements a thread, so that a row takes few threads and many rows are on their
+    // way. Few rows, or short ones: one vector a thread.
+    constexpr int kMost = 32 / N;
+    const int nv = a.dim / N;
+    const int per = nv > 1024 || (a.rows > 148 && nv > 64) ? kMost : 1;
+    const int threads = ((nv + per - 1) / per + 31) / 32 * 32;
+    if (per == 1) rms_norm_i8_rows_kernel<T, W, 1, 1024><<<a.rows, threads, 0, stream>>>(a);
+    else if (threads <= 256) rms_norm_i8_rows_kernel<T, W, kMost, 256><<<a.rows, threads, 0, stream>>>(a);
+    else rms_norm_i8_rows_kernel<T, W, kMost, 1024><<<a.rows, threads, 0, stream>>>(a);
     return cudaGetLastError();
 }
 

@@ -61,25 +61,35 @@ def _hidden_code(t, what: str) -> int:
     return code
 
 
+_raw_stream = None
+
+
 def _stream_on(device: int, stream) -> int:
     """The stream of a call on `device`: the given one, or the device's current one."""
-    import torch
-    return (torch.cuda.current_stream(device) if stream is None else stream).cuda_stream
+    global _raw_stream
+    if stream is not None:
+        return stream.cuda_stream
+    if _raw_stream is None:
+        import torch
+        # The handle of current_stream(device) without the object around it (1.3 us a call).
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
 
 
-def _empty(shape, dtype, device, stream):
-    """An output. With a stream of the caller's it is allocated under that one, so that its memory
-    is reused in that stream's order."""
-    import torch
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+def _output(like, shape, dtype, stream):
+    """An output on the device of `like`. With a stream of the caller's it is allocated under that
+    one, so that its memory is reused in that stream's order."""
+    if stream is not None:
+        import torch
+        with torch.cuda.stream(stream):
+            return like.new_empty(shape, dtype=dtype)
+    # Without the keyword the call takes half the time.
+    return like.new_empty(shape) if like.dtype is dtype else like.new_empty(shape, dtype=dtype)
 
 
-def _need(t, what: str, device: int, dtype=None, shape=None, rows=False):
-    """Argument check of a device tensor: its device, type and shape; contiguous, or with
-    `rows` a matrix whose rows are contiguous."""
+def _need(t, what: str, device: int, dtype, shape):
+    """Checks a contiguous tensor's device, type and shape (dtype or shape None: any)."""
     if t.get_device() != device:
         raise ValueError(f"{what} must be a tensor on cuda:{device}, got {t.device}")
     if dtype is not None and t.dtype is not dtype:
@@ -87,19 +97,22 @@ def _need(t, what: str, device: int, dtype=None, shape=None, rows=False):
     if shape is not None and t.shape != shape:
         raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if not t.is_contiguous():
-        if not rows:
-            raise ValueError(f"{what} must be contiguous")
-        if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-            raise ValueError(f"{what} must be a matrix with contiguous rows")
-    elif rows and t.dim() != 2:
+        raise ValueError(f"{what} must be contiguous")
+
+
+def _matrix(t, what: str, device: int, dtype, shape) -> int:
+    """Checks a matrix with contiguous rows (dtype None: any); returns the elements between its
+    rows (a lone row's stride says nothing)."""
+    if t.get_device() != device:
+        raise ValueError(f"{what} must be a tensor on cuda:{device}, got {t.device}")
+    if dtype is not None and t.dtype is not dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    stride = t.stride()
+    if len(stride) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError(f"{what} must be a matrix with contiguous rows")
-    return t
-
-
-def _pitch(t) -> int:
-    """Elements between the rows of a matrix (a lone row's stride says nothing)."""
-    rows, width = t.shape
-    return t.stride(0) if rows > 1 else max(t.stride(0), width)
+    return stride[0] if shape[0] > 1 else max(stride[0], shape[1])
 
 
 class SamplerContext:
@@ -186,32 +199,32 @@ class SamplerContext:
         ``x`` or ``residual`` for an update in place. A ``q`` made here has rows padded to a
         multiple of 16 bytes, as ``I8Weights.unembed`` takes it."""
         import torch
-        dev, code, wcode = self.device, _hidden_code(x, "x"), _hidden_code(weight, "weight")
-        _need(x, "x", dev, rows=True)
-        shape = x.shape
+        dev, dtype, shape = self.device, x.dtype, x.shape
+        code, wcode = _hidden_code(x, "x"), _hidden_code(weight, "weight")
+        pitch = _matrix(x, "x", dev, None, shape)
         rows, dim = shape
         _need(weight, "weight", dev, None, (dim,))
+        rp = hp = 0
         if residual is not None:
-            _need(residual, "residual", dev, x.dtype, shape, True)
+            rp = _matrix(residual, "residual", dev, dtype, shape)
             if out_hidden is None:
-                out_hidden = _empty(shape, x.dtype, x.device, stream)
-        if out_hidden is not None:
-            _need(out_hidden, "out_hidden", dev, x.dtype, shape, True)
+                out_hidden, hp = _output(x, shape, dtype, stream), dim
+        if out_hidden is not None and not hp:
+            hp = _matrix(out_hidden, "out_hidden", dev, dtype, shape)
         if q is None:
-            room = -(-dim // 16) * 16
-            q = _empty((rows, room), torch.int8, x.device, stream)
-            if room != dim:
+            qp = -(-dim // 16) * 16
+            q = _output(x, (rows, qp), torch.int8, stream)
+            if qp != dim:
                 q = q[:, :dim]
         else:
-            _need(q, "q", dev, torch.int8, shape, True)
+            qp = _matrix(q, "q", dev, torch.int8, shape)
         if scale is None:
-            scale = _empty(rows, torch.float32, x.device, stream)
+            scale = _output(weight, rows, torch.float32, stream)
         else:
             _need(scale, "scale", dev, torch.float32, (rows,))
-        rc = self.lib.vdxs_rms_norm_i8(self._h, _ptr(x), _pitch(x), _ptr(residual),
-                                       0 if residual is None else _pitch(residual), code, _ptr(weight), wcode, rows, dim,
-                                       eps, _ptr(out_hidden), 0 if out_hidden is None else _pitch(out_hidden), _ptr(q),
-                                       _pitch(q), _ptr(scale), _stream_on(dev, stream))
+        rc = self.lib.vdxs_rms_norm_i8(self._h, x.data_ptr(), pitch, _ptr(residual), rp, code, weight.data_ptr(), wcode,
+                                       rows, dim, eps, _ptr(out_hidden), hp, q.data_ptr(), qp, scale.data_ptr(),
+                                       _stream_on(dev, stream))
         if rc:
             check(rc, self._h)
         return q, scale, out_hidden
@@ -522,19 +535,19 @@ class I8Weights:
                    torch.int8: abi.WEIGHTS_I8}
         if weight.dtype not in formats:
             raise TypeError(f"weight must be int8, float32, bfloat16 or float16, got {weight.dtype}")
-        _need(weight, "weight", ctx.device, rows=True)
+        pitch = _matrix(weight, "weight", ctx.device, None, weight.shape)
         out_dim, in_dim = weight.shape
         if (weight.dtype == torch.int8) != (scales is not None):
             raise ValueError("scales go with int8 weights, and with those alone")
         if scales is not None:
             _need(scales, "scales", ctx.device, torch.float32, (out_dim,))
-        self._prepare(ctx, weight, formats[weight.dtype], scales, _pitch(weight), in_dim, out_dim, stream)
+        self._prepare(ctx, weight, formats[weight.dtype], scales, pitch, in_dim, out_dim, stream)
 
     @classmethod
     def from_q4_0(cls, ctx: SamplerContext, q4_0, in_dim: int, out_dim: int, stream=None) -> "I8Weights":
         """From the reference's Q4_0 blocks (the uint8 tensor that Q4Weights takes)."""
         import torch
-        _need(q4_0, "q4_0", ctx.device, torch.uint8)
+        _need(q4_0, "q4_0", ctx.device, torch.uint8, None)
         if q4_0.numel() != out_dim * (in_dim // 32) * 18:
             raise ValueError(f"{q4_0.numel()} bytes are not {out_dim} x {in_dim} in Q4_0 blocks")
         w = cls.__new__(cls)
@@ -564,21 +577,17 @@ class I8Weights:
         """logits [batch, out_dim] (float32 or bfloat16) of 8-bit rows ``q`` [batch, in_dim] with
         ``scale`` [batch], as SamplerContext.rms_norm_i8 returns them."""
         import torch
-        dev = self.ctx.device
-        _need(q, "q", dev, torch.int8, None, True)
-        batch, width = q.shape
-        if width != self.in_dim:
-            raise ValueError(f"q must have {self.in_dim} columns, got {width}")
+        dev, batch, n = self.ctx.device, q.shape[0], self.out_dim
+        qp = _matrix(q, "q", dev, torch.int8, (batch, self.in_dim))
+        if batch == 1:
+            qp = -(-self.in_dim // 16) * 16
         _need(scale, "scale", dev, torch.float32, (batch,))
         if logits is None:
-            logits = _empty((batch, self.out_dim), dtype or torch.float32, q.device, stream)
-            pitch = self.out_dim
+            logits, pitch = _output(scale, (batch, n), dtype or torch.float32, stream), n
         else:
-            _need(logits, "logits", dev, dtype, (batch, self.out_dim), True)
-            pitch = _pitch(logits)
-        rc = self.lib.vdxs_unembed_i8(self.ctx._h, self._h, _ptr(q),
-                                      q.stride(0) if batch > 1 else -(-width // 16) * 16, _ptr(scale), batch,
-                                      _ptr(logits), _dtype_code(logits), pitch, _stream_on(dev, stream))
+            pitch = _matrix(logits, "logits", dev, dtype, (batch, n))
+        rc = self.lib.vdxs_unembed_i8(self.ctx._h, self._h, q.data_ptr(), qp, scale.data_ptr(), batch, logits.data_ptr(),
+                                      _dtype_code(logits), pitch, _stream_on(dev, stream))
         if rc:
             check(rc, self.ctx._h)
         return logits
@@ -587,30 +596,26 @@ class I8Weights:
                history=None, history_count=None, tokens=None, stream=None):
         """vdxs_sample_unembed_i8: norm, unembedding and sampling in one call; returns tokens."""
         import torch
-        dev = self.ctx.device
+        dev, batch = self.ctx.device, x.shape[0]
+        shape = (batch, self.in_dim)
         code, wcode = _hidden_code(x, "x"), _hidden_code(norm_weight, "norm_weight")
-        _need(x, "x", dev, None, (x.shape[0], self.in_dim), True)
+        pitch = _matrix(x, "x", dev, None, shape)
+        rp = 0 if residual is None else _matrix(residual, "residual", dev, x.dtype, shape)
+        hp = 0 if out_hidden is None else _matrix(out_hidden, "out_hidden", dev, x.dtype, shape)
         _need(norm_weight, "norm_weight", dev, None, (self.in_dim,))
-        for t, what in ((residual, "residual"), (out_hidden, "out_hidden")):
-            if t is not None:
-                _need(t, what, dev, x.dtype, x.shape, True)
-        batch = x.shape[0]
         if tokens is None:
-            tokens = _empty(batch, torch.int32, x.device, stream)
-        for t, what, dtype, shape in ((uniforms, "uniforms", torch.float32, (batch,)),
-                                      (history_count, "history_count", torch.int32, (batch,)),
-                                      (tokens, "tokens", torch.int32, (batch,))):
+            tokens = _output(x, batch, torch.int32, stream)
+        for t, what, dtype in ((uniforms, "uniforms", torch.float32), (history_count, "history_count", torch.int32),
+                               (tokens, "tokens", torch.int32)):
             if t is not None:
-                _need(t, what, dev, dtype, shape)
+                _need(t, what, dev, dtype, (batch,))
         hs = 1
         if history is not None:
-            _need(history, "history", dev, torch.int32, (batch, history.shape[1]))
             hs = history.shape[1]
-        check(self.lib.vdxs_sample_unembed_i8(self.ctx._h, C.byref(cfg), self._h, _ptr(x), _pitch(x), _ptr(residual),
-                                              0 if residual is None else _pitch(residual), code, _ptr(norm_weight),
-                                              wcode, eps, _ptr(out_hidden),
-                                              0 if out_hidden is None else _pitch(out_hidden), batch, _ptr(history), hs,
-                                              _ptr(history_count), _ptr(uniforms), _ptr(tokens),
+            _need(history, "history", dev, torch.int32, (batch, hs))
+        check(self.lib.vdxs_sample_unembed_i8(self.ctx._h, C.byref(cfg), self._h, x.data_ptr(), pitch, _ptr(residual), rp,
+                                              code, norm_weight.data_ptr(), wcode, eps, _ptr(out_hidden), hp, batch,
+                                              _ptr(history), hs, _ptr(history_count), _ptr(uniforms), tokens.data_ptr(),
                                               _stream_on(dev, stream)), self.ctx._h)
         return tokens
 
@@ -634,7 +639,8 @@ class BeamState:
         def own(t, dtype, *shape):
             if t is None:
                 return torch.zeros(shape, dtype=dtype, device=device)
-            return _need(t, "state", device.index, dtype, shape)
+            _need(t, "state", device.index, dtype, shape)
+            return t
 
         if scores is None:
             scores = torch.full((batch, beams), -float("inf"), dtype=torch.float32, device=device)
@@ -735,37 +741,41 @@ class BeamSearch:
         """One step (vdxs_beam_step): (tokens, parents) as int32 [batch, beams]. ``out`` receives the
         rows after it (``state`` itself, in place, when None)."""
         import torch
-        dev, rows, shape = self.ctx.device, self.batch * self.beams, (self.batch, self.beams)
-        out = state if out is None else out
-        _need(logits, "logits", dev, None, (rows, self.vocab), True)
-        for s in (state, out):
-            if s.batch != self.batch or s.beams != self.beams or s.window != state.window:
-                raise ValueError(f"a state of {s.batch} x {s.beams}, window {s.window}, for a search of {self.batch} x "
-                                 f"{self.beams}, window {state.window}")
-            if s.scores.get_device() != dev:
-                raise ValueError(f"the state is on {s.scores.device}, the search on cuda:{dev}")
+        dev, batch, beams, i32 = self.ctx.device, self.batch, self.beams, torch.int32
+        shape = (batch, beams)
+        pitch = _matrix(logits, "logits", dev, None, (batch * beams, self.vocab))
+        self._check_state(state, state.window)
+        a = b = state.rows()
+        if out is not None and out is not state:
+            self._check_state(out, state.window)
+            b = out.rows()
         n_stop = 0
         if stop_ids is not None:
-            _need(stop_ids, "stop_ids", dev, torch.int32)
+            _need(stop_ids, "stop_ids", dev, i32, None)
             n_stop = stop_ids.numel()
         if tokens is None:
-            tokens = _empty(shape, torch.int32, logits.device, stream)
+            tokens = _output(state.finished, shape, i32, stream)
         else:
-            _need(tokens, "tokens", dev, torch.int32, shape)
+            _need(tokens, "tokens", dev, i32, shape)
         if parents is None:
-            parents = _empty(shape, torch.int32, logits.device, stream)
+            parents = _output(state.finished, shape, i32, stream)
         else:
-            _need(parents, "parents", dev, torch.int32, shape)
+            _need(parents, "parents", dev, i32, shape)
         cfg = abi.VdxsBeamConfig(length_alpha, repeat_penalty, state.window, pad_token, 0)
-        a = state.rows()
-        b = a if out is state else out.rows()
-        moved, n = self._caches(caches)
-        rc = self.lib.vdxs_beam_step(self._h, C.byref(cfg), _ptr(logits), _dtype_code(logits), _pitch(logits), C.byref(a),
-                                     C.byref(b), _ptr(stop_ids), n_stop, moved, n, _ptr(tokens), _ptr(parents),
+        moved, n = self._caches(caches) if caches else (None, 0)
+        rc = self.lib.vdxs_beam_step(self._h, C.byref(cfg), logits.data_ptr(), _dtype_code(logits), pitch, C.byref(a),
+                                     C.byref(b), _ptr(stop_ids), n_stop, moved, n, tokens.data_ptr(), parents.data_ptr(),
                                      _stream_on(dev, stream))
         if rc:
             check(rc, self.ctx._h)
         return tokens, parents
+
+    def _check_state(self, s: BeamState, window: int):
+        if s.batch != self.batch or s.beams != self.beams or s.window != window:
+            raise ValueError(f"a state of {s.batch} x {s.beams}, window {s.window}, for a search of {self.batch} x "
+                             f"{self.beams}, window {window}")
+        if s.scores.get_device() != self.ctx.device:
+            raise ValueError(f"the state is on {s.scores.device}, the search on cuda:{self.ctx.device}")
 
     def reorder(self, parents, caches, stream=None):
         """Moves caches by a step's parents (vdxs_beam_reorder)."""
