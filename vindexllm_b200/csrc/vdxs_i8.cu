@@ -56,9 +56,10 @@ __device__ __forceinline__ int quantum(double t, double top) { return (int)rint(
 // each (2^-24 relative), so v is off by at most 127 * 3 * 2^-24 = 2.3e-5; a v that is 1e-4 from
 // a border rounds as the exact quotient does. Else (one value in 5000) false.
 __device__ __forceinline__ bool quick_quantum(float t32, float f, int* q) {
-    const float v = t32 * f, r = rintf(v);
-    *q = (int)r;
-    return fabsf(v - r) <= 0.4999f;
+    // Adding 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low bits.
+    const float v = t32 * f, r = __fadd_rn(v, 12582912.0f);
+    *q = __float_as_int(r) - 0x4B400000;
+    return fabsf(v - __fadd_rn(r, -12582912.0f)) <= 0.4999f;
 }
 
 // A row in 64 bits throughout. `done`: h is in p.hidden (or is x itself) already.
@@ -168,7 +169,7 @@ __device__ __forceinline__ void get_weights(const W* p, float* f) {
 // of it, and q from fp32 except next to a border. A row whose fp32 maximum says nothing
 // (NaN, overflow, subnormal) is done again in 64 bits.
 template <typename T, typename W, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT) rms_norm_i8_rows_kernel(const __grid_constant__ NormI8Args p) {
+__global__ void __launch_bounds__(MAXT, 1024 / MAXT) rms_norm_i8_rows_kernel(const __grid_constant__ NormI8Args p) {
     constexpr int N = Pack<T>::N;
     __shared__ unsigned long long s_top;
     const int64_t row = blockIdx.x;
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(MAXT) rms_norm_i8_rows_kernel(const __grid_con
     const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + row * p.x_stride);
     const W* w = static_cast<const W*>(p.weight);
     uint4 h[NV];
-    float t[NV][N];
+    float largest[NV];  // of each vector's products
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int v = threadIdx.x + j * blockDim.x;
@@ -218,13 +219,15 @@ __global__ void __launch_bounds__(MAXT) rms_norm_i8_rows_kernel(const __grid_con
 #pragma unroll
         for (int i = 0; i < N; ++i) b[i] = 0.0f;
         if (v < nv) get_weights<W, N>(w + v * N, b);
+        largest[j] = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            t[j][i] = a[i] * b[i];
-            most = fmaxf(most, fabsf(t[j][i]));
-            check += t[j][i] * 0.0f;  // NaN where a product is NaN or infinite
+            const float t = a[i] * b[i];
+            largest[j] = fmaxf(largest[j], fabsf(t));
+            check += t * 0.0f;  // NaN where a product is NaN or infinite
             sum += (double)a[i] * (double)a[i];
         }
+        most = fmaxf(most, largest[j]);
     }
     if (!(check == 0.0f)) most = INFINITY;
     if (threadIdx.x == 0) s_top = 0ull;
@@ -240,10 +243,7 @@ __global__ void __launch_bounds__(MAXT) rms_norm_i8_rows_kernel(const __grid_con
     const float near = most * 0.9999996f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        float m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(t[j][i]));
-        if (m >= near) {
+        if (largest[j] >= near) {
             float a[N], b[N];
             Pack<T>::get(h[j], a);
             get_weights<W, N>(w + (threadIdx.x + j * blockDim.x) * N, b);
@@ -264,17 +264,17 @@ __global__ void __launch_bounds__(MAXT) rms_norm_i8_rows_kernel(const __grid_con
         if (v >= nv) break;
         uint32_t word[N / 4];
         bool sure = true;
+        float a[N], b[N];
+        Pack<T>::get(h[j], a);
+        get_weights<W, N>(w + v * N, b);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             int k;
-            sure &= quick_quantum(t[j][i], f, &k);
+            sure &= quick_quantum(a[i] * b[i], f, &k);
             if (i % 4 == 0) word[i / 4] = 0u;
             word[i / 4] |= (uint32_t)(k & 0xFF) << (8 * (i % 4));
         }
         if (!sure) {
-            float a[N], b[N];
-            Pack<T>::get(h[j], a);
-            get_weights<W, N>(w + v * N, b);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const uint32_t k = (uint32_t)(quantum((double)a[i] * (double)b[i], top) & 0xFF);
