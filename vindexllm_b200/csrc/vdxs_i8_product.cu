@@ -52,43 +52,67 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
                  : "memory");
     return done != 0u;
 }
-// Waits for a phase, at most about two seconds (false: gave up).
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity) {
-    if (bar_try(bar, parity)) return true;
+// Waits for a phase, at most about two seconds; `good` turns false when it gives up, and later
+// waits return at once. No branch of the caller hangs on the outcome, so a warp that waits
+// together stays together.
+__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, bool& good) {
+    if (bar_try(bar, parity) || !good) return;
     uint64_t t0, t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
     for (;;) {
         for (int i = 0; i < 64; ++i)
-            if (bar_try(bar, parity)) return true;
+            if (bar_try(bar, parity)) return;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-        if (t - t0 > 2000000000ull) return false;
+        if (t - t0 > 2000000000ull) break;
     }
+    good = false;
+}
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t e;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+    return e;
 }
 
-__device__ __forceinline__ void copy_tile(const CUtensorMap* map, void* dst, int x, int y, uint64_t* bar) {
+// Instructions that one thread issues run with the whole warp converged and a predicate that
+// holds in one lane (`one`): their operands then stay in uniform registers. Issued from a
+// branch of a single lane, each product took 125 cycles of the issuing thread.
+__device__ __forceinline__ void copy_tile(uint32_t one, const CUtensorMap* map, uint32_t dst, int x, int y,
+                                          uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            smem_addr(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
+        "{\n .reg .pred q;\n setp.ne.u32 q, %5, 0;\n"
+        " @q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];\n}" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t one, uint32_t bar, uint32_t bytes) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %2, 0;\n @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(
+            bar),
+        "r"(bytes), "r"(one)
         : "memory");
 }
 
-// Shared-memory operand: rows of 128 bytes, 128-byte swizzle, 8 rows (1024 bytes) to a group.
-__device__ __forceinline__ uint64_t operand(const void* p) {
-    return (uint64_t)((smem_addr(p) & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// Shared-memory operand at an address: rows of 128 bytes, 128-byte swizzle, 8 rows (1024 bytes)
+// to a group.
+__device__ __forceinline__ uint64_t operand(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
 }
 
-__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_i8(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
         : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
+__device__ __forceinline__ void mma_commit(uint32_t one, uint32_t bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar),
+        "r"(one)
+        : "memory");
 }
 __device__ __forceinline__ void load16(uint32_t addr, uint32_t* v) {
     asm volatile(
@@ -147,54 +171,60 @@ __global__ void __launch_bounds__(kThreadsP, 1)
 
     bool good = true;
     if (warp == 0) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t phase = 0;
-            int issued = 0;  // stages with a copy that nobody has waited for, should a wait give up
-            for (int64_t t = blockIdx.x; good && t < p.tiles; t += gridDim.x) {
-                const int m = (int)(t / p.n_tiles), n = (int)(t - (int64_t)m * p.n_tiles);
-                for (int c = 0; c < chunks; ++c) {
-                    if (!(good = bar_wait(&empty[s], phase ^ 1))) break;
-                    unsigned char* a = stages + s * stage_bytes;
-                    bar_expect(&full[s], stage_bytes);
-                    copy_tile(&map_w, a, c * kChunkK, m * kTileM, &full[s]);
-                    copy_tile(&map_q, a + kStageBytesA, c * kChunkK, n * p.n, &full[s]);
-                    issued = min(issued + 1, p.stages);
-                    if (++s == p.stages) s = 0, phase ^= 1;
-                }
-            }
-            // The copies in flight land before the CTA may end.
-            if (!good)
-                for (; issued > 0; --issued) {
-                    if (--s < 0) s = p.stages - 1, phase ^= 1;
-                    bar_wait(&full[s], phase);
-                }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            // D: 32-bit integers; A, B: signed 8 bits, K-major.
-            const uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(p.n >> 3) << 17 | (uint32_t)(kTileM >> 4) << 24;
-            int s = 0, acc = 0;
-            uint32_t phase = 0, acc_phase = 0;
-            for (int64_t t = blockIdx.x; good && t < p.tiles; t += gridDim.x) {
-                if (!(good = bar_wait(&acc_empty[acc], acc_phase ^ 1))) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t d = tmem + acc * (p.columns >> 1);
-                for (int c = 0; c < chunks; ++c) {
-                    if (!(good = bar_wait(&full[s], phase))) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t a = operand(stages + s * stage_bytes);
-                    const uint64_t b = operand(stages + s * stage_bytes + kStageBytesA);
-                    // What lies behind in_dim is zero in shared memory; whole steps of it are left out.
-                    const int steps = min(4, (p.in_dim - c * kChunkK + 31) / 32);
-                    for (int k = 0; k < steps; ++k) mma_i8(d, a + 2 * k, b + 2 * k, idesc, c > 0 || k > 0);
-                    mma_commit(&empty[s]);
-                    if (++s == p.stages) s = 0, phase ^= 1;
-                }
+        const uint32_t one = elect_one();
+        const uint32_t base = smem_addr(stages), full0 = smem_addr(full);
+        int s = 0, issued = 0;
+        uint32_t phase = 0;
+        for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
+            const int m = (int)(t / p.n_tiles), n = (int)(t - (int64_t)m * p.n_tiles);
+            for (int c = 0; c < chunks; ++c) {
+                bar_wait(&empty[s], phase ^ 1, good);
                 if (!good) break;
-                mma_commit(&acc_full[acc]);
-                if (++acc == 2) acc = 0, acc_phase ^= 1;
+                const uint32_t a = base + s * stage_bytes, bar = full0 + 8 * s;
+                bar_expect(one, bar, stage_bytes);
+                copy_tile(one, &map_w, a, c * kChunkK, m * kTileM, bar);
+                copy_tile(one, &map_q, a + kStageBytesA, c * kChunkK, n * p.n, bar);
+                issued = min(issued + 1, p.stages);
+                if (++s == p.stages) s = 0, phase ^= 1;
             }
+            if (!good) break;
+        }
+        // Should a wait have given up: the copies in flight land before the CTA may end.
+        if (!good)
+            for (; issued > 0; --issued) {
+                if (--s < 0) s = p.stages - 1, phase ^= 1;
+                bool again = true;
+                bar_wait(&full[s], phase, again);
+            }
+    } else if (warp == 1) {
+        // D: 32-bit integers; A, B: signed 8 bits, K-major.
+        const uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(p.n >> 3) << 17 | (uint32_t)(kTileM >> 4) << 24;
+        const uint32_t one = elect_one();
+        const uint32_t empty0 = smem_addr(empty), base = smem_addr(stages);
+        // What lies behind in_dim is zero in shared memory; whole steps of it are left out.
+        const int last = (p.in_dim - (chunks - 1) * kChunkK + 31) / 32;
+        int s = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
+            bar_wait(&acc_empty[acc], acc_phase ^ 1, good);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t d = tmem + acc * (p.columns >> 1);
+            for (int c = 0; c < chunks; ++c) {
+                bar_wait(&full[s], phase, good);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t a = operand(base + s * stage_bytes);
+                const uint64_t b = operand(base + s * stage_bytes + kStageBytesA);
+                if (c + 1 < chunks || last == 4) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_i8(one, d, a + 2 * k, b + 2 * k, idesc, (uint32_t)(c | k));
+                } else {
+                    for (int k = 0; k < last; ++k) mma_i8(one, d, a + 2 * k, b + 2 * k, idesc, (uint32_t)(c | k));
+                }
+                mma_commit(one, empty0 + 8 * s);
+                if (++s == p.stages) s = 0, phase ^= 1;
+            }
+            mma_commit(one, smem_addr(&acc_full[acc]));
+            if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
     } else {
         const int quad = warp & 3;  // the tensor memory lanes that this warp may read
@@ -205,7 +235,8 @@ __global__ void __launch_bounds__(kThreadsP, 1)
             const int64_t row = (int64_t)m * kTileM + quad * 32 + lane;
             const bool have = row < p.out_dim;
             const float ws = have ? __ldg(p.w_scale + row) : 0.0f;
-            if (!(good = __all_sync(0xFFFFFFFFu, bar_wait(&acc_full[acc], acc_phase)))) break;
+            bar_wait(&acc_full[acc], acc_phase, good);
+            if (!__all_sync(0xFFFFFFFFu, good)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t src = tmem + acc * (p.columns >> 1) + ((uint32_t)quad * 32 << 16);
             const int b0 = n * p.n;
