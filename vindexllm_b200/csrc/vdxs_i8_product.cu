@@ -7,8 +7,12 @@
 // neighbouring vocabulary entries, so the logits go out as whole 128-byte lines without a
 // stop in shared memory.
 //
-// One persistent CTA per SM, six warps: warp 0 copies 128-byte wide tiles of both operands
-// into a ring of stages (TMA, 128-byte swizzle), warp 1 issues the products, warps 2 to 5
+// Batches above 128 use pairs of CTAs: one product then spans both SMs of a pair (256 vocabulary
+// entries, 128 to a CTA) and each CTA holds half of the batch columns' rows, which halves what
+// the batch operand costs each SM in shared-memory fills.
+//
+// One persistent CTA per SM, ten warps: warp 0 copies 128-byte wide tiles of both operands
+// into a ring of stages (TMA, 128-byte swizzle), warp 1 issues the products, warps 2 to 9
 // scale and store one accumulator while the next tile is summed in the other one. Sums are
 // exact 32-bit integers; the two scales are applied in fp32.
 #include "vdxs_internal.h"
@@ -24,13 +28,17 @@
 namespace vdxs {
 namespace {
 
-constexpr int kThreadsP = 192;
+constexpr int kEpiWarps = 8;         // two for each quarter of the accumulator's rows
+constexpr int kThreadsP = 64 + 32 * kEpiWarps;
 constexpr int kTileM = 128;          // vocabulary entries of a tile
 constexpr int kChunkK = 128;         // bytes of a row in a stage: one swizzle span
 constexpr int kMaxN = 256;           // batch columns of a tile
 constexpr int kMaxStages = 12;
 constexpr int kStageBytesA = kTileM * kChunkK;
 constexpr int kSmemBudget = 220 * 1024;
+#ifndef VDXS_PAIR
+#define VDXS_PAIR 128
+#endif
 constexpr int32_t kErrTimeout = 3;   // the context's device error word: a bounded wait gave up
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -52,16 +60,28 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
                  : "memory");
     return done != 0u;
 }
+__device__ __forceinline__ bool bar_try_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, "
+        "p;\n}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return done != 0u;
+}
 // Waits for a phase, at most about two seconds; `good` turns false when it gives up, and later
 // waits return at once. No branch of the caller hangs on the outcome, so a warp that waits
 // together stays together.
+template <bool CLUSTER = false>
 __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, bool& good) {
-    if (bar_try(bar, parity) || !good) return;
+    auto ready = [&] { return CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity); };
+    if (ready() || !good) return;
     uint64_t t0, t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
     for (;;) {
         for (int i = 0; i < 64; ++i)
-            if (bar_try(bar, parity)) return;
+            if (ready()) return;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
         if (t - t0 > 2000000000ull) break;
     }
@@ -76,14 +96,24 @@ __device__ __forceinline__ uint32_t elect_one() {
 // Instructions that one thread issues run with the whole warp converged and a predicate that
 // holds in one lane (`one`): their operands then stay in uniform registers. Issued from a
 // branch of a single lane, each product took 125 cycles of the issuing thread.
+// `bar`: a barrier of this CTA, or with PAIR the address of one of the pair's first CTA.
+template <bool PAIR>
 __device__ __forceinline__ void copy_tile(uint32_t one, const CUtensorMap* map, uint32_t dst, int x, int y,
                                           uint32_t bar) {
-    asm volatile(
-        "{\n .reg .pred q;\n setp.ne.u32 q, %5, 0;\n"
-        " @q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];\n}" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar), "r"(one)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.u32 q, %5, 0;\n"
+            " @q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+            "[%1, {%2, %3}], [%4];\n}" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar), "r"(one)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.u32 q, %5, 0;\n"
+            " @q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+            "[%4];\n}" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(bar), "r"(one)
+            : "memory");
 }
 __device__ __forceinline__ void bar_expect(uint32_t one, uint32_t bar, uint32_t bytes) {
     asm volatile(
@@ -100,20 +130,48 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr) {
            (uint64_t)2 << 61;
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void mma_i8(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-    asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
-        " @q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+            " @q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+            " @q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(one)
+            : "memory");
 }
+// With PAIR the barrier at the same place in both CTAs is arrived at.
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint32_t one, uint32_t bar) {
-    asm volatile(
-        "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
-        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar),
-        "r"(one)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n .reg .pred q;\n .reg .b16 both;\n mov.b16 both, 3;\n setp.ne.u32 q, %1, 0;\n"
+            " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], "
+            "both;\n}" ::"r"(bar),
+            "r"(one)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+            " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar),
+            "r"(one)
+            : "memory");
 }
+// The address of this CTA's `addr` in the pair's first CTA.
+__device__ __forceinline__ uint32_t in_first(uint32_t addr) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+    return a;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ void load16(uint32_t addr, uint32_t* v) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
@@ -135,128 +193,162 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bf
 
 struct ProductParams {
     int in_dim, out_dim, batch, n, n_tiles, stages, columns;
-    int64_t tiles;  // vocabulary tiles * n_tiles
+    int64_t tiles;  // vocabulary tiles (of two CTAs, in pairs) * n_tiles
     const float *w_scale, *scale;
     void* logits;
     int64_t stride;
     int32_t* err;
 };
 
-template <typename O>
+template <typename O, bool PAIR>
 __global__ void __launch_bounds__(kThreadsP, 1)
     unembed_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q,
                       const ProductParams p) {
     extern __shared__ unsigned char raw[];
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_base;
+    __shared__ __align__(16) float scales[2][kMaxN];
     unsigned char* stages = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int stage_bytes = kStageBytesA + p.n * kChunkK;
+    constexpr int kCtas = PAIR ? 2 : 1;
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;  // in the pair
+    const int q_rows = p.n / kCtas;                     // batch rows that this CTA holds
+    const int stage_bytes = kStageBytesA + q_rows * kChunkK;
     const int chunks = (p.in_dim + kChunkK - 1) / kChunkK;
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) bar_init(&full[i], 1), bar_init(&empty[i], 1);
-        for (int i = 0; i < 2; ++i) bar_init(&acc_full[i], 1), bar_init(&acc_empty[i], 4);
+        for (int i = 0; i < 2; ++i) bar_init(&acc_full[i], 1), bar_init(&acc_empty[i], kEpiWarps * kCtas);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
-                     "r"(p.columns)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                         "r"(p.columns)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                         "r"(p.columns)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_base;
 
     bool good = true;
     if (warp == 0) {
         const uint32_t one = elect_one();
-        const uint32_t base = smem_addr(stages), full0 = smem_addr(full);
+        const uint32_t base = smem_addr(stages), mine0 = smem_addr(full), full0 = PAIR ? in_first(mine0) : mine0;
         int s = 0, issued = 0;
         uint32_t phase = 0;
-        for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
+        for (int64_t t = blockIdx.x / kCtas; t < p.tiles; t += gridDim.x / kCtas) {
             const int m = (int)(t / p.n_tiles), n = (int)(t - (int64_t)m * p.n_tiles);
             for (int c = 0; c < chunks; ++c) {
                 bar_wait(&empty[s], phase ^ 1, good);
                 if (!good) break;
+                // A pair's stages are counted together by its first CTA.
                 const uint32_t a = base + s * stage_bytes, bar = full0 + 8 * s;
-                bar_expect(one, bar, stage_bytes);
-                copy_tile(one, &map_w, a, c * kChunkK, m * kTileM, bar);
-                copy_tile(one, &map_q, a + kStageBytesA, c * kChunkK, n * p.n, bar);
+                if (rank == 0) bar_expect(one, mine0 + 8 * s, kCtas * stage_bytes);
+                copy_tile<PAIR>(one, &map_w, a, c * kChunkK, (m * kCtas + rank) * kTileM, bar);
+                copy_tile<PAIR>(one, &map_q, a + kStageBytesA, c * kChunkK, n * p.n + rank * q_rows, bar);
                 issued = min(issued + 1, p.stages);
                 if (++s == p.stages) s = 0, phase ^= 1;
             }
             if (!good) break;
         }
-        // Should a wait have given up: the copies in flight land before the CTA may end.
-        if (!good)
+        // Should a wait have given up: the copies in flight land before the CTA (the pair) may end.
+        if (!good && rank == 0)
             for (; issued > 0; --issued) {
                 if (--s < 0) s = p.stages - 1, phase ^= 1;
                 bool again = true;
                 bar_wait(&full[s], phase, again);
             }
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {
         // D: 32-bit integers; A, B: signed 8 bits, K-major.
-        const uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(p.n >> 3) << 17 | (uint32_t)(kTileM >> 4) << 24;
-        const uint32_t one = elect_one();
+        const uint32_t idesc =
+            2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(p.n >> 3) << 17 | (uint32_t)(kCtas * kTileM >> 4) << 24;
+        uint32_t one = elect_one();
         const uint32_t empty0 = smem_addr(empty), base = smem_addr(stages);
         // What lies behind in_dim is zero in shared memory; whole steps of it are left out.
         const int last = (p.in_dim - (chunks - 1) * kChunkK + 31) / 32;
         int s = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
-        for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
-            bar_wait(&acc_empty[acc], acc_phase ^ 1, good);
+        for (int64_t t = blockIdx.x / kCtas; t < p.tiles; t += gridDim.x / kCtas) {
+            bar_wait<PAIR>(&acc_empty[acc], acc_phase ^ 1, good);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t d = tmem + acc * (p.columns >> 1);
             for (int c = 0; c < chunks; ++c) {
                 bar_wait(&full[s], phase, good);
+                if (!good) one = 0;  // nothing more is issued
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t a = operand(base + s * stage_bytes);
                 const uint64_t b = operand(base + s * stage_bytes + kStageBytesA);
                 if (c + 1 < chunks || last == 4) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_i8(one, d, a + 2 * k, b + 2 * k, idesc, (uint32_t)(c | k));
+                    for (int k = 0; k < 4; ++k) mma_i8<PAIR>(one, d, a + 2 * k, b + 2 * k, idesc, (uint32_t)(c | k));
                 } else {
-                    for (int k = 0; k < last; ++k) mma_i8(one, d, a + 2 * k, b + 2 * k, idesc, (uint32_t)(c | k));
+                    for (int k = 0; k < last; ++k) mma_i8<PAIR>(one, d, a + 2 * k, b + 2 * k, idesc, (uint32_t)(c | k));
                 }
-                mma_commit(one, empty0 + 8 * s);
+                mma_commit<PAIR>(one, empty0 + 8 * s);
                 if (++s == p.stages) s = 0, phase ^= 1;
             }
-            mma_commit(one, smem_addr(&acc_full[acc]));
+            mma_commit<PAIR>(one, smem_addr(&acc_full[acc]));
             if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
-    } else {
-        const int quad = warp & 3;  // the tensor memory lanes that this warp may read
+    } else if (warp >= 2) {
+        const int quad = warp & 3;             // the tensor memory lanes that this warp may read
+        const int half = (warp - 2) >> 2;      // even or odd groups of 16 columns
+        const int thread = threadIdx.x - 64;
         int acc = 0;
         uint32_t acc_phase = 0;
-        for (int64_t t = blockIdx.x; t < p.tiles; t += gridDim.x) {
+        for (int64_t t = blockIdx.x / kCtas; t < p.tiles; t += gridDim.x / kCtas) {
             const int m = (int)(t / p.n_tiles), n = (int)(t - (int64_t)m * p.n_tiles);
-            const int64_t row = (int64_t)m * kTileM + quad * 32 + lane;
+            const int64_t row = ((int64_t)m * kCtas + rank) * kTileM + quad * 32 + lane;
             const bool have = row < p.out_dim;
             const float ws = have ? __ldg(p.w_scale + row) : 0.0f;
+            const int b0 = n * p.n, columns = min(p.n, p.batch - b0);
+            // (This buffer was read two tiles ago, before the barrier of the last tile.)
+            if (thread < columns) scales[acc][thread] = __ldg(p.scale + b0 + thread);
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+            // Should the wait give up, the warps still meet at the barriers to come.
             bar_wait(&acc_full[acc], acc_phase, good);
-            if (!__all_sync(0xFFFFFFFFu, good)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t src = tmem + acc * (p.columns >> 1) + ((uint32_t)quad * 32 << 16);
-            const int b0 = n * p.n;
-            O* out = static_cast<O*>(p.logits) + row;
-            for (int c = 0; c < p.n && b0 + c < p.batch; c += 16) {
+            O* out = static_cast<O*>(p.logits) + (b0 + 16 * half) * p.stride + row;
+            for (int c = 16 * half; c < columns; c += 32, out += 32 * p.stride) {
                 uint32_t v[16];
                 load16(src + c, v);
-                const int bl = b0 + c + (lane & 15);
-                const float xs = bl < p.batch ? __ldg(p.scale + bl) : 0.0f;
-                wait16(v);
+                float x[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float x = __shfl_sync(0xFFFFFFFFu, xs, j);
-                    const int b = b0 + c + j;
-                    if (have && b < p.batch)
-                        put(out + b * p.stride, __fmul_rn(__fmul_rn((float)(int)v[j], ws), x));
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(&scales[acc][c + j]);
+                    x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
                 }
+                wait16(v);
+                O* o = out;
+                if (have && c + 16 <= columns) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j, o += p.stride) put(o, __fmul_rn(__fmul_rn((float)(int)v[j], ws), x[j]));
+                } else if (have) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j, o += p.stride)
+                        if (c + j < columns) put(o, __fmul_rn(__fmul_rn((float)(int)v[j], ws), x[j]));
+                }
+                __syncwarp();
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            if (lane == 0) bar_arrive(&acc_empty[acc]);
+            if (lane == 0) {
+                if constexpr (PAIR)
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                     in_first(smem_addr(&acc_empty[acc])))
+                                 : "memory");
+                else
+                    bar_arrive(&acc_empty[acc]);
+            }
             if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
     }
@@ -264,9 +356,14 @@ __global__ void __launch_bounds__(kThreadsP, 1)
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (warp == 2)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.columns));
+    if (warp == 2) {
+        if constexpr (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.columns));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.columns));
+    }
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -300,6 +397,26 @@ cudaError_t make_map(CUtensorMap* map, const void* base, int width, int rows, in
 
 }  // namespace
 
+template <typename O, bool PAIR>
+static cudaError_t launch_product(const CUtensorMap& map_w, const CUtensorMap& map_q, const ProductParams& p, int smem,
+                                  int sm_count, cudaStream_t stream) {
+    constexpr int kCtas = PAIR ? 2 : 1;
+    static SmemLimit limit;
+    cudaError_t e = limit.raise(unembed_i8_kernel<O, PAIR>, kSmemBudget);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute pair{};
+    pair.id = cudaLaunchAttributeClusterDimension;
+    pair.val.clusterDim.x = 2, pair.val.clusterDim.y = 1, pair.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(p.tiles, sm_count / kCtas) * kCtas));
+    cfg.blockDim = dim3(kThreadsP);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cfg.attrs = &pair;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, unembed_i8_kernel<O, PAIR>, map_w, map_q, p);
+}
+
 cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, const float* scale, int batch,
                        void* logits, int dtype, int64_t logits_stride, int32_t* err, int sm_count, cudaStream_t stream,
                        int* launches) {
@@ -307,14 +424,16 @@ cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, con
     p.in_dim = w.in_dim;
     p.out_dim = w.out_dim;
     p.batch = batch;
-    // Equal column tiles of at most 256, a multiple of 16 wide.
+    // Equal column tiles of at most 256, a multiple of 16 wide (of 32 in pairs).
+    const bool pair = batch > VDXS_PAIR && w.out_dim > kTileM;
+    const int ctas = pair ? 2 : 1;
     p.n_tiles = (batch + kMaxN - 1) / kMaxN;
-    p.n = ((batch + p.n_tiles - 1) / p.n_tiles + 15) / 16 * 16;
+    p.n = ((batch + p.n_tiles - 1) / p.n_tiles + 16 * ctas - 1) / (16 * ctas) * (16 * ctas);
     p.columns = 32;
     while (p.columns < 2 * p.n) p.columns *= 2;
-    const int stage_bytes = kStageBytesA + p.n * kChunkK;
+    const int stage_bytes = kStageBytesA + p.n / ctas * kChunkK;
     p.stages = std::min(kMaxStages, (kSmemBudget - 1024) / stage_bytes);
-    p.tiles = (int64_t)((w.out_dim + kTileM - 1) / kTileM) * p.n_tiles;
+    p.tiles = (int64_t)((w.out_dim + ctas * kTileM - 1) / (ctas * kTileM)) * p.n_tiles;
     p.w_scale = w.scale;
     p.scale = scale;
     p.logits = logits;
@@ -323,19 +442,16 @@ cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, con
     CUtensorMap map_w, map_q;
     static_assert(sizeof(map_w) == sizeof(w.map), "tensor map size");
     memcpy(&map_w, w.map, sizeof(map_w));
-    cudaError_t e = make_map(&map_q, q, w.in_dim, batch, q_stride, p.n);
+    cudaError_t e = make_map(&map_q, q, w.in_dim, batch, q_stride, p.n / ctas);
     if (e != cudaSuccess) return e;
     const int smem = p.stages * stage_bytes + 1024;
-    const int grid = (int)std::min<int64_t>(p.tiles, sm_count);
-    static SmemLimit limit[2];
-    if (dtype == VDXS_DTYPE_BF16) {
-        if ((e = limit[0].raise(unembed_i8_kernel<__nv_bfloat16>, kSmemBudget)) != cudaSuccess) return e;
-        unembed_i8_kernel<__nv_bfloat16><<<grid, kThreadsP, smem, stream>>>(map_w, map_q, p);
-    } else {
-        if ((e = limit[1].raise(unembed_i8_kernel<float>, kSmemBudget)) != cudaSuccess) return e;
-        unembed_i8_kernel<float><<<grid, kThreadsP, smem, stream>>>(map_w, map_q, p);
-    }
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if (dtype == VDXS_DTYPE_BF16)
+        e = pair ? launch_product<__nv_bfloat16, true>(map_w, map_q, p, smem, sm_count, stream)
+                 : launch_product<__nv_bfloat16, false>(map_w, map_q, p, smem, sm_count, stream);
+    else
+        e = pair ? launch_product<float, true>(map_w, map_q, p, smem, sm_count, stream)
+                 : launch_product<float, false>(map_w, map_q, p, smem, sm_count, stream);
+    if (e != cudaSuccess) return e;
     ++*launches;
     return cudaSuccess;
 }
