@@ -77,14 +77,13 @@ struct SelectShared {
     uint32_t marked;  // tiles with marks
     int flag;
     float fbound;
-    float wm[kBWarps];
-    double ws[kBWarps];
-    // The prompt's rows before the step, and what becomes of them.
+    float2 sums[kBThreads];  // each thread's maximum, and its sum of exponentials relative to that
+    double total;
+    // The prompt's rows before the step.
     float score[VDXS_BEAM_MAX_BEAMS];
     int done[VDXS_BEAM_MAX_BEAMS], old[VDXS_BEAM_MAX_BEAMS];
     int stop[kStopsKept];
-    double lse[VDXS_BEAM_MAX_BEAMS], size[VDXS_BEAM_MAX_BEAMS];
-    int parent[VDXS_BEAM_MAX_BEAMS], place[VDXS_BEAM_MAX_BEAMS];
+    double lse[VDXS_BEAM_MAX_BEAMS], size[VDXS_BEAM_MAX_BEAMS];  // size: length^alpha
     unsigned short group[kGroups];
 };
 static_assert(kMaxTiles * kBThreads * sizeof(float) <= sizeof(u64) * kListCap, "the groups' maxima lie in the list");
@@ -195,7 +194,7 @@ struct Vec<float> {
         return __uint_as_float(i % 4 == 0 ? w.x : i % 4 == 1 ? w.y : i % 4 == 2 ? w.z : w.w);
     }
     // A vector of which only the elements [lo, hi) may be read.
-    static __device__ uint4 edge(const float* p, int e, int lo, int hi) {
+    static __device__ __noinline__ uint4 edge(const float* p, int e, int lo, int hi) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = e + i >= lo && e + i < hi ? __float_as_uint(__ldg(p + e + i)) : kLowest;
@@ -212,7 +211,7 @@ struct Vec<__nv_bfloat16> {
         const uint32_t w = j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w;
         return __uint_as_float(i % 2 ? w & 0xFFFF0000u : w << 16);
     }
-    static __device__ uint4 edge(const __nv_bfloat16* p, int e, int lo, int hi) {
+    static __device__ __noinline__ uint4 edge(const __nv_bfloat16* p, int e, int lo, int hi) {
         const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
         uint32_t w[4];
 #pragma unroll
@@ -293,20 +292,21 @@ __device__ __noinline__ void select_slow(SelectShared& sh, const T* base, const 
     }
 }
 
-// The prompt's offers: ranks of all of them in shared memory, each beam's in order, so K
-// times the best head of a beam is taken. Lane l holds the heads of beams l and l + 32.
+// The prompt's offers: the K best of at most K * K. The order is that of the ranks in 64 bits with
+// the offer's number (beam, then place in the beam's order) in the last 12 of them, so that
+// equal ranks go to the lower beam; ranks within 2^-40 of one another count as equal.
 __device__ __noinline__ void select_prompt(SelectShared& sh, const BeamArgs& p, int prompt) {
-    const int tid = threadIdx.x, lane = tid & 31, K = p.beams;
+    const int tid = threadIdx.x, K = p.beams;
     const int64_t row0 = (int64_t)prompt * K;
-    u64* ranks = sh.list;           // [beams][K] order_of(rank); 0: none
-    u64* keys = sh.list + K * K;    // the offers' keys, where there is room for them
-    const bool kept = 2 * K * K <= kListCap;
+    u64* keys = sh.list + K * K + 1;  // the offers' keys, where there is room (the select uses one place more)
+    const bool kept = 2 * K * K + 1 <= kListCap;
     if (tid < min(p.n_stop, kStopsKept)) sh.stop[tid] = p.stop_ids[tid];
     if (tid >= 64 && tid < 64 + K) {
         const int b = tid - 64;
         sh.lse[b] = sh.done[b] ? 0.0 : __ldcg(p.ws.lse + row0 + b);
         if (p.alpha != 0.0) sh.size[b] = pow((double)max(sh.done[b] ? sh.old[b] : sh.old[b] + 1, 1), p.alpha);
     }
+    if (tid == 0) sh.count = K * K;
     auto offer = [&](int b, u64 key) { return (double)sh.score[b] + ((double)key_value(key) - sh.lse[b]); };
     for (int e0 = 0; e0 < K * K; e0 += kBThreads) {
         const int e = e0 + tid, b = e / K, i = e - b * K;
@@ -319,59 +319,29 @@ __device__ __noinline__ void select_prompt(SelectShared& sh, const BeamArgs& p, 
         if (k) score = offer(b, k);
         else if (i == 0 && sh.done[b]) score = sh.score[b];
         if (p.alpha != 0.0) score /= sh.size[b];
-        ranks[e] = score > -INFINITY ? order_of(score) : 0;
+        sh.list[e] = score > -INFINITY ? (order_of(score) & ~4095ull) | (u64)(4095 - e) : 0;
     }
-    __syncthreads();
-    if (tid >= 32) return;
-    int at0 = 0, at1 = 0;
-    u64 h0 = lane < K ? ranks[lane * K] : 0, h1 = lane + 32 < K ? ranks[(lane + 32) * K] : 0;
-    for (int k = 0; k < K; ++k) {
-        const bool second = h1 > h0;
-        u64 h = second ? h1 : h0;
-        // The highest rank: by its upper half, where that is not enough by the lower, and among
-        // equals the lowest beam.
-        const uint32_t hi = __reduce_max_sync(FULLMASK, (uint32_t)(h >> 32));
-        bool top = (uint32_t)(h >> 32) == hi;
-        uint32_t who = __ballot_sync(FULLMASK, top);
-        if (who & (who - 1)) {
-            const uint32_t lo = __reduce_max_sync(FULLMASK, top ? (uint32_t)h : 0u);
-            top = top && (uint32_t)h == lo;
-            const uint32_t first = __reduce_min_sync(FULLMASK, top ? (uint32_t)(second ? lane + 32 : lane) : 64u);
-            who = 1u << (first & 31);
-        }
-        if (hi == 0) {  // no offer is left (a rank's upper half is never 0)
-            if (lane == 0) sh.parent[k] = -1;
-        } else if (who >> lane & 1) {
-            sh.parent[k] = second ? lane + 32 : lane;
-            if (second) {
-                sh.place[k] = at1;
-                h1 = ++at1 < K ? ranks[(lane + 32) * K + at1] : 0;
-            } else {
-                sh.place[k] = at0;
-                h0 = ++at0 < K ? ranks[lane * K + at0] : 0;
-            }
-        }
+    block_select(sh, K);
+    if (tid >= K) return;
+    const int64_t r = row0 + tid;
+    const u64 pick = sh.best[tid];
+    const bool nothing = pick == 0;
+    const int e = 4095 - (int)(pick & 4095), b = nothing ? tid : e / K;
+    const bool fresh = !nothing && !sh.done[b];
+    u64 key = 0;
+    if (fresh) key = kept ? keys[e] : __ldcg(p.ws.best + row0 * K + e);
+    const int token = fresh ? key_token(key) : p.pad;
+    bool stop = false;
+    if (fresh) {
+        for (int i = 0; i < min(p.n_stop, kStopsKept); ++i) stop |= sh.stop[i] == token;
+        for (int i = kStopsKept; i < p.n_stop; ++i) stop |= p.stop_ids[i] == token;
     }
-    __syncwarp();
-    for (int k = lane; k < K; k += 32) {
-        const int64_t r = row0 + k;
-        const int b = sh.parent[k];
-        const bool nothing = b < 0, fresh = !nothing && !sh.done[b];
-        u64 key = 0;
-        if (fresh) key = kept ? keys[b * K + sh.place[k]] : __ldcg(p.ws.best + (row0 + b) * K + sh.place[k]);
-        const int token = fresh ? key_token(key) : p.pad;
-        bool stop = false;
-        if (fresh) {
-            for (int i = 0; i < min(p.n_stop, kStopsKept); ++i) stop |= sh.stop[i] == token;
-            for (int i = kStopsKept; i < p.n_stop; ++i) stop |= p.stop_ids[i] == token;
-        }
-        p.tokens[r] = token;
-        p.parents[r] = nothing ? k : b;
-        p.scores[r] = nothing ? -INFINITY : fresh ? (float)offer(b, key) : sh.score[b];
-        p.lengths[r] = nothing ? sh.old[k] : sh.old[b] + fresh;
-        p.finished[r] = nothing ? 0 : fresh ? stop : 1;
-        p.ws.push[r] = fresh;
-    }
+    p.tokens[r] = token;
+    p.parents[r] = b;
+    p.scores[r] = nothing ? -INFINITY : fresh ? (float)offer(b, key) : sh.score[b];
+    p.lengths[r] = sh.old[b] + fresh;
+    p.finished[r] = nothing ? 0 : fresh ? stop : 1;
+    p.ws.push[r] = fresh;
 }
 
 template <typename T, bool PEN>
@@ -404,8 +374,14 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
         const int lo = c == 0 ? off : 0, hi = (int)min((int64_t)p.chunk, p.vocab + off - c0);
         const int shift = (int)(c0 - off);
         auto load = [&](int u0, uint4* v) {
+            const T* at = base + u0 + tid * VN;
+            if (u0 >= lo && u0 + kUnit <= hi) {
 #pragma unroll
-            for (int u = 0; u < kVecs; ++u) v[u] = load_vector<T>(base, u0 + (u * kBThreads + tid) * VN, lo, hi);
+                for (int u = 0; u < kVecs; ++u) v[u] = __ldg(reinterpret_cast<const uint4*>(at + u * kBThreads * VN));
+            } else {
+#pragma unroll
+                for (int u = 0; u < kVecs; ++u) v[u] = load_vector<T>(base, u0 + (u * kBThreads + tid) * VN, lo, hi);
+            }
         };
         uint4 next[kVecs];
         load(0, next);
@@ -499,15 +475,25 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
                 s += sum0 + sum1;
             }
         }
-        float wm = m;
-        for (int d = 16; d > 0; d >>= 1) wm = fmaxf(wm, __shfl_xor_sync(FULLMASK, wm, d));
-        double ws = (double)s * ex2((m - wm) * kLog2e);
-        for (int d = 16; d > 0; d >>= 1) ws += __shfl_xor_sync(FULLMASK, ws, d);
-        if (lane == 0) sh.wm[warp] = wm, sh.ws[warp] = ws;
+        sh.sums[tid] = make_float2(m, s);
         if (tid == 0) sh.count = 0, sh.reach = 0;
         block_bound(sh, most, K);
         const float tau = sh.fbound;
+        const int64_t slot = (int64_t)row * p.chunks + c;
+        if (warp == kBWarps - 1) {
+            float2 part[kBWarps];
+            float M = -FLT_MAX;
+#pragma unroll
+            for (int j = 0; j < kBWarps; ++j) part[j] = sh.sums[lane + 32 * j], M = fmaxf(M, part[j].x);
+            for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(FULLMASK, M, d));
+            double S = 0.0;
+#pragma unroll
+            for (int j = 0; j < kBWarps; ++j) S += (double)part[j].y * ex2((part[j].x - M) * kLog2e);
+            for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(FULLMASK, S, d);
+            if (lane == 0) reinterpret_cast<double2*>(p.ws.part)[slot] = make_double2(M, S);
+        }
         if (most >= tau) {
+#pragma unroll 4
             for (int t = 0; t < tiles; ++t) {
                 const float top = tops[t * kBThreads + tid];
                 if (top >= tau && top > -INFINITY) {
@@ -544,16 +530,7 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
             }
         }
         block_select(sh, K);
-        const int64_t slot = (int64_t)row * p.chunks + c;
         if (tid < K) p.ws.cand[slot * K + tid] = sh.best[tid];
-        if (tid == 0) {
-            float M = sh.wm[0];
-            for (int w = 1; w < kBWarps; ++w) M = fmaxf(M, sh.wm[w]);
-            double S = 0.0;
-            for (int w = 0; w < kBWarps; ++w) S += sh.ws[w] * ex2((sh.wm[w] - M) * kLog2e);
-            p.ws.part[2 * slot] = M;
-            p.ws.part[2 * slot + 1] = S;
-        }
     }
     // The row's last CTA merges its chunks.
     __syncthreads();
@@ -573,12 +550,12 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
             double S = a.y * ex2(((float)a.x - M) * kLog2e) + b.y * ex2(((float)b.x - M) * kLog2e);
             for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(FULLMASK, S, d);
             // A NaN sum (a NaN or +infinity in the row), or none, offers nothing.
-            if (lane == 0) p.ws.lse[row] = M + log(S), sh.ws[0] = S;
+            if (lane == 0) p.ws.lse[row] = M + log(S), sh.total = S;
         }
         // Empty places have key 0 and stay below every entry.
         for (int i = tid; i < n; i += kBThreads) sh.list[i] = __ldcg(p.ws.cand + (int64_t)row * n + i);
         block_select(sh, K);
-        if (tid < K) p.ws.best[(int64_t)row * K + tid] = sh.ws[0] > 0.0 ? sh.best[tid] : 0;
+        if (tid < K) p.ws.best[(int64_t)row * K + tid] = sh.total > 0.0 ? sh.best[tid] : 0;
     }
     __syncthreads();
     if (tid == 0) {
