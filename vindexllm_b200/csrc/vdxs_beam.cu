@@ -32,7 +32,6 @@ constexpr int kListShort = 96;                // entries that are ranked without
 constexpr int kListCap = kTile + kListLimit;  // a tile may add every element it has
 constexpr int kMaxTiles = 32;                 // tiles of a chunk
 constexpr int kGroups = kBThreads;            // groups that may be read again
-constexpr int kValues = (kListCap * 8 - kMaxHistory * 4) / 4;  // penalised logits kept in the list's room
 constexpr int kStopsKept = 64;                // stop ids in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 typedef unsigned long long u64;
@@ -86,6 +85,10 @@ struct SelectShared {
     double lse[VDXS_BEAM_MAX_BEAMS], size[VDXS_BEAM_MAX_BEAMS];  // size: length^alpha
     unsigned short group[kGroups];
 };
+// The selection's shared memory, named anew in every function: through a reference its accesses
+// would be generic ones.
+extern __shared__ __align__(16) unsigned char select_smem[];
+__device__ __forceinline__ SelectShared& select_shared() { return *reinterpret_cast<SelectShared*>(select_smem); }
 static_assert(kMaxTiles * kBThreads * sizeof(float) <= sizeof(u64) * kListCap, "the groups' maxima lie in the list");
 static_assert(kGroups * kPer <= kListCap, "a list holds the groups' elements");
 
@@ -104,7 +107,8 @@ __device__ __forceinline__ int count_above(const float* p, int n, float mine, in
 
 // The K-th largest of 64 (K <= 16) or 128 disjoint groups' maxima, of one value per thread: a
 // lower bound of the K-th largest of what the values are the maxima of. In sh.fbound.
-__device__ __forceinline__ void block_bound(SelectShared& sh, float v, int K) {
+__device__ __forceinline__ void block_bound(float v, int K) {
+    SelectShared& sh = select_shared();
     float* groups = reinterpret_cast<float*>(sh.maxima);
     const int tid = threadIdx.x, share = K <= 16 ? 4 : 2, n = kBThreads / share;
     v = fmaxf(v, __shfl_xor_sync(FULLMASK, v, 1));
@@ -115,13 +119,16 @@ __device__ __forceinline__ void block_bound(SelectShared& sh, float v, int K) {
     __syncthreads();
 }
 
-// Keeps list[0..n) entries that are at least `bound`; their number in sh.count.
-__device__ __forceinline__ void block_keep(SelectShared& sh, int n, u64 bound) {
+// Keeps list[0..n) entries that are at least `bound`, n at most M for each thread; their number
+// in sh.count.
+template <int M>
+__device__ __forceinline__ void block_keep(int n, u64 bound) {
+    SelectShared& sh = select_shared();
     const int tid = threadIdx.x;
-    u64 mine[kListCap / kBThreads];
+    u64 mine[M];
     int m = 0;
 #pragma unroll
-    for (int j = 0; j < kListCap / kBThreads; ++j) {
+    for (int j = 0; j < M; ++j) {
         const int i = tid + j * kBThreads;
         mine[j] = i < n && sh.list[i] >= bound ? sh.list[i] : 0;
         m += mine[j] != 0;
@@ -130,7 +137,7 @@ __device__ __forceinline__ void block_keep(SelectShared& sh, int n, u64 bound) {
     __syncthreads();
     int at = m ? atomicAdd(&sh.count, m) : 0;
 #pragma unroll
-    for (int j = 0; j < kListCap / kBThreads; ++j)
+    for (int j = 0; j < M; ++j)
         if (mine[j]) sh.list[at++] = mine[j];
     __syncthreads();
 }
@@ -140,7 +147,8 @@ __device__ __forceinline__ void block_keep(SelectShared& sh, int n, u64 bound) {
 // list is still long, each thread takes the largest key of its share, the K-th largest of
 // those (keys are all different) is a bound again, and at most a quarter plus K remain. Then
 // every entry counts the ones above it.
-__device__ __noinline__ void block_select(SelectShared& sh, int K) {
+__device__ __noinline__ void block_select(int K) {
+    SelectShared& sh = select_shared();
     const int tid = threadIdx.x;
     __syncthreads();
     int n = sh.count;
@@ -148,8 +156,10 @@ __device__ __noinline__ void block_select(SelectShared& sh, int K) {
     if (n > kListShort) {
         u64 mx = 0;
         for (int i = tid; i < n; i += kBThreads) mx = max(mx, sh.list[i]);
-        block_bound(sh, mx ? key_value(mx) : -INFINITY, K);
-        block_keep(sh, n, (make_key(sh.fbound, -1) >> 32) << 32);
+        block_bound(mx ? key_value(mx) : -INFINITY, K);
+        const u64 bound = (make_key(sh.fbound, -1) >> 32) << 32;
+        if (n <= 2 * kBThreads) block_keep<2>(n, bound);
+        else block_keep<kListCap / kBThreads>(n, bound);
         n = sh.count;
     }
     while (n > kListLimit) {
@@ -164,20 +174,24 @@ __device__ __noinline__ void block_select(SelectShared& sh, int K) {
         }
         if (above == K - 1) sh.bound = mx;
         __syncthreads();
-        block_keep(sh, n, sh.bound);
+        block_keep<kListCap / kBThreads>(n, sh.bound);
         n = sh.count;
     }
     if (tid == 0) sh.list[n] = 0;  // an even number of entries
     __syncthreads();
-    for (int i = tid; i < n; i += kBThreads) {
-        const u64 mine = sh.list[i];
+    // A short list's entries have 8, 4 or 2 neighbouring threads each, which share the counting.
+    const int lanes = n <= 32 ? 8 : n <= 64 ? 4 : n <= 128 ? 2 : 1;
+    for (int i0 = 0; i0 < n; i0 += kBThreads / lanes) {
+        const int i = i0 + tid / lanes;
+        const u64 mine = i < n ? sh.list[i] : ~0ull;
         int above = 0;
-#pragma unroll 2
-        for (int j = 0; j < n; j += 2) {
+#pragma unroll 4
+        for (int j = 2 * (tid % lanes); j < n; j += 2 * lanes) {
             const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(sh.list + j);
             above += (o.x > mine) + (o.y > mine);
         }
-        if (above < K) sh.best[above] = mine;
+        for (int d = 1; d < lanes; d *= 2) above += __shfl_xor_sync(FULLMASK, above, d);
+        if (i < n && above < K) sh.best[above] = mine;
     }
     __syncthreads();
 }
@@ -189,6 +203,12 @@ struct Vec<float> {
     static constexpr int N = 4;
     static constexpr uint32_t kLowest = 0xFF800000u;  // -infinity
     static __device__ __forceinline__ float one(const float* p) { return __ldg(p); }
+    // Elements e..e+3 (e a multiple of 4); what lies outside [lo, hi) is -infinity.
+    static __device__ __forceinline__ void four(const float* p, int e, int lo, int hi, float* v) {
+        const uint4 w = e >= lo && e + 4 <= hi ? __ldg(reinterpret_cast<const uint4*>(p + e)) : edge(p, e, lo, hi);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = at(&w, i);
+    }
     static __device__ __forceinline__ float at(const uint4* v, int i) {
         const uint4 w = v[i / 4];
         return __uint_as_float(i % 4 == 0 ? w.x : i % 4 == 1 ? w.y : i % 4 == 2 ? w.z : w.w);
@@ -205,6 +225,17 @@ template <>
 struct Vec<__nv_bfloat16> {
     static constexpr int N = 8;
     static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ void four(const __nv_bfloat16* p, int e, int lo, int hi, float* v) {
+        uint4 w;
+        if (e >= lo && e + 4 <= hi) {
+            const uint2 two = __ldg(reinterpret_cast<const uint2*>(p + e));
+            w = make_uint4(two.x, two.y, 0u, 0u);
+        } else {
+            w = edge(p, e, lo, hi);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = at(&w, i);
+    }
     static __device__ __forceinline__ float at(const uint4* v, int i) {
         const uint4 q = v[i / 8];
         const int j = (i % 8) / 2;
@@ -254,8 +285,9 @@ __device__ __forceinline__ uint4 load_vector(const T* base, int e, int lo, int h
 
 // The elements of a vector that can be among the K largest enter the list.
 template <typename T>
-__device__ __forceinline__ void enter(SelectShared& sh, const T* base, const uint32_t* marks, int e, int lo, int hi,
+__device__ __forceinline__ void enter(const T* base, const uint32_t* marks, int e, int lo, int hi,
                                       float tau, bool equal, int shift) {
+    SelectShared& sh = select_shared();
     const uint4 raw = load_vector(base, e, lo, hi);
     const uint32_t out = marks && e < hi ? marks[e >> 5] >> (e & 31) : 0u;
 #pragma unroll
@@ -270,8 +302,9 @@ __device__ __forceinline__ void enter(SelectShared& sh, const T* base, const uin
 // its K largest whenever it is long. From the first cut on the K entries have lower
 // tokens than what follows, so an element equal to the K-th stays out.
 template <typename T>
-__device__ __noinline__ void select_slow(SelectShared& sh, const T* base, const uint32_t* marks, int lo, int hi,
-                                         float tau, int shift, int K) {
+__device__ __noinline__ void select_slow(const T* base, bool marked, int lo, int hi, float tau, int shift, int K) {
+    SelectShared& sh = select_shared();
+    const uint32_t* marks = marked ? reinterpret_cast<uint32_t*>(select_smem + sizeof(SelectShared)) : nullptr;
     const int tid = threadIdx.x;
     __syncthreads();
     if (tid == 0) sh.count = 0;
@@ -279,10 +312,10 @@ __device__ __noinline__ void select_slow(SelectShared& sh, const T* base, const 
     __syncthreads();
     for (int t0 = 0; t0 < hi; t0 += kTile) {
         for (int u = 0; u < kPer / Vec<T>::N; ++u)
-            enter<T>(sh, base, marks, t0 + (u * kBThreads + tid) * Vec<T>::N, lo, hi, tau, equal, shift);
+            enter<T>(base, marks, t0 + (u * kBThreads + tid) * Vec<T>::N, lo, hi, tau, equal, shift);
         __syncthreads();
         if (sh.count > kListLimit) {
-            block_select(sh, K);
+            block_select(K);
             if (tid < K) sh.list[tid] = sh.best[tid];
             if (tid == 0) sh.count = K;
             tau = key_value(sh.best[K - 1]);
@@ -295,7 +328,8 @@ __device__ __noinline__ void select_slow(SelectShared& sh, const T* base, const 
 // The prompt's offers: the K best of at most K * K. The order is that of the ranks in 64 bits with
 // the offer's number (beam, then place in the beam's order) in the last 12 of them, so that
 // equal ranks go to the lower beam; ranks within 2^-40 of one another count as equal.
-__device__ __noinline__ void select_prompt(SelectShared& sh, const BeamArgs& p, int prompt) {
+__device__ __forceinline__ void select_prompt(const BeamArgs& p, int prompt) {
+    SelectShared& sh = select_shared();
     const int tid = threadIdx.x, K = p.beams;
     const int64_t row0 = (int64_t)prompt * K;
     u64* keys = sh.list + K * K + 1;  // the offers' keys, where there is room (the select uses one place more)
@@ -304,7 +338,6 @@ __device__ __noinline__ void select_prompt(SelectShared& sh, const BeamArgs& p, 
     if (tid >= 64 && tid < 64 + K) {
         const int b = tid - 64;
         sh.lse[b] = sh.done[b] ? 0.0 : __ldcg(p.ws.lse + row0 + b);
-        if (p.alpha != 0.0) sh.size[b] = pow((double)max(sh.done[b] ? sh.old[b] : sh.old[b] + 1, 1), p.alpha);
     }
     if (tid == 0) sh.count = K * K;
     auto offer = [&](int b, u64 key) { return (double)sh.score[b] + ((double)key_value(key) - sh.lse[b]); };
@@ -321,7 +354,7 @@ __device__ __noinline__ void select_prompt(SelectShared& sh, const BeamArgs& p, 
         if (p.alpha != 0.0) score /= sh.size[b];
         sh.list[e] = score > -INFINITY ? (order_of(score) & ~4095ull) | (u64)(4095 - e) : 0;
     }
-    block_select(sh, K);
+    block_select(K);
     if (tid >= K) return;
     const int64_t r = row0 + tid;
     const u64 pick = sh.best[tid];
@@ -346,10 +379,13 @@ __device__ __noinline__ void select_prompt(SelectShared& sh, const BeamArgs& p, 
 
 template <typename T, bool PEN>
 __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select_kernel(const __grid_constant__ BeamArgs p) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    SelectShared& sh = *reinterpret_cast<SelectShared*>(smem);
-    uint32_t* marks = reinterpret_cast<uint32_t*>(smem + sizeof(SelectShared));  // PEN: a bit for each position
-    u64* extra = reinterpret_cast<u64*>(smem + sizeof(SelectShared) + p.chunk / 8);  // PEN: the ring's tokens
+    SelectShared& sh = select_shared();
+    uint32_t* marks = reinterpret_cast<uint32_t*>(select_smem + sizeof(SelectShared));  // PEN: a bit for each position
+    struct Held {
+        int held;
+        float value;
+    };
+    Held* extra = reinterpret_cast<Held*>(select_smem + sizeof(SelectShared) + p.chunk / 8);  // PEN: the ring's tokens
     constexpr int VN = Vec<T>::N;
     constexpr int kUnit = kBThreads * kVecs * VN;  // elements that are loaded together: one tile, two of bf16
     asm volatile("griddepcontrol.launch_dependents;");
@@ -386,44 +422,31 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
         uint4 next[kVecs];
         load(0, next);
         float m = -FLT_MAX, s = 0.0f;
+        // The chunk's tokens that the ring holds leave the stream (their marks) and are added behind
+        // it, with x / p for x > 0, else x * p, once for each time that the ring holds them
+        // (Sampler.pas:285-303). The entry whose thread sets the mark stands for the token
+        // (held >= 0), the others are ~token.
+        const int32_t* ring = PEN ? p.hist_in + (int64_t)row * p.window : nullptr;
+        int my_place = -1;
+        float my_value = 0.0f;
         if (PEN) {
-            // The chunk's tokens that the ring holds leave the stream (their marks) and enter here,
-            // with x / p for x > 0, else x * p, once for each time that the ring holds them
-            // (Sampler.pas:285-303). The entry whose thread sets the mark stands for the token.
-            const int32_t* ring = p.hist_in + (int64_t)row * p.window;
             const int count = p.count_in[row];
-            int* tokens = reinterpret_cast<int*>(sh.list);
-            float* values = reinterpret_cast<float*>(tokens + kMaxHistory);
-            if (tid == 0) sh.count = 0, sh.extra = 0, sh.marked = 0;
+            if (tid == 0) sh.extra = 0, sh.marked = 0;
             for (int i = tid; i < p.chunk / 32; i += kBThreads) marks[i] = 0;
-            for (int i0 = 0; i0 < p.window; i0 += kBThreads) {
-                const int i = i0 + tid, token = i < p.window ? ring[i] : -1;
-                const int64_t e = (int64_t)token - shift;
-                const bool in = i < count && token >= 0 && token < p.vocab && e >= lo && e < hi;
-                const float v = in ? Vec<T>::one(base + e) : 0.0f;
-                if (i0 == 0) __syncthreads();
-                if (in) {
-                    const uint32_t bit = 1u << (e & 31);
-                    const uint32_t before = atomicOr(&marks[e >> 5], bit);
-                    atomicOr(&sh.marked, 1u << (e / kTile));
-                    const int at = atomicAdd(&sh.count, 1);
-                    tokens[at] = before & bit ? ~token : token;
-                    if (at < kValues) values[at] = v;
-                }
-            }
+            int token = tid < p.window ? ring[tid] : -1;
             __syncthreads();
-            const int n = sh.count;
-            for (int i = tid; i < n; i += kBThreads) {
-                const int token = tokens[i];
-                if (token < 0) continue;
-                float v = i < kValues ? values[i] : Vec<T>::one(base + (token - shift));
-                for (int j = 0; j < n; ++j)
-                    if (tokens[j] == token || ~tokens[j] == token)
-                        v = v > 0.0f ? __fdiv_rn(v, p.penalty) : __fmul_rn(v, p.penalty);
-                if (v > m) s *= ex2((m - v) * kLog2e), m = v;
-                s += ex2((v - m) * kLog2e);
-                // Kept beside the list: a ring is at most kMaxHistory entries long.
-                if (v > -INFINITY) extra[atomicAdd(&sh.extra, 1)] = make_key(v, token);
+            for (int i = tid; i < p.window && i < count; i += kBThreads) {
+                if (i != tid) token = ring[i];
+                const int64_t e = (int64_t)token - shift;
+                if (token >= 0 && token < p.vocab && e >= lo && e < hi) {
+                    const uint32_t bit = 1u << (e & 31);
+                    const bool first = !(atomicOr(&marks[e >> 5], bit) & bit);
+                    atomicOr(&sh.marked, 1u << (e / kTile));
+                    const int at = atomicAdd(&sh.extra, 1);
+                    extra[at].held = first ? token : ~token;
+                    if (i == tid) my_place = at, my_value = Vec<T>::one(base + e);
+                    else extra[at].value = Vec<T>::one(base + e);
+                }
             }
             __syncthreads();
         }
@@ -475,10 +498,40 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
                 s += sum0 + sum1;
             }
         }
+        const int extras = PEN ? sh.extra : 0;
+        if (PEN) {
+            if (my_place >= 0) extra[my_place].value = my_value;  // fetched while the stream ran
+            __syncthreads();
+            for (int i = tid; i < extras; i += kBThreads) {
+                const int token = extra[i].held;
+                if (token < 0) continue;
+                float v = extra[i].value;
+                int times = 0;
+                for (int j = 0; j < extras; ++j) {
+                    const int other = extra[j].held;
+                    times += other == token || ~other == token;
+                }
+                for (; times > 0; --times) v = v > 0.0f ? __fdiv_rn(v, p.penalty) : __fmul_rn(v, p.penalty);
+                extra[i].value = v;
+                if (v > m) s *= ex2((m - v) * kLog2e), m = v;
+                s += ex2((v - m) * kLog2e);
+            }
+        }
         sh.sums[tid] = make_float2(m, s);
         if (tid == 0) sh.count = 0, sh.reach = 0;
-        block_bound(sh, most, K);
+        block_bound(most, K);
         const float tau = sh.fbound;
+        if (most >= tau) {
+#pragma unroll 4
+            for (int t = 0; t < tiles; ++t) {
+                const float top = tops[t * kBThreads + tid];
+                if (top >= tau && top > -INFINITY) {
+                    const int at = atomicAdd(&sh.reach, 1);
+                    if (at < kGroups) sh.group[at] = (unsigned short)(t * kBThreads + tid);
+                }
+            }
+        }
+        __syncthreads();
         const int64_t slot = (int64_t)row * p.chunks + c;
         if (warp == kBWarps - 1) {
             float2 part[kBWarps];
@@ -492,44 +545,39 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
             for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(FULLMASK, S, d);
             if (lane == 0) reinterpret_cast<double2*>(p.ws.part)[slot] = make_double2(M, S);
         }
-        if (most >= tau) {
-#pragma unroll 4
-            for (int t = 0; t < tiles; ++t) {
-                const float top = tops[t * kBThreads + tid];
-                if (top >= tau && top > -INFINITY) {
-                    const int at = atomicAdd(&sh.reach, 1);
-                    if (at < kGroups) sh.group[at] = (unsigned short)(t * kBThreads + tid);
+        const int reach = sh.reach;
+        if (reach <= kGroups) {
+            // Four elements for each thread.
+            for (int q = tid; q < reach * (kPer / 4); q += kBThreads) {
+                const int at = sh.group[q / (kPer / 4)], i = q % (kPer / 4) * 4;
+                const int e0 = at / kBThreads * kTile + (i / VN * kBThreads + at % kBThreads) * VN + i % VN;
+                float v[4];
+                Vec<T>::four(base, e0, lo, hi, v);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = e0 + j;
+                    if (v[j] >= tau && v[j] > -INFINITY && !(PEN && (marks[e >> 5] >> (e & 31) & 1)))
+                        sh.list[atomicAdd(&sh.count, 1)] = make_key(v[j], e + shift);
                 }
             }
-        }
-        __syncthreads();
-        const int reach = sh.reach;
-        const uint32_t* out = PEN ? marks : nullptr;
-        if (reach <= kGroups) {
-            // One element for each thread.
-            for (int q = tid; q < reach * kPer; q += kBThreads) {
-                const int at = sh.group[q / kPer], i = q % kPer;
-                const int e = at / kBThreads * kTile + (i / VN * kBThreads + at % kBThreads) * VN + i % VN;
-                if (e < lo || e >= hi) continue;
-                const float v = Vec<T>::one(base + e);
-                if (v >= tau && v > -INFINITY && !(PEN && (marks[e >> 5] >> (e & 31) & 1)))
-                    sh.list[atomicAdd(&sh.count, 1)] = make_key(v, e + shift);
-            }
         } else {
-            select_slow<T>(sh, base, out, lo, hi, tau, shift, K);
+            select_slow<T>(base, PEN, lo, hi, tau, shift, K);
         }
         if (PEN) {
-            // The ring's tokens join the rest, which is cut to K first.
-            const int more = sh.extra;
-            for (int i0 = 0; i0 < more; i0 += kTile) {
-                block_select(sh, K);
-                const int now = min(kTile, more - i0);
-                if (tid < K) sh.list[tid] = sh.best[tid];
-                for (int i = tid; i < now; i += kBThreads) sh.list[K + i] = extra[i0 + i];
-                if (tid == 0) sh.count = K + now;
+            // The ring's tokens join the rest: at most a list's limit at a time, the rest cut before.
+            for (int i0 = 0; i0 < extras; i0 += kListLimit) {
+                if (i0 > 0 || reach > kGroups) {
+                    block_select(K);
+                    if (tid < K) sh.list[tid] = sh.best[tid];
+                    if (tid == 0) sh.count = K;
+                    __syncthreads();
+                }
+                for (int i = i0 + tid; i < min(extras, i0 + kListLimit); i += kBThreads)
+                    if (extra[i].held >= 0 && extra[i].value >= tau && extra[i].value > -INFINITY)
+                        sh.list[atomicAdd(&sh.count, 1)] = make_key(extra[i].value, extra[i].held);
             }
         }
-        block_select(sh, K);
+        block_select(K);
         if (tid < K) p.ws.cand[slot * K + tid] = sh.best[tid];
     }
     // The row's last CTA merges its chunks.
@@ -537,6 +585,11 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
     if (tid == 0) sh.flag = count_in(&p.ws.row_done[row]) == (uint32_t)p.chunks - 1;
     __syncthreads();
     if (!sh.flag) return;
+    if (p.alpha != 0.0 && tid >= 64 && tid < 64 + K) {
+        // For the prompt's last CTA, and beside the loads below.
+        const int b = tid - 64;
+        sh.size[b] = pow((double)max(sh.done[b] ? sh.old[b] : sh.old[b] + 1, 1), p.alpha);
+    }
     if (live) {
         const int n = p.chunks * K;
         if (tid == 0) sh.count = n;
@@ -554,7 +607,7 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
         }
         // Empty places have key 0 and stay below every entry.
         for (int i = tid; i < n; i += kBThreads) sh.list[i] = __ldcg(p.ws.cand + (int64_t)row * n + i);
-        block_select(sh, K);
+        block_select(K);
         if (tid < K) p.ws.best[(int64_t)row * K + tid] = sh.total > 0.0 ? sh.best[tid] : 0;
     }
     __syncthreads();
@@ -564,7 +617,7 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
     }
     __syncthreads();
     if (!sh.flag) return;
-    select_prompt(sh, p, prompt);
+    select_prompt(p, prompt);
     if (tid == 0) p.ws.prompt_done[prompt] = 0;
 }
 
@@ -681,7 +734,7 @@ void beam_plan(int rows, int vocab, int sm_count, int* chunks, int* chunk) {
 
 cudaError_t beam_select(const BeamArgs& a, cudaStream_t stream) {
     const bool pen = a.window > 0 && a.penalty != 1.0f;
-    const size_t smem = sizeof(SelectShared) + (pen ? (size_t)a.chunk / 8 + (size_t)std::min(a.window, a.chunk) * 8 : 0);
+    const size_t smem = sizeof(SelectShared) + (pen ? (size_t)a.chunk / 8 + (size_t)a.window * 8 : 0);
     const int grid = a.batch * a.beams * a.chunks;
     const bool half = a.dtype == VDXS_DTYPE_BF16;
     void (*kern)(BeamArgs) = half ? (pen ? beam_select_kernel<__nv_bfloat16, true> : beam_select_kernel<__nv_bfloat16, false>)
