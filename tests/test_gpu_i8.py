@@ -63,6 +63,24 @@ def test_norm_many_rows(gpu_ctx, rows):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("dim", [64, 72, 520, 1032, 5000, 16384, 32768])
+def test_norm_many_rows_of_every_width(gpu_ctx, dtype, dim):
+    """More rows than SMs, where a row takes few threads (or 1024 of them, in the widest), and rows
+    that need 64 bits among ordinary ones."""
+    import torch
+    x = _hidden(150, dim, dim, dtype)
+    x[3] = 0
+    x[5, dim // 2] = float("nan")
+    x[7, 1] = float("inf")
+    if dtype != "f16":
+        x[9] *= 1e-38
+        x[11] *= 1e37
+    w = _t(np.linspace(-1.5, 1.5, dim).astype(np.float32), dtype)
+    q, scale, _ = gpu_ctx.rms_norm_i8(x, w, 1e-6)
+    _check_norm(q, scale, x, w, 1e-6)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("dim", [40, 1001, 2560])
 def test_norm_strides_in_place_and_untouched_bytes(gpu_ctx, dtype, dim):
     """Views with a row stride, a base off the 16-byte boundary, outputs in place of x and of
@@ -152,6 +170,41 @@ def test_product_larger_batches(gpu_ctx, batch):
     w = I8Weights(gpu_ctx, _t(wq), _t(ws))
     for dtype in (torch.float32, torch.bfloat16):
         _check_product(w.unembed(_t(q), _t(xs), dtype=dtype), q, xs, wq, ws)
+    w.close()
+
+
+@pytest.mark.parametrize("batch,n,k", [(200, 100, 256), (200, 129, 64), (256, 128, 48), (300, 700, 2000), (1000, 257, 130),
+                                       (1, 40000, 80), (77, 40001, 100), (256, 40001, 33), (513, 20001, 160)])
+def test_product_shapes(gpu_ctx, batch, n, k):
+    """A vocabulary of one tile with a batch of two CTAs' width, the last tile of a pair half empty,
+    more tiles than CTAs, several column tiles."""
+    import torch
+    from vindexllm_b200.sampler import I8Weights
+    wq, q = _ints(n, k, 1), _ints(batch, k, 2, -(-k // 16) * 16)
+    ws, xs = np.linspace(1e-4, 2e-3, n).astype(np.float32), np.linspace(0.01, 0.2, batch).astype(np.float32)
+    w = I8Weights(gpu_ctx, _t(wq), _t(ws))
+    for dtype in (torch.float32, torch.bfloat16):
+        _check_product(w.unembed(_t(q)[:, :k], _t(xs), dtype=dtype), q[:, :k], xs, wq, ws)
+    gpu_ctx.device_status()
+    w.close()
+
+
+def test_product_on_two_streams(gpu_ctx):
+    """Two calls with the same weights at once, one of them of pairs."""
+    import torch
+    from vindexllm_b200.sampler import I8Weights
+    n, k = 60000, 512
+    w = I8Weights(gpu_ctx, torch.randn(n, k, device="cuda", generator=torch.Generator("cuda").manual_seed(1)))
+    q = [_t(_ints(b, k, b)) for b in (7, 300)]
+    xs = [torch.rand(b.shape[0], device="cuda") for b in q]
+    want = [w.unembed(a, b) for a, b in zip(q, xs)]
+    streams = [torch.cuda.Stream() for _ in q]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        got = [w.unembed(a, b, stream=s) for a, b, s in zip(q, xs, streams)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
     w.close()
 
 
