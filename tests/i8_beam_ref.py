@@ -19,8 +19,8 @@ def norm_i8(h, weight, eps):
 
 
 def product_i8(q, scale, wq, ws):
-    acc = q.astype(np.int64) @ wq.astype(np.int64).T
-    return acc.astype(np.float64) * np.asarray(scale, np.float64)[:, None] * np.asarray(ws, np.float64)[None, :]
+    acc = q.astype(np.float64) @ wq.astype(np.float64).T  # whole numbers below 2^53: exact
+    return acc * np.asarray(scale, np.float64)[:, None] * np.asarray(ws, np.float64)[None, :]
 
 
 def penalise(x, ring, penalty):

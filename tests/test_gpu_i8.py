@@ -174,10 +174,13 @@ def test_product_larger_batches(gpu_ctx, batch):
 
 
 @pytest.mark.parametrize("batch,n,k", [(200, 100, 256), (200, 129, 64), (256, 128, 48), (300, 700, 2000), (1000, 257, 130),
-                                       (1, 40000, 80), (77, 40001, 100), (256, 40001, 33), (513, 20001, 160)])
+                                       (1, 40000, 80), (77, 40001, 100), (256, 40001, 33), (513, 20001, 160),
+                                       (300, 40001, 2100), (256, 1000, 8192), (144, 1000, 8192), (500, 100, 4096),
+                                       (9, 1, 32768), (33, 8000, 4100), (600, 3000, 1100)])
 def test_product_shapes(gpu_ctx, batch, n, k):
     """A vocabulary of one tile with a batch of two CTAs' width, the last tile of a pair half empty,
-    more tiles than CTAs, several column tiles."""
+    more tiles than CTAs, several column tiles, sums split over 2, 4 and 8 CTAs, their columns in
+    groups that the CTAs share unevenly."""
     import torch
     from vindexllm_b200.sampler import I8Weights
     wq, q = _ints(n, k, 1), _ints(batch, k, 2, -(-k // 16) * 16)

@@ -10,6 +10,9 @@
 // Batches above 128 use pairs of CTAs: one product then spans both SMs of a pair (256 vocabulary
 // entries, 128 to a CTA) and each CTA holds half of the batch columns' rows, which halves what
 // the batch operand costs each SM in shared-memory fills.
+// A small vocabulary has fewer tiles than the GPU has SMs, and one SM takes 0.3 us for each
+// 128 bytes of a tile's rows: there a cluster of 2, 4 or 8 CTAs splits a tile's sums, and
+// each adds up a share of the columns from all of them, in its shared memory.
 //
 // One persistent CTA per SM, ten warps: warp 0 copies 128-byte wide tiles of both operands
 // into a ring of stages (TMA, 128-byte swizzle), warp 1 issues the products, warps 2 to 9
@@ -36,9 +39,6 @@ constexpr int kMaxN = 256;           // batch columns of a tile
 constexpr int kMaxStages = 12;
 constexpr int kStageBytesA = kTileM * kChunkK;
 constexpr int kSmemBudget = 220 * 1024;
-#ifndef VDXS_PAIR
-#define VDXS_PAIR 128
-#endif
 constexpr int32_t kErrTimeout = 3;   // the context's device error word: a bounded wait gave up
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -52,41 +52,29 @@ __device__ __forceinline__ void bar_expect(uint64_t* bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-__device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(done)
-                 : "r"(smem_addr(bar)), "r"(parity)
-                 : "memory");
-    return done != 0u;
-}
-__device__ __forceinline__ bool bar_try_cluster(uint64_t* bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, "
-        "p;\n}"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity)
-        : "memory");
-    return done != 0u;
-}
-// Waits for a phase, at most about two seconds; `good` turns false when it gives up, and later
-// waits return at once. No branch of the caller hangs on the outcome, so a warp that waits
-// together stays together.
+// Waits for a phase, at most about two seconds; `good` turns false when that gives up, and later
+// waits try twice. The loop is closed to the compiler and no branch of the caller hangs on its
+// outcome, so that a warp that waits together is known to stay together, which keeps the
+// operands of what it issues in uniform registers.
+#define VDXS_WAIT(TRY)                                                                        \
+    asm volatile(                                                                             \
+        "{\n .reg .pred p, q;\n .reg .u64 t, end;\n " TRY " p, [%1], %2;\n @p bra over;\n"     \
+        " mov.u64 t, %%globaltimer;\n add.u64 end, t, %3;\n"                                  \
+        "again:\n " TRY " p, [%1], %2;\n @p bra over;\n"                                      \
+        " mov.u64 t, %%globaltimer;\n setp.lt.u64 q, t, end;\n @q bra again;\n"               \
+        "over:\n selp.u32 %0, 1, 0, p;\n}"                                                    \
+        : "=r"(done)                                                                          \
+        : "r"(smem_addr(bar)), "r"(parity), "l"(limit)                                        \
+        : "memory")
 template <bool CLUSTER = false>
 __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, bool& good) {
-    auto ready = [&] { return CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity); };
-    if (ready() || !good) return;
-    uint64_t t0, t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-    for (;;) {
-        for (int i = 0; i < 64; ++i)
-            if (ready()) return;
-        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-        if (t - t0 > 2000000000ull) break;
-    }
-    good = false;
+    uint32_t done;
+    const uint64_t limit = good ? 2000000000ull : 0ull;
+    if constexpr (CLUSTER) VDXS_WAIT("mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64");
+    else VDXS_WAIT("mbarrier.try_wait.parity.shared::cta.b64");
+    good = good && done != 0u;
 }
+#undef VDXS_WAIT
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t e;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(e));
@@ -162,10 +150,10 @@ __device__ __forceinline__ void mma_commit(uint32_t one, uint32_t bar) {
             "r"(one)
             : "memory");
 }
-// The address of this CTA's `addr` in the pair's first CTA.
-__device__ __forceinline__ uint32_t in_first(uint32_t addr) {
+// The address of this CTA's `addr` in a CTA of the cluster.
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
     uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
     return a;
 }
 __device__ __forceinline__ void cluster_sync() {
@@ -192,7 +180,7 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 struct ProductParams {
-    int in_dim, out_dim, batch, n, n_tiles, stages, columns;
+    int in_dim, out_dim, batch, n, n_tiles, stages, columns, split;
     int64_t tiles;  // vocabulary tiles (of two CTAs, in pairs) * n_tiles
     const float *w_scale, *scale;
     void* logits;
@@ -200,7 +188,29 @@ struct ProductParams {
     int32_t* err;
 };
 
-template <typename O, bool PAIR>
+// 16 columns of a thread's row to the logits; `columns` of them are in the batch.
+template <typename O>
+__device__ __forceinline__ void store16(O* o, int64_t stride, const uint32_t* v, const float* scales, float ws,
+                                        int columns, bool have) {
+    float x[16];
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(scales + j);
+        x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
+    }
+    if (have && columns >= 16) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j, o += stride) put(o, __fmul_rn(__fmul_rn((float)(int)v[j], ws), x[j]));
+    } else if (have) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j, o += stride)
+            if (j < columns) put(o, __fmul_rn(__fmul_rn((float)(int)v[j], ws), x[j]));
+    }
+}
+
+enum Mode : int { kSingle = 0, kPair = 1, kSplit = 2 };
+
+template <typename O, int MODE>
 __global__ void __launch_bounds__(kThreadsP, 1)
     unembed_i8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q,
                       const ProductParams p) {
@@ -209,12 +219,19 @@ __global__ void __launch_bounds__(kThreadsP, 1)
     __shared__ uint32_t tmem_base;
     __shared__ __align__(16) float scales[2][kMaxN];
     unsigned char* stages = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (A shuffled value is one for the whole warp to the compiler too.)
+    const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    constexpr bool PAIR = MODE == kPair, SPLIT = MODE == kSplit;
     constexpr int kCtas = PAIR ? 2 : 1;
     const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;  // in the pair
+    const int part = SPLIT ? (int)(blockIdx.x % p.split) : 0;
+    const int64_t first = SPLIT ? blockIdx.x / p.split : blockIdx.x / kCtas;      // of this CTA's tiles
+    const int64_t step = SPLIT ? gridDim.x / p.split : gridDim.x / kCtas;         // (with SPLIT it has one)
     const int q_rows = p.n / kCtas;                     // batch rows that this CTA holds
     const int stage_bytes = kStageBytesA + q_rows * kChunkK;
     const int chunks = (p.in_dim + kChunkK - 1) / kChunkK;
+    const int chunk0 = SPLIT ? (int)((int64_t)chunks * part / p.split) : 0;
+    const int chunk1 = SPLIT ? (int)((int64_t)chunks * (part + 1) / p.split) : chunks;
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) bar_init(&full[i], 1), bar_init(&empty[i], 1);
         for (int i = 0; i < 2; ++i) bar_init(&acc_full[i], 1), bar_init(&acc_empty[i], kEpiWarps * kCtas);
@@ -242,12 +259,12 @@ __global__ void __launch_bounds__(kThreadsP, 1)
     bool good = true;
     if (warp == 0) {
         const uint32_t one = elect_one();
-        const uint32_t base = smem_addr(stages), mine0 = smem_addr(full), full0 = PAIR ? in_first(mine0) : mine0;
+        const uint32_t base = smem_addr(stages), mine0 = smem_addr(full), full0 = PAIR ? in_cta(mine0, 0) : mine0;
         int s = 0, issued = 0;
         uint32_t phase = 0;
-        for (int64_t t = blockIdx.x / kCtas; t < p.tiles; t += gridDim.x / kCtas) {
+        for (int64_t t = first; t < p.tiles; t += step) {
             const int m = (int)(t / p.n_tiles), n = (int)(t - (int64_t)m * p.n_tiles);
-            for (int c = 0; c < chunks; ++c) {
+            for (int c = chunk0; c < chunk1; ++c) {
                 bar_wait(&empty[s], phase ^ 1, good);
                 if (!good) break;
                 // A pair's stages are counted together by its first CTA.
@@ -277,11 +294,11 @@ __global__ void __launch_bounds__(kThreadsP, 1)
         const int last = (p.in_dim - (chunks - 1) * kChunkK + 31) / 32;
         int s = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
-        for (int64_t t = blockIdx.x / kCtas; t < p.tiles; t += gridDim.x / kCtas) {
+        for (int64_t t = first; t < p.tiles; t += step) {
             bar_wait<PAIR>(&acc_empty[acc], acc_phase ^ 1, good);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t d = tmem + acc * (p.columns >> 1);
-            for (int c = 0; c < chunks; ++c) {
+            for (int c = chunk0; c < chunk1; ++c) {
                 bar_wait(&full[s], phase, good);
                 if (!good) one = 0;  // nothing more is issued
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -289,9 +306,9 @@ __global__ void __launch_bounds__(kThreadsP, 1)
                 const uint64_t b = operand(base + s * stage_bytes + kStageBytesA);
                 if (c + 1 < chunks || last == 4) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_i8<PAIR>(one, d, a + 2 * k, b + 2 * k, idesc, (uint32_t)(c | k));
+                    for (int k = 0; k < 4; ++k) mma_i8<PAIR>(one, d, a + 2 * k, b + 2 * k, idesc, (uint32_t)((c - chunk0) | k));
                 } else {
-                    for (int k = 0; k < last; ++k) mma_i8<PAIR>(one, d, a + 2 * k, b + 2 * k, idesc, (uint32_t)(c | k));
+                    for (int k = 0; k < last; ++k) mma_i8<PAIR>(one, d, a + 2 * k, b + 2 * k, idesc, (uint32_t)((c - chunk0) | k));
                 }
                 mma_commit<PAIR>(one, empty0 + 8 * s);
                 if (++s == p.stages) s = 0, phase ^= 1;
@@ -305,7 +322,7 @@ __global__ void __launch_bounds__(kThreadsP, 1)
         const int thread = threadIdx.x - 64;
         int acc = 0;
         uint32_t acc_phase = 0;
-        for (int64_t t = blockIdx.x / kCtas; t < p.tiles; t += gridDim.x / kCtas) {
+        for (int64_t t = first; t < p.tiles; t += step) {
             const int m = (int)(t / p.n_tiles), n = (int)(t - (int64_t)m * p.n_tiles);
             const int64_t row = ((int64_t)m * kCtas + rank) * kTileM + quad * 32 + lane;
             const bool have = row < p.out_dim;
@@ -319,37 +336,63 @@ __global__ void __launch_bounds__(kThreadsP, 1)
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t src = tmem + acc * (p.columns >> 1) + ((uint32_t)quad * 32 << 16);
             O* out = static_cast<O*>(p.logits) + (b0 + 16 * half) * p.stride + row;
-            for (int c = 16 * half; c < columns; c += 32, out += 32 * p.stride) {
+            for (int c = 16 * half; !SPLIT && c < columns; c += 32, out += 32 * p.stride) {
                 uint32_t v[16];
                 load16(src + c, v);
-                float x[16];
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(&scales[acc][c + j]);
-                    x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
-                }
                 wait16(v);
-                O* o = out;
-                if (have && c + 16 <= columns) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j, o += p.stride) put(o, __fmul_rn(__fmul_rn((float)(int)v[j], ws), x[j]));
-                } else if (have) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j, o += p.stride)
-                        if (c + j < columns) put(o, __fmul_rn(__fmul_rn((float)(int)v[j], ws), x[j]));
-                }
+                store16(out, p.stride, v, &scales[acc][c], ws, columns - c, have);
                 __syncwarp();
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) {
                 if constexpr (PAIR)
                     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                                     in_first(smem_addr(&acc_empty[acc])))
+                                     in_cta(smem_addr(&acc_empty[acc]), 0))
                                  : "memory");
                 else
                     bar_arrive(&acc_empty[acc]);
             }
             if (++acc == 2) acc = 0, acc_phase ^= 1;
+        }
+    }
+    if constexpr (SPLIT) {
+        // All parts of the tile are summed and every CTA's ring is idle: group g of 16 columns goes to
+        // CTA g mod split, [part][its group][column][row] in the ring's room.
+        __syncwarp();
+        cluster_sync();
+        const int quad = warp & 3, half = (warp - 2) >> 2, groups = p.n / 16;
+        const int own = (groups + p.split - 1) / p.split;
+        const uint32_t room = smem_addr(stages);
+        if (warp >= 2) {
+            for (int g = half; g < groups; g += 2) {
+                uint32_t v[16];
+                load16(tmem + ((uint32_t)quad * 32 << 16) + 16 * g, v);
+                wait16(v);
+                const uint32_t to = in_cta(room, g % p.split) +
+                                    ((part * own + g / p.split) * 16 * kTileM + quad * 32 + lane) * 4;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + j * kTileM * 4), "r"(v[j]) : "memory");
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+        if (warp >= 2 && first < p.tiles) {
+            const int m = (int)(first / p.n_tiles), n = (int)(first - (int64_t)m * p.n_tiles);
+            const int64_t row = (int64_t)m * kTileM + quad * 32 + lane;
+            const int b0 = n * p.n;
+            const bool have = row < p.out_dim;
+            const float ws = have ? __ldg(p.w_scale + row) : 0.0f;
+            for (int i = half; i < own && i * p.split + part < groups; i += 2) {
+                const int c = 16 * (i * p.split + part);
+                const uint32_t* in = reinterpret_cast<const uint32_t*>(stages) + i * 16 * kTileM + quad * 32 + lane;
+                uint32_t v[16] = {};
+                for (int r = 0; r < p.split; ++r, in += own * 16 * kTileM)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] += in[j * kTileM];
+                store16(static_cast<O*>(p.logits) + (int64_t)(b0 + c) * p.stride + row, p.stride, v, &scales[0][c], ws,
+                        p.batch - b0 - c, have);
+            }
         }
     }
     if (!good) *p.err = kErrTimeout;
@@ -397,24 +440,32 @@ cudaError_t make_map(CUtensorMap* map, const void* base, int width, int rows, in
 
 }  // namespace
 
-template <typename O, bool PAIR>
+template <typename O, int MODE>
 static cudaError_t launch_product(const CUtensorMap& map_w, const CUtensorMap& map_q, const ProductParams& p, int smem,
                                   int sm_count, cudaStream_t stream) {
-    constexpr int kCtas = PAIR ? 2 : 1;
     static SmemLimit limit;
-    cudaError_t e = limit.raise(unembed_i8_kernel<O, PAIR>, kSmemBudget);
+    cudaError_t e = limit.raise(unembed_i8_kernel<O, MODE>, kSmemBudget);
     if (e != cudaSuccess) return e;
-    cudaLaunchAttribute pair{};
-    pair.id = cudaLaunchAttributeClusterDimension;
-    pair.val.clusterDim.x = 2, pair.val.clusterDim.y = 1, pair.val.clusterDim.z = 1;
+    const int ctas = MODE == kPair ? 2 : MODE == kSplit ? p.split : 1;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = (unsigned)ctas, cluster.val.clusterDim.y = 1, cluster.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(p.tiles, sm_count / kCtas) * kCtas));
+    cfg.gridDim = dim3((unsigned)((MODE == kSplit ? p.tiles : std::min<int64_t>(p.tiles, sm_count / ctas)) * ctas));
     cfg.blockDim = dim3(kThreadsP);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
-    cfg.attrs = &pair;
-    cfg.numAttrs = PAIR ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, unembed_i8_kernel<O, PAIR>, map_w, map_q, p);
+    cfg.attrs = &cluster;
+    cfg.numAttrs = MODE == kSingle ? 0 : 1;
+    return cudaLaunchKernelEx(&cfg, unembed_i8_kernel<O, MODE>, map_w, map_q, p);
+}
+
+template <typename O>
+static cudaError_t launch_mode(int mode, const CUtensorMap& map_w, const CUtensorMap& map_q, const ProductParams& p,
+                               int smem, int sm_count, cudaStream_t stream) {
+    if (mode == kPair) return launch_product<O, kPair>(map_w, map_q, p, smem, sm_count, stream);
+    if (mode == kSplit) return launch_product<O, kSplit>(map_w, map_q, p, smem, sm_count, stream);
+    return launch_product<O, kSingle>(map_w, map_q, p, smem, sm_count, stream);
 }
 
 cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, const float* scale, int batch,
@@ -425,15 +476,22 @@ cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, con
     p.out_dim = w.out_dim;
     p.batch = batch;
     // Equal column tiles of at most 256, a multiple of 16 wide (of 32 in pairs).
-    const bool pair = batch > VDXS_PAIR && w.out_dim > kTileM;
-    const int ctas = pair ? 2 : 1;
     p.n_tiles = (batch + kMaxN - 1) / kMaxN;
+    const int64_t tiles = (int64_t)((w.out_dim + kTileM - 1) / kTileM) * p.n_tiles;
+    const int chunks = (w.in_dim + kChunkK - 1) / kChunkK;
+    // Pairs where the batch operand weighs and the sums are long.
+    const bool pair = batch > 128 && w.in_dim >= 2048 && tiles > sm_count;
+    // A split's share is four chunks at least, and its clusters fit the GPU at once.
+    p.split = 1;
+    for (int s = 2; s <= 8 && tiles * s <= sm_count * (s < 8 ? 7 : 6) / 8 && chunks >= 4 * s; s *= 2) p.split = s;
+    const int mode = pair ? kPair : p.split > 1 ? kSplit : kSingle;
+    const int ctas = pair ? 2 : 1;
     p.n = ((batch + p.n_tiles - 1) / p.n_tiles + 16 * ctas - 1) / (16 * ctas) * (16 * ctas);
     p.columns = 32;
     while (p.columns < 2 * p.n) p.columns *= 2;
     const int stage_bytes = kStageBytesA + p.n / ctas * kChunkK;
     p.stages = std::min(kMaxStages, (kSmemBudget - 1024) / stage_bytes);
-    p.tiles = (int64_t)((w.out_dim + ctas * kTileM - 1) / (ctas * kTileM)) * p.n_tiles;
+    p.tiles = pair ? (int64_t)((w.out_dim + 2 * kTileM - 1) / (2 * kTileM)) * p.n_tiles : tiles;
     p.w_scale = w.scale;
     p.scale = scale;
     p.logits = logits;
@@ -445,12 +503,8 @@ cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, con
     cudaError_t e = make_map(&map_q, q, w.in_dim, batch, q_stride, p.n / ctas);
     if (e != cudaSuccess) return e;
     const int smem = p.stages * stage_bytes + 1024;
-    if (dtype == VDXS_DTYPE_BF16)
-        e = pair ? launch_product<__nv_bfloat16, true>(map_w, map_q, p, smem, sm_count, stream)
-                 : launch_product<__nv_bfloat16, false>(map_w, map_q, p, smem, sm_count, stream);
-    else
-        e = pair ? launch_product<float, true>(map_w, map_q, p, smem, sm_count, stream)
-                 : launch_product<float, false>(map_w, map_q, p, smem, sm_count, stream);
+    e = dtype == VDXS_DTYPE_BF16 ? launch_mode<__nv_bfloat16>(mode, map_w, map_q, p, smem, sm_count, stream)
+                                 : launch_mode<float>(mode, map_w, map_q, p, smem, sm_count, stream);
     if (e != cudaSuccess) return e;
     ++*launches;
     return cudaSuccess;
