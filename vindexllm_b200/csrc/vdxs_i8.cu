@@ -168,6 +168,12 @@ __device__ __forceinline__ void get_weights(const W* p, float* f) {
 // maximum is found in fp32, its exact value among the few products that are within rounding
 // of it, and q from fp32 except next to a border. A row whose fp32 maximum says nothing
 // (NaN, overflow, subnormal) is done again in 64 bits.
+//
+// 8192 rows of 3840 bf16 with a residual take 52 us (4.2 TB/s, 0.65 of the copy rate). Issue
+// slots and the latency of a row's three steps (load, sum, round) share it: 64 registers a
+// thread hold 32 elements, which keeps seven rows on their way on an SM. With the products
+// kept in registers instead of the weights read again it took 73 us, with 64-bit arithmetic
+// for every element 115.
 template <typename T, typename W, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT, 1024 / MAXT) rms_norm_i8_rows_kernel(const __grid_constant__ NormI8Args p) {
     constexpr int N = Pack<T>::N;
@@ -349,8 +355,9 @@ cudaError_t launch_norm(const NormI8Args& a, cudaStream_t stream) {
         rms_norm_i8_kernel<T, W><<<a.rows, kNormThreads, 0, stream>>>(a);
         return cudaGetLastError();
     }
-    // Many rows: 32 elements a thread, so that a row takes few threads and many rows are on their
-    // way. Few rows, or short ones: one vector a thread.
+    // More rows than SMs: 32 elements a thread, so that a row takes few threads and many rows are
+    // on their way. Few rows, or short ones: one vector a thread, for the latency (1 row of 2560
+    // fp32 in 3.1 us, with the launch).
     constexpr int kMost = 32 / N;
     const int nv = a.dim / N;
     const int per = nv > 1024 || (a.rows > 148 && nv > 64) ? kMost : 1;
