@@ -159,6 +159,27 @@ def test_strides_and_offsets(gpu_ctx):
             search.close()
 
 
+def test_offsets_beyond_32_bits(gpu_ctx):
+    """Rows of logits and of a cache that lie more than 2^31 elements apart from first to last."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    vocab, beams = 5001, 9
+    wide = torch.empty(beams, 1 << 28, dtype=torch.bfloat16, device="cuda")
+    view = wide[:, 3:3 + vocab]
+    view.copy_(torch.randn(view.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(1)))
+    cache = wide[:, 1 << 27:(1 << 27) + 777]
+    cache.copy_(torch.randn(cache.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(2)))
+    before = cache.clone()
+    s = _state(1, beams, 0, vocab, 3)
+    s["scores"][:] = np.linspace(-2, -2.4, beams)
+    want = ref.beam_step(view.float().cpu().numpy(), 1, beams, s)
+    search, out = BeamSearch(gpu_ctx, 1, beams, vocab), _device(s, 1, beams, 0)
+    got = search.step(_device(s, 1, beams, 0), view, out=out, caches=[cache])
+    _check((*got, out), want, 1, beams)
+    assert torch.equal(cache, before[got[1][0].long()])
+    search.close()
+
+
 def test_finished_rows_are_not_read(gpu_ctx):
     """Logits of finished and dead beams may hold anything."""
     import torch

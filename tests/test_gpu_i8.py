@@ -104,6 +104,46 @@ def test_norm_strides_in_place_and_untouched_bytes(gpu_ctx, dtype, dim):
                 assert torch.equal(now[:, :off], keep[:, :off]) and torch.equal(now[:, off + dim:], keep[:, off + dim:])
 
 
+def test_norm_hidden_without_residual_and_offset_weights(gpu_ctx):
+    """The hidden state written without a residual, and weights off the 16-byte boundary."""
+    import torch
+    for rows in (3, 200):
+        x, wb = _hidden(rows, 2048, 1, "bf16"), torch.rand(2049, device="cuda")
+        for w in (wb[:2048], wb[1:]):
+            out = torch.zeros_like(x)
+            q, scale, h = gpu_ctx.rms_norm_i8(x, w, 1e-6, out_hidden=out)
+            assert h is out and torch.equal(out, x)
+            _check_norm(q, scale, x, w, 1e-6)
+
+
+def test_offsets_beyond_32_bits(gpu_ctx):
+    """More than 2^31 elements between the first row and the last: hidden states, 8-bit rows
+    and logits."""
+    import torch
+    from vindexllm_b200.sampler import I8Weights
+    wide = torch.empty(9, 1 << 28, dtype=torch.bfloat16, device="cuda")
+    x = wide[:, 64:64 + 1040]
+    x.copy_(_hidden(9, 1040, 3, "bf16"))
+    w = torch.ones(1040, device="cuda")
+    q8 = torch.empty(9, 1 << 28, dtype=torch.int8, device="cuda")
+    q, scale, h = gpu_ctx.rms_norm_i8(x, w, 1e-6, residual=x, out_hidden=x, q=q8[:, :1040])
+    _check_norm(q, scale, x, w, 1e-6)
+    n, batch = 262144, 8300
+    wq = torch.randint(-127, 128, (n, 1040), dtype=torch.int8, device="cuda")
+    weights = I8Weights(gpu_ctx, wq, torch.ones(n, device="cuda"))
+    want = (q.double() @ wq.double().T)
+    got = weights.unembed(q, torch.ones(9, device="cuda"))
+    assert torch.equal(got.double(), want)  # whole numbers below 2^24
+    del wide, q8
+    torch.cuda.empty_cache()
+    rows = torch.randint(-127, 128, (batch, 1040), dtype=torch.int8, device="cuda")
+    got = weights.unembed(rows, torch.ones(batch, device="cuda"), dtype=torch.bfloat16)
+    assert got.numel() > 1 << 31
+    for part in (slice(0, 3), slice(8190, 8195), slice(8297, 8300)):
+        assert torch.equal(got[part], (rows[part].double() @ wq.double().T).to(torch.bfloat16))
+    weights.close()
+
+
 def test_norm_values_on_the_edge(gpu_ctx):
     """Rows of zeros, NaN, infinities, subnormals, values whose squares overflow fp32, and values on
     rounding borders (k + 1/2 of a step), which go to the even integer."""

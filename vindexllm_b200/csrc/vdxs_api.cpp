@@ -1530,6 +1530,7 @@ VDXS_API int32_t vdxs_sample_unembed_i8(vdxs_context* ctx, const vdxs_config* cf
 // ---------------------------------------------------------------------------------
 struct vdxs_beam {
     vdxs_context* ctx = nullptr;
+    int device = 0;
     int batch = 0, beams = 0, vocab = 0, chunks = 0, chunk = 0;
     BeamWorkspace ws;
 };
@@ -1613,6 +1614,7 @@ VDXS_API int32_t vdxs_beam_create(vdxs_context* ctx, int32_t batch, int32_t beam
     auto* b = new (std::nothrow) vdxs_beam();
     if (!b) return fail(ctx, VDXS_E_NO_MEMORY, "out of host memory");
     b->ctx = ctx;
+    b->device = ctx->device;
     b->batch = batch;
     b->beams = beams;
     b->vocab = vocab;
@@ -1641,7 +1643,7 @@ VDXS_API int32_t vdxs_beam_create(vdxs_context* ctx, int32_t batch, int32_t beam
 
 VDXS_API int32_t vdxs_beam_destroy(vdxs_beam* b) {
     if (!b) return VDXS_OK;
-    DeviceGuard g(b->ctx->device);
+    DeviceGuard g(b->device);
     free_beam(b);
     return VDXS_OK;
 }
