@@ -487,7 +487,8 @@ VDXS_API int32_t vdxs_sample_unembed_i8(vdxs_context* ctx, const vdxs_config* cf
  *   - the `beams` offers with the highest score / max(length, 1)^length_alpha stay, in that
  *     order (equal ones: the lower beam, then the beam's own order).
  * Log-probabilities and the order of the offers are taken in 64 bits (exponentials in fp32;
- * ranks within 2^-40 of one another count as equal); scores are stored in fp32. A slot that gets no offer has token pad_token, its own slot as the parent, score
+ * values within 2^-39 of one another count as equal, and two such offers of one beam may
+ * stand in either order); scores are stored in fp32. A slot that gets no offer has token pad_token, its own slot as the parent, score
  * -infinity, finished 0, and the length that stood there; it offers nothing in later steps.
  * ---------------------------------------------------------------------------- */
 #define VDXS_BEAM_MAX_BEAMS 64

@@ -1716,6 +1716,9 @@ VDXS_API int32_t vdxs_beam_step(vdxs_beam* b, const vdxs_beam_config* cfg, const
         delete[] moved;
         return rc;
     }
+    bool moves = false;
+    for (int32_t i = 0; i < n_caches; ++i) moves |= moved[i].segments > 0;
+    a.move_rings = a.window > 0 && a.window <= kBeamShortWindow && !moves;
     DeviceGuard g(ctx->device);
     const cudaStream_t st = (cudaStream_t)stream;
     int launches = 1;

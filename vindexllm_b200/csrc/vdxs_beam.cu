@@ -5,8 +5,9 @@
 // running maximum with a sum of exponentials relative to it, and notes the maximum of its 16
 // elements of every tile. The K-th largest of disjoint groups' maxima is a lower bound of the
 // chunk's K-th largest element (K = beams), and only the groups whose maximum reaches the
-// bound, hardly more than K of them, are read again for their elements. The last CTA of a row
-// merges the row's lists and sums, the last row of a prompt merges the beams' offers; both are
+// bound, hardly more than K of them, are read again for their elements. The last CTA of a prompt
+// merges the lists and sums of its rows, and moves its rings where nothing else moves; where the
+// lists are too many for one CTA, the last CTA of each row merges that row's first. Both are
 // found by counters that reset themselves.
 //
 // Rounding: exponentials and a thread's sum (at most 512 of them) are fp32, the sums of threads
@@ -15,9 +16,8 @@
 //
 // What bounds it: with many rows the logits' bytes (512 rows of 262144 fp32 in 93 us, 5.8 TB/s,
 // 0.89 of the copy rate), with few the chain of dependent steps behind the stream (64 rows of
-// bf16 with rings in 28.5 us, of which the logits take 6; 4 rows of 32000 in 9.1 us): two
-// merges by the last CTA, each a count, a load and a select, some 3 us together, and the
-// rings' launch. Notes of group maxima instead of a list that the stream itself fills took
+// bf16 with rings in 25 us, of which the logits take 6; 4 rows of 32000 in 8.7 us): bound,
+// elements, selection, and a merge or two, each a count, loads and a selection. Notes of group maxima instead of a list that the stream itself fills took
 // the 512 rows from 177 to 97 us: the list's code cost the loop its registers.
 #include "vdxs_internal.h"
 #include "../../include/vdx_sampler.h"
@@ -43,6 +43,7 @@ constexpr int kListShort = 96;                // entries that are ranked without
 constexpr int kListCap = kTile + kListLimit;  // a tile may add every element it has
 constexpr int kMaxTiles = 32;                 // tiles of a chunk
 constexpr int kGroups = kBThreads;            // groups that may be read again
+constexpr int kOneMerge = 512;                // entries of a prompt's lists that are merged at once
 constexpr int kStopsKept = 64;                // stop ids in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 typedef unsigned long long u64;
@@ -88,11 +89,13 @@ struct SelectShared {
     int flag;
     float fbound;
     float2 sums[kBThreads];  // each thread's maximum, and its sum of exponentials relative to that
-    double total;
     // The prompt's rows before the step.
     float score[VDXS_BEAM_MAX_BEAMS];
     int done[VDXS_BEAM_MAX_BEAMS], old[VDXS_BEAM_MAX_BEAMS];
     int stop[kStopsKept];
+    // What becomes of them: where the rings are moved here.
+    int parent[VDXS_BEAM_MAX_BEAMS], token[VDXS_BEAM_MAX_BEAMS], slot[VDXS_BEAM_MAX_BEAMS];
+    int pos[VDXS_BEAM_MAX_BEAMS], held[VDXS_BEAM_MAX_BEAMS];
     double lse[VDXS_BEAM_MAX_BEAMS], size[VDXS_BEAM_MAX_BEAMS];  // size: length^alpha
     unsigned short group[kGroups];
 };
@@ -336,56 +339,112 @@ __device__ __noinline__ void select_slow(const T* base, bool marked, int lo, int
     }
 }
 
-// The prompt's offers: the K best of at most K * K. The order is that of the ranks in 64 bits with
-// the offer's number (beam, then place in the beam's order) in the last 12 of them, so that
-// equal ranks go to the lower beam; ranks within 2^-40 of one another count as equal.
+// A row's sum of exponentials and its logarithm from its chunks (at most 64), by one warp.
+__device__ __forceinline__ void row_sum(const BeamArgs& p, int64_t row, double* sum, double* lse) {
+    const int lane = threadIdx.x & 31;
+    const double2* part = reinterpret_cast<const double2*>(p.ws.part) + row * p.chunks;
+    const double2 zero = make_double2(-INFINITY, 0.0);
+    const double2 a = lane < p.chunks ? __ldcg(part + lane) : zero;
+    const double2 b = lane + 32 < p.chunks ? __ldcg(part + lane + 32) : zero;
+    float M = (float)fmax(a.x, b.x);  // maxima of fp32 values
+    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(FULLMASK, M, d));
+    double S = a.y * ex2(((float)a.x - M) * kLog2e) + b.y * ex2(((float)b.x - M) * kLog2e);
+    for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(FULLMASK, S, d);
+    *sum = S;
+    *lse = M + log(S);
+}
+
+// The prompt's offers: the K best of each beam's K (or, unmerged, of its chunks' lists). The order
+// is that of the ranks in 64 bits with the offer's number (beam, then place) in the last 13 of
+// them, so that equal ranks go to the lower beam and in a beam to the lower chunk and place;
+// ranks within 2^-39 of one another count as equal.
 __device__ __forceinline__ void select_prompt(const BeamArgs& p, int prompt) {
     SelectShared& sh = select_shared();
     const int tid = threadIdx.x, K = p.beams;
     const int64_t row0 = (int64_t)prompt * K;
-    u64* keys = sh.list + K * K + 1;  // the offers' keys, where there is room (the select uses one place more)
-    const bool kept = 2 * K * K + 1 <= kListCap;
+    const int per = p.merge_rows ? K : p.chunks * K, n = K * per;  // offers of a beam, of the prompt
+    const u64* lists = (p.merge_rows ? p.ws.best : p.ws.cand) + row0 * per;
+    u64* keys = sh.list + n + 1;  // the offers' keys, where there is room (the select uses one place more)
+    const bool kept = 2 * n + 1 <= kListCap;
     if (tid < min(p.n_stop, kStopsKept)) sh.stop[tid] = p.stop_ids[tid];
-    if (tid >= 64 && tid < 64 + K) {
-        const int b = tid - 64;
-        sh.lse[b] = sh.done[b] ? 0.0 : __ldcg(p.ws.lse + row0 + b);
+    if (p.merge_rows) {
+        if (tid < K) sh.lse[tid] = sh.done[tid] ? 0.0 : __ldcg(p.ws.lse + row0 + tid);
+    } else {
+        for (int b = tid >> 5; b < K; b += kBWarps) {
+            if (sh.done[b] || !(sh.score[b] > -INFINITY)) continue;
+            double sum, lse;
+            row_sum(p, row0 + b, &sum, &lse);
+            // A NaN sum (a NaN or +infinity in the row), or none, offers nothing: its offers are NaN.
+            if ((tid & 31) == 0) sh.lse[b] = sum > 0.0 ? lse : nan("");
+        }
     }
-    if (tid == 0) sh.count = K * K;
+    if (tid == 0) sh.count = n;
     auto offer = [&](int b, u64 key) { return (double)sh.score[b] + ((double)key_value(key) - sh.lse[b]); };
-    for (int e0 = 0; e0 < K * K; e0 += kBThreads) {
-        const int e = e0 + tid, b = e / K, i = e - b * K;
-        const bool mine = e < K * K;
-        const u64 k = mine && !sh.done[b] ? __ldcg(p.ws.best + row0 * K + e) : 0;
+    for (int e0 = 0; e0 < n; e0 += kBThreads) {
+        const int e = e0 + tid, b = e / per, i = e - b * per;
+        const bool mine = e < n;
+        const u64 k = mine && !sh.done[b] ? __ldcg(lists + e) : 0;
         if (e0 == 0) __syncthreads();
         if (!mine) break;
         if (kept) keys[e] = k;
         double score = -INFINITY;
-        if (k) score = offer(b, k);
-        else if (i == 0 && sh.done[b]) score = sh.score[b];
+        if (sh.done[b] ? i == 0 : !(sh.score[b] > -INFINITY)) score = sh.score[b];
+        else if (k) score = offer(b, k);
         if (p.alpha != 0.0) score /= sh.size[b];
-        sh.list[e] = score > -INFINITY ? (order_of(score) & ~4095ull) | (u64)(4095 - e) : 0;
+        sh.list[e] = score > -INFINITY ? (order_of(score) & ~8191ull) | (u64)(8191 - e) : 0;
     }
     block_select(K);
-    if (tid >= K) return;
-    const int64_t r = row0 + tid;
-    const u64 pick = sh.best[tid];
-    const bool nothing = pick == 0;
-    const int e = 4095 - (int)(pick & 4095), b = nothing ? tid : e / K;
-    const bool fresh = !nothing && !sh.done[b];
-    u64 key = 0;
-    if (fresh) key = kept ? keys[e] : __ldcg(p.ws.best + row0 * K + e);
-    const int token = fresh ? key_token(key) : p.pad;
-    bool stop = false;
-    if (fresh) {
-        for (int i = 0; i < min(p.n_stop, kStopsKept); ++i) stop |= sh.stop[i] == token;
-        for (int i = kStopsKept; i < p.n_stop; ++i) stop |= p.stop_ids[i] == token;
+    if (tid < K) {
+        const int64_t r = row0 + tid;
+        const u64 pick = sh.best[tid];
+        const bool nothing = pick == 0;
+        const int e = 8191 - (int)(pick & 8191), b = nothing ? tid : e / per;
+        const bool fresh = !nothing && !sh.done[b];
+        u64 key = 0;
+        if (fresh) key = kept ? keys[e] : __ldcg(lists + e);
+        const int token = fresh ? key_token(key) : p.pad;
+        bool stop = false;
+        if (fresh) {
+            for (int i = 0; i < min(p.n_stop, kStopsKept); ++i) stop |= sh.stop[i] == token;
+            for (int i = kStopsKept; i < p.n_stop; ++i) stop |= p.stop_ids[i] == token;
+        }
+        if (p.move_rings) {
+            sh.parent[tid] = b;
+            sh.token[tid] = token;
+            const int at = p.pos_in[row0 + b] % p.window;
+            sh.pos[tid] = at < 0 ? at + p.window : at;
+            sh.held[tid] = p.count_in[row0 + b];
+            sh.slot[tid] = fresh ? sh.pos[tid] : -1;
+        }
+        p.tokens[r] = token;
+        p.parents[r] = b;
+        p.scores[r] = nothing ? -INFINITY : fresh ? (float)offer(b, key) : sh.score[b];
+        p.lengths[r] = sh.old[b] + fresh;
+        p.finished[r] = nothing ? 0 : fresh ? stop : 1;
+        p.ws.push[r] = fresh;
     }
-    p.tokens[r] = token;
-    p.parents[r] = b;
-    p.scores[r] = nothing ? -INFINITY : fresh ? (float)offer(b, key) : sh.score[b];
-    p.lengths[r] = sh.old[b] + fresh;
-    p.finished[r] = nothing ? 0 : fresh ? stop : 1;
-    p.ws.push[r] = fresh;
+    if (!p.move_rings) return;
+    // The rings, and AddToHistory (Sampler.pas:530-539) of the new tokens: as many columns of all
+    // beams at a time as the list's room holds, read before any is written.
+    const int W = p.window, most = (int)(sizeof(sh.list) / 4) / K;
+    int32_t* stage = reinterpret_cast<int32_t*>(sh.list);
+    for (int j0 = 0; j0 < W; j0 += most) {
+        const int c = min(most, W - j0);
+        __syncthreads();
+        for (int i = tid; i < K * c; i += kBThreads)
+            stage[i] = p.hist_in[(row0 + sh.parent[i / c]) * W + j0 + i % c];
+        __syncthreads();
+        for (int i = tid; i < K * c; i += kBThreads) {
+            const int k = i / c, j = j0 + i % c;
+            p.hist[(row0 + k) * W + j] = sh.slot[k] == j ? sh.token[k] : stage[i];
+        }
+    }
+    if (tid < K) {
+        const bool push = sh.slot[tid] >= 0;
+        const int held = sh.held[tid];
+        p.pos[row0 + tid] = push ? (sh.pos[tid] + 1) % W : sh.pos[tid];
+        p.count[row0 + tid] = push && held < W ? max(held, 0) + 1 : held;
+    }
 }
 
 template <typename T, bool PEN>
@@ -591,45 +650,38 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
         block_select(K);
         if (tid < K) p.ws.cand[slot * K + tid] = sh.best[tid];
     }
-    // The row's last CTA merges its chunks.
     __syncthreads();
-    if (tid == 0) sh.flag = count_in(&p.ws.row_done[row]) == (uint32_t)p.chunks - 1;
+    const int group = p.merge_rows ? K : K * p.chunks;  // that are counted for a prompt
+    if (p.merge_rows) {
+        // The row's last CTA merges its chunks.
+        if (tid == 0) sh.flag = count_in(&p.ws.row_done[row]) == (uint32_t)p.chunks - 1;
+        __syncthreads();
+        if (!sh.flag) return;
+        if (live) {
+            const int n = p.chunks * K;
+            if (tid == 0) sh.count = n;
+            if (warp == kBWarps - 1) {
+                double sum, lse;
+                row_sum(p, row, &sum, &lse);
+                if (lane == 0) p.ws.lse[row] = sum > 0.0 ? lse : nan("");
+            }
+            // Empty places have key 0 and stay below every entry.
+            for (int i = tid; i < n; i += kBThreads) sh.list[i] = __ldcg(p.ws.cand + (int64_t)row * n + i);
+            block_select(K);
+            if (tid < K) p.ws.best[(int64_t)row * K + tid] = sh.best[tid];
+        }
+        __syncthreads();
+        if (tid == 0) p.ws.row_done[row] = 0;
+    }
+    if (tid == 0) sh.flag = count_in(&p.ws.prompt_done[prompt]) == (uint32_t)group - 1;
     __syncthreads();
     if (!sh.flag) return;
-    if (p.alpha != 0.0 && tid >= 64 && tid < 64 + K) {
-        // For the prompt's last CTA, and beside the loads below.
-        const int b = tid - 64;
+    if (tid == 0) p.ws.prompt_done[prompt] = 0;
+    if (p.alpha != 0.0 && tid >= kBThreads - K) {
+        const int b = tid - (kBThreads - K);
         sh.size[b] = pow((double)max(sh.done[b] ? sh.old[b] : sh.old[b] + 1, 1), p.alpha);
     }
-    if (live) {
-        const int n = p.chunks * K;
-        if (tid == 0) sh.count = n;
-        if (warp == kBWarps - 1) {
-            const double2* part = reinterpret_cast<const double2*>(p.ws.part) + (int64_t)row * p.chunks;
-            const double2 zero = make_double2(-INFINITY, 0.0);
-            const double2 a = lane < p.chunks ? __ldcg(part + lane) : zero;
-            const double2 b = lane + 32 < p.chunks ? __ldcg(part + lane + 32) : zero;
-            float M = (float)fmax(a.x, b.x);  // maxima of fp32 values
-            for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(FULLMASK, M, d));
-            double S = a.y * ex2(((float)a.x - M) * kLog2e) + b.y * ex2(((float)b.x - M) * kLog2e);
-            for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(FULLMASK, S, d);
-            // A NaN sum (a NaN or +infinity in the row), or none, offers nothing.
-            if (lane == 0) p.ws.lse[row] = M + log(S), sh.total = S;
-        }
-        // Empty places have key 0 and stay below every entry.
-        for (int i = tid; i < n; i += kBThreads) sh.list[i] = __ldcg(p.ws.cand + (int64_t)row * n + i);
-        block_select(K);
-        if (tid < K) p.ws.best[(int64_t)row * K + tid] = sh.total > 0.0 ? sh.best[tid] : 0;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        p.ws.row_done[row] = 0;
-        sh.flag = count_in(&p.ws.prompt_done[prompt]) == (uint32_t)K - 1;
-    }
-    __syncthreads();
-    if (!sh.flag) return;
     select_prompt(p, prompt);
-    if (tid == 0) p.ws.prompt_done[prompt] = 0;
 }
 
 constexpr int kRThreads = 128;
@@ -649,7 +701,7 @@ struct ReorderParams {
 };
 
 // Bound by the bytes: two caches of 64 rows x 4 heads x 2500 x 256 bf16 and their rings move in
-// 171 us (0.66 GB written; parents that beams share are read once from memory and then from L2).
+// 160 us (0.66 GB written; parents that beams share are read once from memory and then from L2).
 //
 // A thread owns one word of every row of a prompt: it reads the parents' words, then
 // writes, so a cache may be moved in place without a second buffer or a barrier.
@@ -747,6 +799,11 @@ void beam_plan(int rows, int vocab, int sm_count, int* chunks, int* chunk) {
 }
 
 cudaError_t beam_select(const BeamArgs& a, cudaStream_t stream) {
+    BeamArgs p = a;
+    // One merge for a prompt while its lists are short; else the rows' first, which run beside one
+    // another (2 x 10 of 262144 fp32, 2200 entries: 14.7 us with two merges, 17.4 with one; 16 x 4
+    // of 262144 bf16, 96 entries: 18.4 and 17.1).
+    p.merge_rows = (int64_t)a.beams * a.chunks * a.beams > kOneMerge;
     const bool pen = a.window > 0 && a.penalty != 1.0f;
     const size_t smem = sizeof(SelectShared) + (pen ? (size_t)a.chunk / 8 + (size_t)a.window * 8 : 0);
     const int grid = a.batch * a.beams * a.chunks;
@@ -756,13 +813,13 @@ cudaError_t beam_select(const BeamArgs& a, cudaStream_t stream) {
     static SmemLimit limit[4];
     cudaError_t e = limit[2 * half + pen].raise(kern, smem);
     if (e != cudaSuccess) return e;
-    kern<<<grid, kBThreads, smem, stream>>>(a);
+    kern<<<grid, kBThreads, smem, stream>>>(p);
     return cudaGetLastError();
 }
 
 cudaError_t beam_reorder(const BeamArgs& a, bool behind_select, const BeamCacheArgs* caches, int n_caches,
                          cudaStream_t stream, int* launches) {
-    bool rings = behind_select && a.window > 0;
+    bool rings = behind_select && a.window > 0 && !a.move_rings;
     const size_t smem = (size_t)a.beams * kRThreads * 16;
     static SmemLimit limit;
     cudaError_t e = limit.raise(beam_reorder_kernel, smem);

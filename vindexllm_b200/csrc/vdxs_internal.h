@@ -219,8 +219,12 @@ struct BeamArgs {
     const int32_t* stop_ids = nullptr;
     int n_stop = 0;
     int32_t *tokens = nullptr, *parents = nullptr;
+    bool merge_rows = false;  // set by beam_select: each row's chunks are merged before the prompt
+    bool move_rings = false;  // the selection moves the rings itself
     BeamWorkspace ws;
 };
+// Rings up to this length are moved by the selection where a step has no caches to move.
+constexpr int kBeamShortWindow = 1024;
 struct BeamCacheArgs {  // vdxs_beam_cache
     const unsigned char* src = nullptr;
     unsigned char* dst = nullptr;
@@ -231,7 +235,7 @@ constexpr int kBeamMaxChunks = 64;
 constexpr int kBeamMaxVocab = 8000000;  // kBeamMaxChunks chunks of the longest kind
 void beam_plan(int rows, int vocab, int sm_count, int* chunks, int* chunk);
 cudaError_t beam_select(const BeamArgs& a, cudaStream_t stream);
-// Caches by a.parents; behind a beam_select on the same stream also the rings (a.window > 0).
+// Caches by a.parents; behind a beam_select on the same stream also the rings that it left.
 cudaError_t beam_reorder(const BeamArgs& a, bool behind_select, const BeamCacheArgs* caches, int n_caches,
                          cudaStream_t stream, int* launches);
 // Device-resident decode state (one thread per row).
