@@ -286,6 +286,46 @@ def test_long_rings(gpu_ctx, vocab, window, held, kind):
         search.close()
 
 
+def test_the_same_bits_every_time(gpu_ctx):
+    """Penalised tokens reach threads in the order of atomics: scores are the same bits all the same, and
+    so are the offers next to one another."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    vocab, beams, window = 30000, 8, 600
+    x = torch.randn(3 * beams, vocab, device="cuda", generator=torch.Generator("cuda").manual_seed(5))
+    s = _state(3, beams, window, vocab, 11)
+    s["hist"] = np.random.default_rng(1).integers(0, 700, s["hist"].shape).astype(np.int32)
+    s["count"][:] = window
+    search, first = BeamSearch(gpu_ctx, 3, beams, vocab), None
+    for _ in range(20):
+        out = _device(s, 3, beams, window)
+        tokens, parents = search.step(_device(s, 3, beams, window), x, out=out, repeat_penalty=1.3, length_alpha=0.5)
+        now = [tokens, parents, out.scores, out.hist]
+        first = first or now
+        assert all(torch.equal(a, b) for a, b in zip(now, first))
+    search.close()
+
+
+def test_penalised_values_that_go_wrong(gpu_ctx):
+    """NaN, infinities and masks among the penalised tokens: as anywhere in the row."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    vocab, beams = 9000, 4
+    for value in (np.nan, np.inf, -np.inf, np.finfo(np.float32).min, 3e38):
+        x = np.random.default_rng(3).standard_normal((beams, vocab)).astype(np.float32)
+        s = _state(1, beams, 6, vocab, 5)
+        s["finished"][:] = 0
+        s["scores"][:] = [-1, -1.5, -2, -2.5]
+        s["hist"][:] = [5, 17, 5, 8999, -3, vocab]
+        s["count"][:] = 6
+        x[1, [5, 8999]] = value
+        want = ref.beam_step(x, 1, beams, s, (), 0, 1.5, 0.0)
+        search, out = BeamSearch(gpu_ctx, 1, beams, vocab), _device(s, 1, beams, 6)
+        got = search.step(_device(s, 1, beams, 6), torch.as_tensor(x, device="cuda"), out=out, repeat_penalty=1.5)
+        _check((*got, out), want, 1, beams)
+        search.close()
+
+
 def test_many_stop_ids(gpu_ctx):
     import torch
     from vindexllm_b200.sampler import BeamSearch

@@ -281,11 +281,11 @@ def test_product_strides_and_untouched_logits(gpu_ctx):
     scales.zero_()
     qb = _ints(batch, 320, 4)
     for dtype, off in ((torch.float32, 0), (torch.float32, 1), (torch.bfloat16, 1), (torch.bfloat16, 2)):
-        lb = torch.full((batch, n + 7), 5.0, dtype=dtype, device="cuda")
-        out = lb[:, off:off + n]
+        lb = torch.full((batch + 3, n + 7), 5.0, dtype=dtype, device="cuda")
+        out = lb[:batch, off:off + n]
         got = w.unembed(_t(qb)[:, 16:16 + k], _t(xs), logits=out)
         _check_product(got, qb[:, 16:16 + k], xs, wb[:, 3:3 + k], ws)
-        assert (lb[:, :off] == 5).all() and (lb[:, off + n:] == 5).all()
+        assert (lb[:, :off] == 5).all() and (lb[:, off + n:] == 5).all() and (lb[batch:] == 5).all()
     w.close()
 
 

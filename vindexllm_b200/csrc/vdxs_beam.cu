@@ -16,7 +16,7 @@
 //
 // What bounds it: with many rows the logits' bytes (512 rows of 262144 fp32 in 93 us, 5.8 TB/s,
 // 0.89 of the copy rate), with few the chain of dependent steps behind the stream (64 rows of
-// bf16 with rings in 25 us, of which the logits take 6; 4 rows of 32000 in 8.7 us): bound,
+// bf16 with rings in 26.5 us, of which the logits take 6; 4 rows of 32000 in 8.7 us): bound,
 // elements, selection, and a merge or two, each a count, loads and a selection. Notes of group maxima instead of a list that the stream itself fills took
 // the 512 rows from 177 to 97 us: the list's code cost the loop its registers.
 #include "vdxs_internal.h"
@@ -86,6 +86,11 @@ struct SelectShared {
     u64 bound;
     int count, extra, reach;
     uint32_t marked;  // tiles with marks
+    // The penalised tokens' maximum (in key order; 0: none), their sum of exponentials relative to it
+    // in units of 2^-40, and whether one of them is NaN or +infinity.
+    uint32_t held_max;
+    int held_bad;
+    u64 held_sum;
     int flag;
     float fbound;
     float2 sums[kBThreads];  // each thread's maximum, and its sum of exponentials relative to that
@@ -501,7 +506,7 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
         float my_value = 0.0f;
         if (PEN) {
             const int count = p.count_in[row];
-            if (tid == 0) sh.extra = 0, sh.marked = 0;
+            if (tid == 0) sh.extra = 0, sh.marked = 0, sh.held_max = 0, sh.held_bad = 0, sh.held_sum = 0;
             for (int i = tid; i < p.chunk / 32; i += kBThreads) marks[i] = 0;
             int token = tid < p.window ? ring[tid] : -1;
             __syncthreads();
@@ -570,6 +575,8 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
         }
         const int extras = PEN ? sh.extra : 0;
         if (PEN) {
+            // Which thread has which token hangs on the order of atomics, so they are summed in whole
+            // numbers.
             if (my_place >= 0) extra[my_place].value = my_value;  // fetched while the stream ran
             __syncthreads();
             for (int i = tid; i < extras; i += kBThreads) {
@@ -583,8 +590,15 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
                 }
                 for (; times > 0; --times) v = v > 0.0f ? __fdiv_rn(v, p.penalty) : __fmul_rn(v, p.penalty);
                 extra[i].value = v;
-                if (v > m) s *= ex2((m - v) * kLog2e), m = v;
-                s += ex2((v - m) * kLog2e);
+                if (!(v < INFINITY)) sh.held_bad = 1;
+                else if (v > -INFINITY) atomicMax(&sh.held_max, (uint32_t)(make_key(v, 0) >> 32));
+            }
+            __syncthreads();
+            const float top = key_value((u64)sh.held_max << 32);
+            for (int i = tid; i < extras; i += kBThreads) {
+                const float v = extra[i].value;
+                if (extra[i].held >= 0 && v > -INFINITY && v < INFINITY)
+                    atomicAdd(&sh.held_sum, (u64)(ex2((v - top) * kLog2e) * 1099511627776.0f));
             }
         }
         sh.sums[tid] = make_float2(m, s);
@@ -613,6 +627,12 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
 #pragma unroll
             for (int j = 0; j < kBWarps; ++j) S += (double)part[j].y * ex2((part[j].x - M) * kLog2e);
             for (int d = 16; d > 0; d >>= 1) S += __shfl_xor_sync(FULLMASK, S, d);
+            if (PEN && sh.held_sum > 0) {
+                const float top = key_value((u64)sh.held_max << 32), both = fmaxf(M, top);
+                S = S * ex2((M - both) * kLog2e) + (double)sh.held_sum * 9.094947017729282e-13 * ex2((top - both) * kLog2e);
+                M = both;
+            }
+            if (PEN && sh.held_bad) S = nan("");
             if (lane == 0) reinterpret_cast<double2*>(p.ws.part)[slot] = make_double2(M, S);
         }
         const int reach = sh.reach;
