@@ -77,15 +77,15 @@ def _stream_on(device: int, stream) -> int:
     return _raw_stream(device)
 
 
-def _output(like, shape, dtype, stream):
+def _output(like, dtype, stream, *shape):
     """An output on the device of `like`. With a stream of the caller's it is allocated under that
     one, so that its memory is reused in that stream's order."""
     if stream is not None:
         import torch
         with torch.cuda.stream(stream):
             return like.new_empty(shape, dtype=dtype)
-    # Without the keyword the call takes half the time.
-    return like.new_empty(shape) if like.dtype is dtype else like.new_empty(shape, dtype=dtype)
+    # Sizes one by one and no keyword: 1.3 us a call instead of 2.2.
+    return like.new_empty(*shape) if like.dtype is dtype else like.new_empty(*shape, dtype=dtype)
 
 
 def _need(t, what: str, device: int, dtype, shape):
@@ -208,18 +208,18 @@ class SamplerContext:
         if residual is not None:
             rp = _matrix(residual, "residual", dev, dtype, shape)
             if out_hidden is None:
-                out_hidden, hp = _output(x, shape, dtype, stream), dim
+                out_hidden, hp = _output(x, dtype, stream, rows, dim), dim
         if out_hidden is not None and not hp:
             hp = _matrix(out_hidden, "out_hidden", dev, dtype, shape)
         if q is None:
             qp = -(-dim // 16) * 16
-            q = _output(x, (rows, qp), torch.int8, stream)
+            q = _output(x, torch.int8, stream, rows, qp)
             if qp != dim:
                 q = q[:, :dim]
         else:
             qp = _matrix(q, "q", dev, torch.int8, shape)
         if scale is None:
-            scale = _output(weight, rows, torch.float32, stream)
+            scale = _output(weight, torch.float32, stream, rows)
         else:
             _need(scale, "scale", dev, torch.float32, (rows,))
         rc = self.lib.vdxs_rms_norm_i8(self._h, x.data_ptr(), pitch, _ptr(residual), rp, code, weight.data_ptr(), wcode,
@@ -583,7 +583,7 @@ class I8Weights:
             qp = -(-self.in_dim // 16) * 16
         _need(scale, "scale", dev, torch.float32, (batch,))
         if logits is None:
-            logits, pitch = _output(scale, (batch, n), dtype or torch.float32, stream), n
+            logits, pitch = _output(scale, dtype or torch.float32, stream, batch, n), n
         else:
             pitch = _matrix(logits, "logits", dev, dtype, (batch, n))
         rc = self.lib.vdxs_unembed_i8(self.ctx._h, self._h, q.data_ptr(), qp, scale.data_ptr(), batch, logits.data_ptr(),
@@ -604,7 +604,7 @@ class I8Weights:
         hp = 0 if out_hidden is None else _matrix(out_hidden, "out_hidden", dev, x.dtype, shape)
         _need(norm_weight, "norm_weight", dev, None, (self.in_dim,))
         if tokens is None:
-            tokens = _output(x, batch, torch.int32, stream)
+            tokens = _output(x, torch.int32, stream, batch)
         for t, what, dtype in ((uniforms, "uniforms", torch.float32), (history_count, "history_count", torch.int32),
                                (tokens, "tokens", torch.int32)):
             if t is not None:
@@ -754,11 +754,11 @@ class BeamSearch:
             _need(stop_ids, "stop_ids", dev, i32, None)
             n_stop = stop_ids.numel()
         if tokens is None:
-            tokens = _output(state.finished, shape, i32, stream)
+            tokens = _output(state.finished, i32, stream, batch, beams)
         else:
             _need(tokens, "tokens", dev, i32, shape)
         if parents is None:
-            parents = _output(state.finished, shape, i32, stream)
+            parents = _output(state.finished, i32, stream, batch, beams)
         else:
             _need(parents, "parents", dev, i32, shape)
         cfg = abi.VdxsBeamConfig(length_alpha, repeat_penalty, state.window, pad_token, 0)
