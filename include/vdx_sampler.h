@@ -408,9 +408,9 @@ VDXS_API int32_t vdxs_sample_unembed_q4_0(vdxs_context* ctx, const vdxs_config* 
  *   y = h * weight / sqrt(mean(h^2) + eps)
  *   scale[row] = max|y| / 127 (fp32),  q = y / (max|y| / 127) rounded to nearest even
  * Sums and the values next to a rounding border are taken in 64 bits, so q is the exact
- * rounding of the row's values. A row of zeros has scale 0 and q 0; a row that holds a
- * NaN or an infinity (in x, the residual or the weights) has scale NaN and q 0, so the
- * logits made from it are NaN.
+ * rounding of the row's values. A row of zeros has scale 0 and q 0, also
+ * where eps is 0; a row that holds a NaN or an infinity (in x, the residual or the weights)
+ * has scale NaN and q 0, so the logits made from it are NaN.
  *   d_x           [rows, x_stride] dtype F32, BF16 or F16 (first `dim` used)
  *   d_residual    [rows, residual_stride] of the same type, or NULL
  *   d_weight      [dim], weight_dtype F32, BF16 or F16

@@ -172,6 +172,21 @@ def test_norm_values_on_the_edge(gpu_ctx):
     assert (q == 0).all()
 
 
+@pytest.mark.parametrize("dim", [64, 254, 8200])
+def test_norm_of_zeros_without_eps(gpu_ctx, dim):
+    """Rows and weights of zeros have scale 0 where eps is 0 too, whatever stands beside them."""
+    import torch
+    x = _hidden(4, dim, 3, "f32")
+    x[1] = 0.0
+    w = torch.ones(dim, device="cuda")
+    q, scale, _ = gpu_ctx.rms_norm_i8(x, w, 0.0)
+    assert scale[1] == 0 and (q[1] == 0).all()
+    rest = torch.tensor([0, 2, 3], device="cuda")
+    _check_norm(q[rest], scale[rest], x[rest], w, 0.0)
+    q, scale, _ = gpu_ctx.rms_norm_i8(x, torch.zeros_like(w), 0.0)
+    assert (scale == 0).all() and (q == 0).all()
+
+
 def _ints(rows, k, seed, room=None):
     rng = np.random.default_rng(seed)
     return rng.integers(-128, 128, size=(rows, room or k)).astype(np.int8)

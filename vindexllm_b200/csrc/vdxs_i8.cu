@@ -83,7 +83,9 @@ __device__ __noinline__ void norm_row(const NormI8Args& p, int64_t row, bool don
     block_sum_max(sum, top);
     bad = __syncthreads_or(bad);
     if (threadIdx.x == 0)
-        p.scale[row] = bad ? nanf("") : (float)(top / 127.0 * (1.0 / sqrt(sum / p.dim + (double)p.eps)));
+        p.scale[row] = bad         ? nanf("")
+                       : top > 0.0 ? (float)(top / 127.0 * (1.0 / sqrt(sum / p.dim + (double)p.eps)))
+                                   : 0.0f;  // (zeros without eps too)
     int8_t* q = p.q + row * p.q_stride;
     const float f = (float)(127.0 / top);
     for (int i = threadIdx.x; i < p.dim; i += blockDim.x) {
