@@ -484,6 +484,7 @@ VDXS_API int32_t vdxs_sample_unembed_i8(vdxs_context* ctx, const vdxs_config* cf
  *     logits of -infinity are never offered (a mask), and a row that holds a NaN or
  *     +infinity, or whose logits are all -infinity, offers nothing;
  *   - a finished beam offers itself, with its score and length, and its logits are not read;
+ *   - an offer whose score or quotient below is NaN or -infinity is none;
  *   - the `beams` offers with the highest score / max(length, 1)^length_alpha stay, in that
  *     order (equal ones: the lower beam, then the beam's own order).
  * Log-probabilities and the order of the offers are taken in 64 bits (exponentials in fp32;
@@ -495,7 +496,7 @@ VDXS_API int32_t vdxs_sample_unembed_i8(vdxs_context* ctx, const vdxs_config* cf
 typedef struct vdxs_beam vdxs_beam;
 
 typedef struct vdxs_beam_config {  /* 24 bytes */
-    double  length_alpha;    /* 0 = order by score alone; any finite value             */
+    double  length_alpha;    /* 0 = order by score alone; within +-1e6                 */
     float   repeat_penalty;  /* 1 = off; as vdxs_config (needs the rings)              */
     int32_t window;          /* ring length; 0 = no rings                              */
     int32_t pad_token;       /* token of finished beams and of slots without an offer  */

@@ -326,6 +326,41 @@ def test_penalised_values_that_go_wrong(gpu_ctx):
         search.close()
 
 
+@pytest.mark.parametrize("alpha", [0.0, 0.7, -1e6])
+def test_scores_that_go_wrong(gpu_ctx, alpha):
+    """Beams with a score of NaN or -infinity, finished or not, are never a parent, nor are those
+    whose quotient is (alpha -1e6: a length above 1 divides by 0); slots without an offer keep
+    their length."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    batch, beams, vocab = 4, 5, 700
+    s = _state(batch, beams, 0, vocab, 21)
+    sc, done = s["scores"].reshape(batch, beams), s["finished"].reshape(batch, beams)
+    done[:] = [0, 1, 0, 1, 0]
+    sc[:] = -3.0
+    sc[0, :2] = np.nan
+    sc[1, 2:] = -np.inf
+    sc[2] = np.nan
+    sc[3] = -np.inf
+    search = BeamSearch(gpu_ctx, batch, beams, vocab)
+    x = torch.as_tensor(np.random.default_rng(22).standard_normal((batch * beams, vocab)).astype(np.float32), device="cuda")
+    tokens, parents = search.step(now := _device(s, batch, beams, 0), x, length_alpha=alpha, pad_token=9)
+    t, p, out = tokens.cpu().numpy(), parents.cpu().numpy(), now.scores.reshape(batch, beams).cpu().numpy()
+    length = s["lengths"].reshape(batch, beams)
+    assert not np.isnan(out).any()
+    for g in range(batch):
+        fine = [b for b in range(beams) if sc[g, b] > -np.inf and (alpha > -1e6 or length[g, b] + 1 - done[g, b] < 2)]
+        offers = sum(1 if done[g, b] else beams for b in fine)
+        for k in range(beams):
+            if k < offers:
+                assert p[g, k] in fine and np.isfinite(out[g, k])
+            else:
+                assert p[g, k] == k and t[g, k] == 9 and out[g, k] == -np.inf
+                assert now.finished.reshape(batch, beams)[g, k] == 0
+                assert now.lengths.reshape(batch, beams)[g, k] == length[g, k]
+    search.close()
+
+
 def test_many_stop_ids(gpu_ctx):
     import torch
     from vindexllm_b200.sampler import BeamSearch
