@@ -15,12 +15,13 @@
 // on 1e-8 and not on 1e-6; scores are stored in fp32.
 //
 // What bounds it: with many rows the logits' bytes and the selection behind each chunk's stream
-// (512 rows of 262144 fp32 of which 15 % are finished and not read: 444 MB in 93 us, 4.7 TB/s;
+// (512 rows of 262144 fp32 of which 15 % are finished and not read: 444 MB in 92 us, 4.8 TB/s;
 // the stream alone takes 75, 5.9 TB/s or 0.92 of the copy rate; deeper rings in shared memory
-// and a fetch of the next chunk into L2 changed neither), with few the chain of dependent steps behind the stream (64 rows of
-// bf16 with rings in 26.5 us, of which the logits take 6; 4 rows of 32000 in 8.7 us): bound,
-// elements, selection, and a merge or two, each a count, loads and a selection. Notes of group maxima instead of a list that the stream itself fills took
-// the 512 rows from 177 to 97 us: the list's code cost the loop its registers.
+// and a fetch of the next chunk into L2 changed neither). With few rows the chain of dependent
+// steps behind the stream (64 rows of bf16 with rings in 26.5 us, of which the logits take 6; 4
+// rows of 32000 in 8.7 us): bound, elements, selection, and a merge or two, each a count, loads
+// and a selection. Notes of group maxima instead of a list that the stream itself fills took the
+// 512 rows from 177 to 97 us: the list's code cost the loop its registers.
 #include "vdxs_internal.h"
 #include "../../include/vdx_sampler.h"
 
