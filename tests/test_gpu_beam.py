@@ -361,6 +361,47 @@ def test_scores_that_go_wrong(gpu_ctx, alpha):
     search.close()
 
 
+@pytest.mark.parametrize("batch,beams,vocab", [(2, 12, 1000), (1, 4, 32000), (1, 30, 700), (3, 64, 300)])
+@pytest.mark.parametrize("alpha", [-306.0, -305.5, 306.0])
+def test_quotients_of_every_magnitude(gpu_ctx, batch, beams, vocab, alpha):
+    """More than 96 offers whose quotients reach 2e307 or down to 1e-305: finite, so none is lost, and
+    in their order. The scores stand far enough apart (checked here) that rounding cannot
+    exchange two picks."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    rows = batch * beams
+    rng = np.random.default_rng(beams)
+    x = (2 * rng.standard_normal((rows, vocab))).astype(np.float32)
+    s = dict(scores=rng.permutation(np.linspace(-16, -12, rows)).astype(np.float32),
+             lengths=np.full(rows, 9, np.int32), finished=np.zeros(rows, np.int32))
+    s["lengths"][1], s["finished"][1] = 10, 1
+    want = ref.beam_step(x, batch, beams, s, (), 5, 1.0, alpha)
+    for g in range(batch):
+        best = np.sort(list(want[4][g].values()))[::-1][:beams + 1] * 10.0 ** alpha
+        assert len(best) == beams + 1 and np.isfinite(best).all() and np.diff(-best).min() > 2 * (ATOL + 16 * RTOL)
+    search, out = BeamSearch(gpu_ctx, batch, beams, vocab), _device(s, batch, beams, 0)
+    tokens, parents = search.step(_device(s, batch, beams, 0), torch.as_tensor(x, device="cuda"), out=out, pad_token=5,
+                                  length_alpha=alpha)
+    assert np.array_equal(tokens.cpu().numpy(), want[0]) and np.array_equal(parents.cpu().numpy(), want[1])
+    assert torch.isfinite(out.scores).all()
+    search.close()
+
+
+def test_quotients_next_to_zero(gpu_ctx):
+    """Finished beams whose quotients are subnormal and negative: they stay, in their order."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch
+    beams = 12
+    order = np.random.default_rng(1).permutation(beams)
+    s = dict(scores=(-1e-9 * (1 + order)).astype(np.float32), lengths=np.full(beams, 10, np.int32),
+             finished=np.ones(beams, np.int32))
+    search, out = BeamSearch(gpu_ctx, 1, beams, 500), _device(s, 1, beams, 0)
+    tokens, parents = search.step(_device(s, 1, beams, 0), torch.zeros(beams, 500, device="cuda"), out=out, pad_token=5,
+                                  length_alpha=306.0)
+    assert (tokens == 5).all() and parents.cpu().numpy().tolist() == [np.argsort(order).tolist()]
+    assert np.array_equal(out.scores.cpu().numpy(), np.sort(s["scores"])[::-1])
+    search.close()
+
 def test_many_stop_ids(gpu_ctx):
     import torch
     from vindexllm_b200.sampler import BeamSearch

@@ -62,6 +62,10 @@ __device__ __forceinline__ float key_value(u64 k) {
     return __uint_as_float((u >> 31) ? u ^ 0x80000000u : ~u);
 }
 __device__ __forceinline__ int key_token(u64 k) { return (int)~(uint32_t)k; }
+// The order of fp32 values without NaN as that of whole numbers (the upper half of their keys), and
+// back.
+__device__ __forceinline__ uint32_t order_of(float v) { return (uint32_t)(make_key(v, 0) >> 32); }
+__device__ __forceinline__ float order_value(uint32_t order) { return key_value((u64)order << 32); }
 // The order of doubles without NaN as that of whole numbers.
 __device__ __forceinline__ u64 order_of(double v) {
     const u64 u = (u64)__double_as_longlong(v + 0.0);
@@ -95,7 +99,7 @@ struct SelectShared {
     int held_bad;
     u64 held_sum;
     int flag;
-    float fbound;
+    uint32_t top_bound;
     float2 sums[kBThreads];  // each thread's maximum, and its sum of exponentials relative to that
     // The prompt's rows before the step.
     float score[VDXS_BEAM_MAX_BEAMS];
@@ -116,11 +120,11 @@ static_assert(kGroups * kPer <= kListCap, "a list holds the groups' elements");
 
 // How many of the n (a multiple of 4) values at p are above mine, or equal to it at a lower
 // place.
-__device__ __forceinline__ int count_above(const float* p, int n, float mine, int place) {
+__device__ __forceinline__ int count_above(const uint32_t* p, int n, uint32_t mine, int place) {
     int above = 0;
 #pragma unroll 4
     for (int j = 0; j < n; j += 4) {
-        const float4 o = *reinterpret_cast<const float4*>(p + j);
+        const uint4 o = *reinterpret_cast<const uint4*>(p + j);
         above += (o.x > mine || (o.x == mine && j < place)) + (o.y > mine || (o.y == mine && j + 1 < place)) +
                  (o.z > mine || (o.z == mine && j + 2 < place)) + (o.w > mine || (o.w == mine && j + 3 < place));
     }
@@ -128,16 +132,18 @@ __device__ __forceinline__ int count_above(const float* p, int n, float mine, in
 }
 
 // The K-th largest of 64 (K <= 16) or 128 disjoint groups' maxima, of one value per thread: a
-// lower bound of the K-th largest of what the values are the maxima of. In sh.fbound.
-__device__ __forceinline__ void block_bound(float v, int K) {
+// lower bound of the K-th largest of what the values are the maxima of. In sh.top_bound. The
+// values are upper halves of keys, compared as whole numbers: those of doubles (select_prompt) are
+// no fp32 values, and some of them would be NaN.
+__device__ __forceinline__ void block_bound(uint32_t v, int K) {
     SelectShared& sh = select_shared();
-    float* groups = reinterpret_cast<float*>(sh.maxima);
+    uint32_t* groups = reinterpret_cast<uint32_t*>(sh.maxima);
     const int tid = threadIdx.x, share = K <= 16 ? 4 : 2, n = kBThreads / share;
-    v = fmaxf(v, __shfl_xor_sync(FULLMASK, v, 1));
-    if (share == 4) v = fmaxf(v, __shfl_xor_sync(FULLMASK, v, 2));
+    v = max(v, __shfl_xor_sync(FULLMASK, v, 1));
+    if (share == 4) v = max(v, __shfl_xor_sync(FULLMASK, v, 2));
     if (tid % share == 0) groups[tid / share] = v;
     __syncthreads();
-    if (tid < n && count_above(groups, n, groups[tid], tid) == K - 1) sh.fbound = groups[tid];
+    if (tid < n && count_above(groups, n, groups[tid], tid) == K - 1) sh.top_bound = groups[tid];
     __syncthreads();
 }
 
@@ -178,8 +184,8 @@ __device__ __noinline__ void block_select(int K) {
     if (n > kListShort) {
         u64 mx = 0;
         for (int i = tid; i < n; i += kBThreads) mx = max(mx, sh.list[i]);
-        block_bound(mx ? key_value(mx) : -INFINITY, K);
-        const u64 bound = (make_key(sh.fbound, -1) >> 32) << 32;
+        block_bound((uint32_t)(mx >> 32), K);
+        const u64 bound = (u64)sh.top_bound << 32;
         if (n <= 2 * kBThreads) block_keep<2>(n, bound);
         else block_keep<kListCap / kBThreads>(n, bound);
         n = sh.count;
@@ -606,8 +612,8 @@ __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select
         }
         sh.sums[tid] = make_float2(m, s);
         if (tid == 0) sh.count = 0, sh.reach = 0;
-        block_bound(most, K);
-        const float tau = sh.fbound;
+        block_bound(order_of(most), K);
+        const float tau = order_value(sh.top_bound);
         // Eight tiles' maxima are compared before any is counted, so that their loads do not wait for an
         // atomic's answer, which a group at a time would: 93.9 -> 92.0 us at 64 x 8 of 262144 fp32.
         if (__any_sync(FULLMASK, most >= tau)) {
