@@ -534,6 +534,52 @@ def test_graph_and_side_stream(gpu_ctx):
         assert torch.equal(s1.scores, s2.scores) and torch.equal(s1.hist, s2.hist) and torch.equal(s1.count, s2.count)
 
 
+def test_two_host_threads(gpu_ctx):
+    """A context for each host thread: searches of different rings, beams and chunks step at once, each as it
+    does alone."""
+    import threading
+
+    import torch
+    from vindexllm_b200.sampler import BeamSearch, SamplerContext
+    shapes = [(1, 30, 9000, 700), (1, 64, 3000, 8192), (2, 5, 140000, 100), (1, 40, 70000, 3000)]
+
+    def steps(ctx, batch, beams, vocab, window, stream):
+        with torch.cuda.stream(stream):
+            g = torch.Generator("cuda").manual_seed(vocab)
+            x = torch.randn(batch * beams, vocab, device="cuda", generator=g)
+            search, out = BeamSearch(ctx, batch, beams, vocab), _device(_state(batch, beams, window, vocab, 9), batch, beams,
+                                                                        window)
+            cache = torch.arange(batch * beams * 64, device="cuda").view(batch * beams, 64)
+            got = []
+            for _ in range(5):
+                t, p = search.step(out, x, repeat_penalty=1.2, caches=[cache])
+                got += [t, p, out.scores.clone(), out.hist.clone(), cache.clone()]
+        torch.cuda.synchronize()
+        search.close()
+        return got
+
+    results, failures = [None] * len(shapes), []
+    gate = threading.Barrier(len(shapes))
+
+    def work(i):
+        try:
+            ctx, stream = SamplerContext(0), torch.cuda.Stream()
+            gate.wait(60)
+            results[i] = steps(ctx, *shapes[i], stream)
+            ctx.close()
+        except BaseException as e:  # noqa: BLE001
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(shapes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not failures, failures
+    for got, shape in zip(results, shapes):
+        want = steps(gpu_ctx, *shape, torch.cuda.Stream())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
 def test_norm_product_beam_run(gpu_ctx):
     """The tail of a decode step as a search runs it: norm, product and beam step, the step held to the
     restatement on the logits that the product gave."""

@@ -2,8 +2,8 @@
 // sm_100a kernels (vdxs_kernels.cu). Not part of the public ABI.
 #pragma once
 
-#include <atomic>
 #include <cstdint>
+#include <mutex>
 #include <string>
 
 #include <cuda_runtime.h>
@@ -171,18 +171,23 @@ struct I8Matrix {            // weights as the product reads them
 };
 // Makes w.map, once the other members are set.
 cudaError_t map_weights_i8(I8Matrix& w);
-// cudaFuncAttributeMaxDynamicSharedMemorySize of a kernel, raised once for each device.
+// cudaFuncAttributeMaxDynamicSharedMemorySize of a kernel on each device. It belongs to the process,
+// and contexts on other threads raise it too: check, call and note are one step, and it is
+// never lowered.
 struct SmemLimit {
-    std::atomic<int> have[64] = {};
+    std::mutex mu;
+    int have[64] = {};
     template <typename F>
     cudaError_t raise(F* kernel, size_t bytes) {
         if (bytes <= 48 * 1024) return cudaSuccess;
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
-        if (dev < 64 && have[dev].load(std::memory_order_relaxed) >= (int)bytes) return cudaSuccess;
+        if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+        std::lock_guard<std::mutex> lock(mu);
+        if (have[dev] >= (int)bytes) return cudaSuccess;
         e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e == cudaSuccess && dev < 64) have[dev].store((int)bytes, std::memory_order_relaxed);
+        if (e == cudaSuccess) have[dev] = (int)bytes;
         return e;
     }
 };
