@@ -449,7 +449,8 @@ VDXS_API int32_t vdxs_i8_release(vdxs_i8_weights* w);
  *   d_scale   [batch] fp32
  *   d_logits  [batch, logits_stride] (logits_stride >= out_dim); what lies between
  *             out_dim and logits_stride is not written
- * Uses no workspace and allocates nothing. */
+ * Uses no workspace and allocates nothing but the context's error word (4 bytes, with its
+ * first product or sampling call), so it may be captured at once. */
 VDXS_API int32_t vdxs_unembed_i8(vdxs_context* ctx, const vdxs_i8_weights* w, const int8_t* d_q,
                                  int64_t q_stride, const float* d_scale, int32_t batch,
                                  void* d_logits, int32_t dtype, int64_t logits_stride,

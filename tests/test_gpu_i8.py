@@ -397,6 +397,34 @@ def test_graph_replay_and_side_stream(gpu_ctx):
     ctx.close()
 
 
+def test_context_made_under_capture(gpu_ctx):
+    """Making a context touches no stream: a capture in global mode goes on around it, work of the
+    default stream is not waited for, and its first product may itself be captured."""
+    import torch
+    from vindexllm_b200.sampler import I8Weights, SamplerContext
+    k, n, batch = 64, 300, 3
+    wq, q = _ints(n, k, 1), _ints(batch, k, 2)
+    w, qt, xs = I8Weights(gpu_ctx, _t(wq), torch.ones(n, device="cuda")), _t(q), torch.ones(batch, device="cuda")
+    lg = torch.zeros(batch, n, device="cuda")
+    torch.cuda._sleep(1 << 29)  # a quarter of a second
+    mark = torch.cuda.Event()
+    mark.record()
+    held = SamplerContext(0)
+    assert not mark.query()
+    held.close()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, capture_error_mode="global"):
+        ctx = SamplerContext(0)
+        rc = ctx.lib.vdxs_unembed_i8(ctx.handle, w._h, qt.data_ptr(), k, xs.data_ptr(), batch, lg.data_ptr(), abi.DTYPE_F32,
+                                     n, torch.cuda.current_stream().cuda_stream)
+        assert rc == abi.OK
+    for _ in range(2):
+        lg.zero_()
+        g.replay()
+        ctx.device_status()
+        _check_product(lg, q, np.ones(batch), wq, np.ones(n))
+    w.close()
+
 def test_refusals(gpu_ctx):
     import torch
     from vindexllm_b200.sampler import I8Weights, VdxsError

@@ -214,14 +214,6 @@ VDXS_API int32_t vdxs_create(int32_t device, vdxs_context** out) {
         return fail(nullptr, VDXS_E_UNSUPPORTED, "device %d is compute capability %d.x; this library is built for sm_100a",
                     device, major);
     }
-    // The error word that kernels set instead of trapping.
-    if ((e = cudaMalloc((void**)&ctx->ws.err, sizeof(int32_t))) != cudaSuccess ||
-        (e = cudaMemset(ctx->ws.err, 0, sizeof(int32_t))) != cudaSuccess ||
-        (e = cudaStreamSynchronize(nullptr)) != cudaSuccess) {
-        cudaFree(ctx->ws.err);
-        delete ctx;
-        return cuda_fail(nullptr, e, "error word");
-    }
     *out = ctx;
     ok(ctx);
     return VDXS_OK;
@@ -1453,8 +1445,10 @@ VDXS_API int32_t vdxs_unembed_i8(vdxs_context* ctx, const vdxs_i8_weights* w, co
         return fail(ctx, VDXS_E_INVALID_ARG, "a pointer is not aligned to its element size");
     DeviceGuard g(ctx->device);
     int launches = 0;
-    const cudaError_t e = unembed_i8(w->m, d_q, q_stride, d_scale, batch, d_logits, dtype, logits_stride,
-                                     ctx->ws.err, ctx->sm_count, (cudaStream_t)stream, &launches);
+    cudaError_t e = ensure_error_word(ctx->ws);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "error word");
+    e = unembed_i8(w->m, d_q, q_stride, d_scale, batch, d_logits, dtype, logits_stride, ctx->ws.err, ctx->sm_count,
+                   (cudaStream_t)stream, &launches);
     ctx->launches += launches;
     if (e != cudaSuccess) return cuda_fail(ctx, e, "8-bit unembedding");
     ok(ctx);

@@ -133,6 +133,8 @@ struct LaunchPlan {
 // cudaErrorInvalidValue).
 cudaError_t plan_topk(const SampleArgs& a, int device_smem_optin, LaunchPlan* plan, std::string* err);
 cudaError_t plan_full(const SampleArgs& a, LaunchPlan* plan, std::string* err);
+// Makes the error word, cleared, where the context has none yet.
+cudaError_t ensure_error_word(Workspace& ws);
 cudaError_t ensure_workspace(Workspace& ws, const SampleArgs& a, const LaunchPlan& plan, int ranks,
                              cudaStream_t stream, std::string* err);
 cudaError_t launch_sample(const SampleArgs& a, const LaunchPlan& plan, Workspace& ws, std::string* err);

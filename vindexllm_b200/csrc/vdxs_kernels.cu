@@ -3594,15 +3594,34 @@ static cudaError_t grow(P** ptr, size_t* cap, size_t want, bool zero, cudaStream
     return cudaSuccess;
 }
 
+// The thread's capture mode is relaxed meanwhile, and the word is cleared on a stream of its own:
+// the call may itself be captured, disturbs no capture of another thread and waits for no
+// other work.
+cudaError_t ensure_error_word(Workspace& ws) {
+    if (ws.err) return cudaSuccess;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return e;
+    cudaStream_t own = nullptr;
+    int32_t* word = nullptr;
+    if ((e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking)) == cudaSuccess) {
+        if ((e = cudaMalloc((void**)&word, sizeof(int32_t))) == cudaSuccess &&
+            (e = cudaMemsetAsync(word, 0, sizeof(int32_t), own)) == cudaSuccess)
+            e = cudaStreamSynchronize(own);
+        cudaStreamDestroy(own);
+    }
+    if (e == cudaSuccess) ws.err = word;
+    else cudaFree(word);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return e;
+}
+
 cudaError_t ensure_workspace(Workspace& ws, const SampleArgs& a, const LaunchPlan& plan, int ranks,
                              cudaStream_t stream, std::string* err) {
     cudaError_t e;
     const size_t B = (size_t)a.B;
     const size_t nch = (size_t)plan.nchunks;
-    if (!ws.err) {
-        if ((e = cudaMalloc((void**)&ws.err, sizeof(int32_t))) != cudaSuccess) return e;
-        if ((e = cudaMemsetAsync(ws.err, 0, sizeof(int32_t), stream)) != cudaSuccess) return e;
-    }
+    if ((e = ensure_error_word(ws)) != cudaSuccess) return e;
     // Completion counters and row thresholds start at zero and every launch leaves them at zero.
     if ((e = grow(&ws.row_counter, &ws.row_counter_cap, B, true, stream)) != cudaSuccess) return e;
     if ((e = grow(&ws.row_tau, &ws.row_tau_cap, B * kTauStride, true, stream)) != cudaSuccess) return e;
