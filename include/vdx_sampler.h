@@ -521,7 +521,9 @@ typedef struct vdxs_beam_rows {
  * row_stride bytes apart. A cache [rows, heads, room, width] of which `used` positions are
  * filled has heads segments of used * width elements. Row r of dst receives row parent(r)
  * of src. dst may be src with the same strides (in place: rows that stay are not touched);
- * otherwise the two do not overlap. Bytes outside the segments are left as they were. */
+ * otherwise the two do not overlap. No target of a call overlaps another cache of it: two with
+ * one target, or a target that is another's source, are refused (list a cache that layers share
+ * once). Bytes outside the segments are left as they were. */
 typedef struct vdxs_beam_cache {
     const void* src;
     void*       dst;

@@ -491,6 +491,32 @@ def test_reorder(gpu_ctx, dtype, width):
     search.close()
 
 
+def test_a_cache_listed_twice_is_refused(gpu_ctx):
+    """A cache that two layers share is listed once: twice, or as a source beside its being a target, is
+    refused and moves nothing. Caches whose bytes lie between one another's are moved."""
+    import torch
+    from vindexllm_b200.sampler import BeamSearch, VdxsError
+    batch, beams = 2, 3
+    rows = batch * beams
+    parents = torch.tensor([[2, 0, 1], [1, 1, 0]], dtype=torch.int32, device="cuda")
+    src = (parents + beams * torch.arange(batch, device="cuda")[:, None]).view(-1).long()
+    search = BeamSearch(gpu_ctx, batch, beams, 10)
+    a, b = (torch.randn(rows, 4, 16, device="cuda") for _ in range(2))
+    keep = [a.clone(), b.clone()]
+    for caches in ([a, a], [a, b, a.view(rows, 64)], [(a, b), b], [(a, b), (b, a)], [a] + [torch.zeros_like(b) for _ in
+                                                                                      range(40)] + [a[:, :2]]):
+        with pytest.raises(VdxsError, match="another cache"):
+            search.reorder(parents, caches)
+    torch.cuda.synchronize()
+    assert torch.equal(a, keep[0]) and torch.equal(b, keep[1])
+    both = torch.randn(rows, 2, 4, 16, device="cuda")
+    want = both[src]
+    search.reorder(parents, [both[:, 0], both[:, 1], b[:, :0], b[:, :0]])
+    assert torch.equal(both, want)
+    search.reorder(parents, [(a, both[:, 0]), (a, both[:, 1])])  # one source, two targets
+    assert torch.equal(both[:, 0], a[src]) and torch.equal(both[:, 1], a[src])
+    search.close()
+
 @pytest.mark.parametrize("beams", [1, 2, 9, 17, 64])
 def test_reorder_other_beam_counts(gpu_ctx, beams):
     import torch

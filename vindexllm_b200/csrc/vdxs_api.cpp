@@ -16,6 +16,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <mutex>
 #include <new>
 #include <string>
@@ -1583,6 +1584,25 @@ int32_t check_caches(vdxs_beam* b, const vdxs_beam_cache* caches, int32_t n, Bea
         out[i].dst_segment = c.segments > 1 ? seg[1] : 0;
         out[i].segment_bytes = c.segment_bytes;
         out[i].segments = c.segments;
+    }
+    // Nothing orders a launch's caches: one listed twice would be moved twice, in a race. (Extents may
+    // well cross, as those of keys and values in one tensor do.)
+    if (n > 1) {
+        std::unique_ptr<const unsigned char*[]> targets(new (std::nothrow) const unsigned char*[(size_t)n]);
+        if (!targets) return fail(b->ctx, VDXS_E_NO_MEMORY, "out of host memory");
+        size_t have = 0;
+        for (int32_t i = 0; i < n; ++i)
+            if (out[i].segments > 0) targets[have++] = out[i].dst;
+        std::sort(targets.get(), targets.get() + have);
+        for (int32_t i = 0; i < n; ++i) {
+            const BeamCacheArgs& c = out[i];
+            if (c.segments == 0) continue;
+            const auto same = std::equal_range(targets.get(), targets.get() + have, (const unsigned char*)c.dst);
+            if (same.second - same.first > 1)
+                return fail(b->ctx, VDXS_E_INVALID_ARG, "cache %d: its target is that of another cache", i);
+            if (c.src != c.dst && std::binary_search(targets.get(), targets.get() + have, c.src))
+                return fail(b->ctx, VDXS_E_INVALID_ARG, "cache %d: its source is another cache's target", i);
+        }
     }
     return VDXS_OK;
 }
