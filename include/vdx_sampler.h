@@ -549,7 +549,8 @@ VDXS_API int32_t vdxs_beam_destroy(vdxs_beam* beam);
  *                 place) or overlaps none of them
  *   d_out_tokens, d_out_parents  [batch * beams] int32; a parent is a beam 0..beams-1 of
  *                 the same prompt
- * caches may be NULL when n_caches is 0. */
+ * caches may be NULL when n_caches is 0. Pointers are aligned to their element size (a cache's
+ * may have any alignment; 16 bytes, of strides and segments too, is the fastest). */
 VDXS_API int32_t vdxs_beam_step(vdxs_beam* beam, const vdxs_beam_config* cfg, const void* d_logits,
                                 int32_t dtype, int64_t row_stride, const vdxs_beam_rows* in,
                                 const vdxs_beam_rows* out, const int32_t* d_stop_ids, int32_t n_stop,

@@ -684,3 +684,31 @@ def test_refusals(gpu_ctx):
     with pytest.raises(TypeError):
         search.step(state, x.half())
     search.close()
+
+
+def test_unaligned_pointers_are_refused(gpu_ctx):
+    from vindexllm_b200.sampler import BeamSearch, BeamState
+    import torch
+    lib, search, state = gpu_ctx.lib, BeamSearch(gpu_ctx, 2, 3, 100), BeamState(2, 3, 4)
+    x, tok = torch.zeros(6, 100, device="cuda"), torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    before = [getattr(state, n).clone() for n in ("scores", "lengths", "finished", "hist", "pos", "count")]
+
+    def step(off=None, side=0, tp=0, pp=0, stop=None):
+        rows = [state.rows(), state.rows()]
+        if off:
+            setattr(rows[side], off, getattr(rows[side], off) + 2)
+        cfg = abi.VdxsBeamConfig(0.0, 1.0, 4, 0, 0)
+        return lib.vdxs_beam_step(search._h, C.byref(cfg), x.data_ptr(), 0, 100, C.byref(rows[0]), C.byref(rows[1]), stop,
+                                  1 if stop else 0, None, 0, tok.data_ptr() + tp, tok.data_ptr() + pp, None)
+
+    for name, _ in abi.VdxsBeamRows._fields_:
+        for side in (0, 1):
+            assert step(name, side) == abi.E_INVALID_ARG, (name, side)
+    assert step(tp=1) == step(pp=2) == step(stop=tok.data_ptr() + 2) == abi.E_INVALID_ARG
+    assert lib.vdxs_beam_reorder(search._h, tok.data_ptr() + 2, None, 0, None) == abi.E_INVALID_ARG
+    assert b"aligned" in lib.vdxs_last_error(gpu_ctx.handle)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, getattr(state, n)) for a, n in
+               zip(before, ("scores", "lengths", "finished", "hist", "pos", "count")))
+    assert step() == abi.OK
+    search.close()

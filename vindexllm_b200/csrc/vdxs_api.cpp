@@ -1292,6 +1292,8 @@ bool hidden_dtype(int32_t dtype) {
     return dtype == VDXS_DTYPE_F32 || dtype == VDXS_DTYPE_BF16 || dtype == VDXS_DTYPE_F16;
 }
 bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+template <typename... P>
+bool all_words(const P*... p) { return (aligned(p, 4) && ...); }
 
 // Everything of vdxs_rms_norm_i8 but its 8-bit outputs.
 int32_t check_norm(vdxs_context* ctx, const NormI8Args& a) {
@@ -1691,6 +1693,11 @@ VDXS_API int32_t vdxs_beam_step(vdxs_beam* b, const vdxs_beam_config* cfg, const
         return fail(ctx, VDXS_E_INVALID_ARG, "history ring buffers are NULL");
     if (n_stop < 0 || (n_stop > 0 && !d_stop_ids))
         return fail(ctx, VDXS_E_INVALID_ARG, "stop list: n_stop %d with a NULL buffer", n_stop);
+    if (!all_words(in->scores, in->lengths, in->finished, out->scores, out->lengths, out->finished, d_out_tokens,
+                   d_out_parents) ||
+        (n_stop > 0 && !all_words(d_stop_ids)) ||
+        (cfg->window > 0 && !all_words(in->hist, in->hist_pos, in->hist_count, out->hist, out->hist_pos, out->hist_count)))
+        return fail(ctx, VDXS_E_INVALID_ARG, "a pointer is not aligned to 4 bytes");
     if (n_caches < 0 || (n_caches > 0 && !caches))
         return fail(ctx, VDXS_E_INVALID_ARG, "n_caches %d with a NULL list", n_caches);
     BeamArgs a;
@@ -1749,6 +1756,7 @@ VDXS_API int32_t vdxs_beam_reorder(vdxs_beam* b, const int32_t* d_parents, const
                                    int32_t n_caches, void* stream) {
     if (!b) return fail(nullptr, VDXS_E_INVALID_ARG, "beam search is NULL");
     if (!d_parents) return fail(b->ctx, VDXS_E_INVALID_ARG, "parents pointer is NULL");
+    if (!all_words(d_parents)) return fail(b->ctx, VDXS_E_INVALID_ARG, "the parents pointer is not aligned to 4 bytes");
     if (n_caches < 0 || (n_caches > 0 && !caches))
         return fail(b->ctx, VDXS_E_INVALID_ARG, "n_caches %d with a NULL list", n_caches);
     auto* moved = new (std::nothrow) BeamCacheArgs[(size_t)n_caches + 1];
