@@ -68,3 +68,17 @@ def test_restatement_against_the_definition():
     assert np.allclose(new["scores"], [np.log(0.5), np.log(0.5) - 0.5]) and new["finished"].tolist() == [0, 1]
     q, scale = ref.norm_i8(np.array([[3.0, -4.0]]), np.ones(2), 0.0)
     assert q.tolist() == [[95, -127]] and np.allclose(scale * q[0, 1], -4 / np.sqrt(12.5))
+
+
+def test_search_of_a_closed_context_is_refused():
+    """A search's handle points to its context's: neither is used once the context is closed."""
+    from types import SimpleNamespace
+
+    from vindexllm_b200.sampler import BeamSearch, VdxsError
+    search = BeamSearch.__new__(BeamSearch)
+    search.ctx, search.lib, search._h = SimpleNamespace(_h=None, device=0), SimpleNamespace(), 1
+    search.batch, search.beams, search.vocab = 1, 2, 10
+    for call in (lambda: search.step(None, None), lambda: search.reorder(None, [])):
+        with pytest.raises(VdxsError, match="context is closed"):
+            call()
+    search._h = None

@@ -707,6 +707,12 @@ class BeamSearch:
         except Exception:
             pass
 
+    def _handle(self):
+        """The search's handle, which points to its context's."""
+        if not self.ctx._h:
+            raise VdxsError(abi.E_INVALID_ARG, "the search's context is closed")
+        return self._h
+
     def _caches(self, caches):
         """A cache is a tensor [rows, ...] (in place) or a pair (source, target) of them; a view
         of the filled part moves that part alone."""
@@ -741,6 +747,7 @@ class BeamSearch:
         """One step (vdxs_beam_step): (tokens, parents) as int32 [batch, beams]. ``out`` receives the
         rows after it (``state`` itself, in place, when None)."""
         import torch
+        h = self._handle()
         dev, batch, beams, i32 = self.ctx.device, self.batch, self.beams, torch.int32
         shape = (batch, beams)
         pitch = _matrix(logits, "logits", dev, None, (batch * beams, self.vocab))
@@ -763,7 +770,7 @@ class BeamSearch:
             _need(parents, "parents", dev, i32, shape)
         cfg = abi.VdxsBeamConfig(length_alpha, repeat_penalty, state.window, pad_token, 0)
         moved, n = self._caches(caches) if caches else (None, 0)
-        rc = self.lib.vdxs_beam_step(self._h, C.byref(cfg), logits.data_ptr(), _dtype_code(logits), pitch, C.byref(a),
+        rc = self.lib.vdxs_beam_step(h, C.byref(cfg), logits.data_ptr(), _dtype_code(logits), pitch, C.byref(a),
                                      C.byref(b), _ptr(stop_ids), n_stop, moved, n, tokens.data_ptr(), parents.data_ptr(),
                                      _stream_on(dev, stream))
         if rc:
@@ -780,7 +787,8 @@ class BeamSearch:
     def reorder(self, parents, caches, stream=None):
         """Moves caches by a step's parents (vdxs_beam_reorder)."""
         import torch
+        h = self._handle()
         _need(parents, "parents", self.ctx.device, torch.int32, (self.batch, self.beams))
         moved, n = self._caches(caches)
-        check(self.lib.vdxs_beam_reorder(self._h, _ptr(parents), moved, n, _stream_on(self.ctx.device, stream)),
+        check(self.lib.vdxs_beam_reorder(h, _ptr(parents), moved, n, _stream_on(self.ctx.device, stream)),
               self.ctx._h)
