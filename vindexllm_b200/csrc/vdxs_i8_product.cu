@@ -280,13 +280,16 @@ __global__ void __launch_bounds__(kThreadsP, 1)
             }
             if (!good) break;
         }
-        // Should a wait have given up: the copies in flight land before the CTA (the pair) may end.
-        if (!good && rank == 0)
+        // The copies in flight land before the CTA (the pair) may end: the products' warp, which waits
+        // for them too, may have given up.
+        if (rank == 0) {
+            bool landed = true;
             for (; issued > 0; --issued) {
                 if (--s < 0) s = p.stages - 1, phase ^= 1;
-                bool again = true;
-                bar_wait(&full[s], phase, again);
+                bar_wait(&full[s], phase, landed);
             }
+            good = good && landed;
+        }
     } else if (warp == 1 && rank == 0) {
         // D: 32-bit integers; A, B: signed 8 bits, K-major.
         const uint32_t idesc =
@@ -319,6 +322,8 @@ __global__ void __launch_bounds__(kThreadsP, 1)
             mma_commit<PAIR>(one, smem_addr(&acc_full[acc]));
             if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
+        // And the last products are in before tensor memory is freed, whether or not the epilogue gave up.
+        if (first < p.tiles) bar_wait(&acc_full[acc ^ 1], acc == 0 ? acc_phase ^ 1 : acc_phase, good);
     } else if (warp >= 2) {
         const int quad = warp & 3;             // the tensor memory lanes that this warp may read
         const int half = (warp - 2) >> 2;      // even or odd groups of 16 columns
