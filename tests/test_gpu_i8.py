@@ -266,6 +266,44 @@ def test_product_on_two_streams(gpu_ctx):
     w.close()
 
 
+# Products of two CTAs on a tile (test_i8_beam_host.py checks that each is one): one column tile and
+# several, 160 to 256 columns (all of tensor memory), whole and partial last chunks, an odd and an
+# even number of 128-entry tiles.
+PAIR_SHAPES = [(129, 20001, 2048), (160, 19968, 2100), (256, 20001, 2048), (256, 19968, 2049), (512, 20001, 2560),
+               (513, 20001, 2304), (512, 10000, 4096)]
+
+
+@pytest.mark.parametrize("batch,n,k", PAIR_SHAPES)
+def test_product_of_pairs(gpu_ctx, batch, n, k):
+    import torch
+    from vindexllm_b200.sampler import I8Weights
+    wq, q = _ints(n, k, 1), _ints(batch, k, 2, -(-k // 16) * 16)
+    ws, xs = np.linspace(1e-4, 2e-3, n).astype(np.float32), np.linspace(0.01, 0.2, batch).astype(np.float32)
+    w = I8Weights(gpu_ctx, _t(wq), _t(ws))
+    for dtype in (torch.float32, torch.bfloat16):
+        _check_product(w.unembed(_t(q)[:, :k], _t(xs), dtype=dtype), q[:, :k], xs, wq, ws)
+    gpu_ctx.device_status()
+    w.close()
+
+
+def test_pairs_beside_another_stream(gpu_ctx):
+    """A product of pairs and one of single CTAs on two streams at once."""
+    import torch
+    from vindexllm_b200.sampler import I8Weights
+    _, n, k = PAIR_SHAPES[2]
+    w = I8Weights(gpu_ctx, torch.randn(n, k, device="cuda", generator=torch.Generator("cuda").manual_seed(1)))
+    q = [_t(_ints(b, k, b)) for b in (7, 256, 300)]
+    xs = [torch.rand(b.shape[0], device="cuda") for b in q]
+    want = [w.unembed(a, b) for a, b in zip(q, xs)]
+    streams = [torch.cuda.Stream() for _ in q]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        got = [w.unembed(a, b, stream=s) for a, b, s in zip(q, xs, streams)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    gpu_ctx.device_status()
+    w.close()
+
 def test_product_extremes(gpu_ctx):
     """The largest sums (-128 * -128 over the largest in_dim), and scales of NaN and infinity."""
     import torch

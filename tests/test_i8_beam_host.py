@@ -82,3 +82,36 @@ def test_search_of_a_closed_context_is_refused():
         with pytest.raises(VdxsError, match="context is closed"):
             call()
     search._h = None
+
+
+def test_forms_of_the_product(tmp_path):
+    """The rule that chooses the product's form, for the shapes that the GPU tests mean to reach each form
+    with, at a B200's 148 SMs."""
+    import os
+    import shutil
+    import subprocess
+
+    from test_gpu_i8 import PAIR_SHAPES
+    include = "/usr/local/cuda/include"
+    if not shutil.which("g++") or not os.path.exists(os.path.join(include, "cuda_runtime.h")):
+        pytest.skip("no g++ or CUDA headers")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src, exe = tmp_path / "form.cpp", tmp_path / "form"
+    src.write_text('#include "vdxs_internal.h"\n#include <cstdio>\nint main() {\n int b, n, k;\n'
+                   ' while (std::scanf("%d %d %d", &b, &n, &k) == 3) {\n'
+                   '  const vdxs::I8ProductForm f = vdxs::i8_product_form(b, k, n, 148);\n'
+                   '  std::printf("%d %d %d %d\\n", f.mode, f.split, f.n_tiles, f.n);\n }\n}\n')
+    subprocess.run(["g++", "-std=c++17", "-I", include, "-I", os.path.join(root, "vindexllm_b200", "csrc"), str(src), "-o",
+                    str(exe)], check=True)
+    single = [(1, 262144, 1152), (64, 262144, 2560), (7, 20001, 2048), (256, 262144, 1152)]
+    split = {(1, 1000, 8192): 8, (256, 1000, 8192): 8, (33, 8000, 4100): 2, (300, 700, 2000): 4}
+    shapes = PAIR_SHAPES + single + list(split)
+    run = subprocess.run([str(exe)], input="\n".join(" ".join(map(str, s)) for s in shapes), capture_output=True, text=True,
+                         check=True)
+    got = {s: tuple(map(int, line.split())) for s, line in zip(shapes, run.stdout.splitlines())}
+    assert all(got[s][0] == 1 for s in PAIR_SHAPES), got
+    assert all(got[s][0] == 0 for s in single), got
+    assert all(got[s][:2] == (2, parts) for s, parts in split.items()), got
+    assert {got[s][3] for s in PAIR_SHAPES} >= {160, 256} and {got[s][2] for s in PAIR_SHAPES} >= {1, 2, 3}
+    for (batch, _, _), (mode, _, n_tiles, n) in got.items():
+        assert n_tiles * n >= batch and (n_tiles - 1) * n < batch and n <= 256 and n % (32 if mode == 1 else 16) == 0

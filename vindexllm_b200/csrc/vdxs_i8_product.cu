@@ -39,9 +39,7 @@ namespace {
 
 constexpr int kEpiWarps = 8;         // two for each quarter of the accumulator's rows
 constexpr int kThreadsP = 64 + 32 * kEpiWarps;
-constexpr int kTileM = 128;          // vocabulary entries of a tile
-constexpr int kChunkK = 128;         // bytes of a row in a stage: one swizzle span
-constexpr int kMaxN = 256;           // batch columns of a tile
+constexpr int kTileM = kI8TileM, kChunkK = kI8ChunkK, kMaxN = kI8MaxN;
 constexpr int kMaxStages = 12;
 constexpr int kStageBytesA = kTileM * kChunkK;
 constexpr int kSmemBudget = 220 * 1024;
@@ -211,7 +209,7 @@ __device__ __forceinline__ void store16(O* o, int64_t stride, const uint32_t* v,
     }
 }
 
-enum Mode : int { kSingle = 0, kPair = 1, kSplit = 2 };
+constexpr int kSingle = I8ProductForm::kSingle, kPair = I8ProductForm::kPair, kSplit = I8ProductForm::kSplit;
 
 template <typename O, int MODE>
 __global__ void __launch_bounds__(kThreadsP, 1)
@@ -483,27 +481,17 @@ cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, con
     p.in_dim = w.in_dim;
     p.out_dim = w.out_dim;
     p.batch = batch;
-    // Equal column tiles of at most 256, a multiple of 16 wide (of 32 in pairs).
-    p.n_tiles = (batch + kMaxN - 1) / kMaxN;
-    const int64_t tiles = (int64_t)((w.out_dim + kTileM - 1) / kTileM) * p.n_tiles;
-    const int chunks = (w.in_dim + kChunkK - 1) / kChunkK;
-    // Pairs where the batch operand weighs, the sums are long and every SM has a tile: batch 512 of
-    // 262144 x 2560 291 us against 312, batch 256 of 32003 x 3840 35.3 against 38.5; but batch 256
-    // of 262144 x 1152 109 against 101, and batch 512 of 8000 x 4096 18.9 against 17.2.
-    const bool pair = batch > 128 && w.in_dim >= 2048 && tiles > sm_count;
-    // A split's share is four chunks at least, and its clusters fit the GPU at once (8-CTA clusters
-    // fill only part of a GPU's SM groups). Batch 1 of 1000 x 8192 7.9 us with 8 parts against
-    // 22.2 with one, of 8000 x 4096 9.4 with 2 against 12.8.
-    p.split = 1;
-    for (int s = 2; s <= 8 && tiles * s <= sm_count * (s < 8 ? 7 : 6) / 8 && chunks >= 4 * s; s *= 2) p.split = s;
-    const int mode = pair ? kPair : p.split > 1 ? kSplit : kSingle;
+    const I8ProductForm form = i8_product_form(batch, w.in_dim, w.out_dim, sm_count);
+    const bool pair = form.mode == kPair;
     const int ctas = pair ? 2 : 1;
-    p.n = ((batch + p.n_tiles - 1) / p.n_tiles + 16 * ctas - 1) / (16 * ctas) * (16 * ctas);
+    p.n_tiles = form.n_tiles;
+    p.n = form.n;
+    p.split = form.split;
     p.columns = 32;
     while (p.columns < 2 * p.n) p.columns *= 2;
     const int stage_bytes = kStageBytesA + p.n / ctas * kChunkK;
     p.stages = std::min(kMaxStages, (kSmemBudget - 1024) / stage_bytes);
-    p.tiles = pair ? (int64_t)((w.out_dim + 2 * kTileM - 1) / (2 * kTileM)) * p.n_tiles : tiles;
+    p.tiles = (int64_t)((w.out_dim + ctas * kTileM - 1) / (ctas * kTileM)) * p.n_tiles;
     p.w_scale = w.scale;
     p.scale = scale;
     p.logits = logits;
@@ -515,8 +503,8 @@ cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, con
     cudaError_t e = make_map(&map_q, q, w.in_dim, batch, q_stride, p.n / ctas);
     if (e != cudaSuccess) return e;
     const int smem = p.stages * stage_bytes + 1024;
-    e = dtype == VDXS_DTYPE_BF16 ? launch_mode<__nv_bfloat16>(mode, map_w, map_q, p, smem, sm_count, stream)
-                                 : launch_mode<float>(mode, map_w, map_q, p, smem, sm_count, stream);
+    e = dtype == VDXS_DTYPE_BF16 ? launch_mode<__nv_bfloat16>(form.mode, map_w, map_q, p, smem, sm_count, stream)
+                                 : launch_mode<float>(form.mode, map_w, map_q, p, smem, sm_count, stream);
     if (e != cudaSuccess) return e;
     ++*launches;
     return cudaSuccess;

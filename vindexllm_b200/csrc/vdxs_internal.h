@@ -196,6 +196,33 @@ struct SmemLimit {
 cudaError_t rms_norm_i8(const NormI8Args& a, cudaStream_t stream);
 // Rows of fp32/bf16/fp16 (format 0..2) or Q4_0 blocks (4) to 8 bits with a scale per row.
 cudaError_t quantise_rows_i8(const void* src, int format, int64_t row_stride, const I8Matrix& w, cudaStream_t stream);
+// The product's form for its sizes.
+constexpr int kI8TileM = 128;   // vocabulary entries of a tile
+constexpr int kI8ChunkK = 128;  // bytes of a row in a stage: one swizzle span
+constexpr int kI8MaxN = 256;    // batch columns of a tile
+struct I8ProductForm {
+    enum Mode : int { kSingle = 0, kPair = 1, kSplit = 2 };
+    int mode = kSingle, split = 1, n_tiles = 1, n = 16;
+};
+inline I8ProductForm i8_product_form(int batch, int in_dim, int out_dim, int sm_count) {
+    I8ProductForm f;
+    // Equal column tiles of at most 256, a multiple of 16 wide (of 32 in pairs).
+    f.n_tiles = (batch + kI8MaxN - 1) / kI8MaxN;
+    const int64_t tiles = (int64_t)((out_dim + kI8TileM - 1) / kI8TileM) * f.n_tiles;
+    const int chunks = (in_dim + kI8ChunkK - 1) / kI8ChunkK;
+    // Pairs where the batch operand weighs, the sums are long and every SM has a tile: batch 512 of
+    // 262144 x 2560 291 us against 312, batch 256 of 32003 x 3840 35.3 against 38.5; but batch 256
+    // of 262144 x 1152 109 against 101, and batch 512 of 8000 x 4096 18.9 against 17.2.
+    const bool pair = batch > 128 && in_dim >= 2048 && tiles > sm_count;
+    // A split's share is four chunks at least, and its clusters fit the GPU at once (8-CTA clusters
+    // fill only part of a GPU's SM groups). Batch 1 of 1000 x 8192 7.9 us with 8 parts against
+    // 22.2 with one, of 8000 x 4096 9.4 with 2 against 12.8.
+    for (int s = 2; s <= 8 && tiles * s <= sm_count * (s < 8 ? 7 : 6) / 8 && chunks >= 4 * s; s *= 2) f.split = s;
+    f.mode = pair ? I8ProductForm::kPair : f.split > 1 ? I8ProductForm::kSplit : I8ProductForm::kSingle;
+    const int step = pair ? 32 : 16, columns = (batch + f.n_tiles - 1) / f.n_tiles;
+    f.n = (columns + step - 1) / step * step;
+    return f;
+}
 cudaError_t unembed_i8(const I8Matrix& w, const int8_t* q, int64_t q_stride, const float* scale, int batch,
                        void* logits, int dtype, int64_t logits_stride, int32_t* err, int sm_count, cudaStream_t stream,
                        int* launches);
