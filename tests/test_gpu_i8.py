@@ -62,6 +62,17 @@ def test_norm_many_rows(gpu_ctx, rows):
         _check_norm(q, scale, (x.float() + r.float()).to(x.dtype), w, 1e-5)
 
 
+def test_norm_about_a_row_for_each_sm(gpu_ctx):
+    """Rows take more threads each while there is no more than one for every SM of this device."""
+    import torch
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for rows in (sms - 1, sms, sms + 1):
+        for dim, dtype in ((640, "bf16"), (2560, "f32"), (3840, "f16")):
+            x, w = _hidden(rows, dim, rows, dtype), _t(np.linspace(0.5, 1.5, dim).astype(np.float32))
+            q, scale, _ = gpu_ctx.rms_norm_i8(x, w, 1e-5)
+            _check_norm(q, scale, x, w, 1e-5)
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("dim", [64, 72, 520, 1032, 5000, 16384, 32768])
 def test_norm_many_rows_of_every_width(gpu_ctx, dtype, dim):

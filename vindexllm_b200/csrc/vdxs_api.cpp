@@ -1350,7 +1350,7 @@ VDXS_API int32_t vdxs_rms_norm_i8(vdxs_context* ctx, const void* d_x, int64_t x_
     if (q_stride < dim) return fail(ctx, VDXS_E_INVALID_ARG, "q_stride is smaller than dim %d", dim);
     if (!aligned(d_scale, 4)) return fail(ctx, VDXS_E_INVALID_ARG, "the scale pointer is not aligned to 4 bytes");
     DeviceGuard g(ctx->device);
-    const cudaError_t e = rms_norm_i8(a, (cudaStream_t)stream);
+    const cudaError_t e = rms_norm_i8(a, ctx->sm_count, (cudaStream_t)stream);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "norm launch");
     ctx->launches += 1;
     ok(ctx);
@@ -1510,7 +1510,7 @@ VDXS_API int32_t vdxs_sample_unembed_i8(vdxs_context* ctx, const vdxs_config* cf
     a.q = ws.i8_q;
     a.q_stride = w->m.pitch;
     a.scale = ws.i8_scale;
-    if ((e = rms_norm_i8(a, st)) != cudaSuccess) return cuda_fail(ctx, e, "norm launch");
+    if ((e = rms_norm_i8(a, ctx->sm_count, st)) != cudaSuccess) return cuda_fail(ctx, e, "norm launch");
     ctx->launches += 1;
     rc = vdxs_unembed_i8(ctx, w, ws.i8_q, w->m.pitch, ws.i8_scale, batch, ws.unembed_logits, VDXS_DTYPE_F32, vocab,
                          stream);

@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kNormThreads) quantise_rows_kernel(S src, I8Ma
 }
 
 template <typename T, typename W>
-cudaError_t launch_norm(const NormI8Args& a, cudaStream_t stream) {
+cudaError_t launch_norm(const NormI8Args& a, int sm_count, cudaStream_t stream) {
     constexpr int N = Pack<T>::N;
     auto whole = [](const void* p, int64_t stride, size_t size, size_t to) {
         return (uintptr_t)p % to == 0 && (uint64_t)stride * size % to == 0;
@@ -362,7 +362,7 @@ cudaError_t launch_norm(const NormI8Args& a, cudaStream_t stream) {
     // fp32 in 3.1 us, with the launch).
     constexpr int kMost = 32 / N;
     const int nv = a.dim / N;
-    const int per = nv > 1024 || (a.rows > 148 && nv > 64) ? kMost : 1;
+    const int per = nv > 1024 || (a.rows > sm_count && nv > 64) ? kMost : 1;
     const int threads = ((nv + per - 1) / per + 31) / 32 * 32;
     if (per == 1) rms_norm_i8_rows_kernel<T, W, 1, 1024><<<a.rows, threads, 0, stream>>>(a);
     else if (threads <= 256) rms_norm_i8_rows_kernel<T, W, kMost, 256><<<a.rows, threads, 0, stream>>>(a);
@@ -371,18 +371,18 @@ cudaError_t launch_norm(const NormI8Args& a, cudaStream_t stream) {
 }
 
 template <typename T>
-cudaError_t launch_norm_w(const NormI8Args& a, cudaStream_t stream) {
-    if (a.weight_dtype == VDXS_DTYPE_BF16) return launch_norm<T, __nv_bfloat16>(a, stream);
-    if (a.weight_dtype == VDXS_DTYPE_F16) return launch_norm<T, __half>(a, stream);
-    return launch_norm<T, float>(a, stream);
+cudaError_t launch_norm_w(const NormI8Args& a, int sm_count, cudaStream_t stream) {
+    if (a.weight_dtype == VDXS_DTYPE_BF16) return launch_norm<T, __nv_bfloat16>(a, sm_count, stream);
+    if (a.weight_dtype == VDXS_DTYPE_F16) return launch_norm<T, __half>(a, sm_count, stream);
+    return launch_norm<T, float>(a, sm_count, stream);
 }
 
 }  // namespace
 
-cudaError_t rms_norm_i8(const NormI8Args& a, cudaStream_t stream) {
-    if (a.dtype == VDXS_DTYPE_BF16) return launch_norm_w<__nv_bfloat16>(a, stream);
-    if (a.dtype == VDXS_DTYPE_F16) return launch_norm_w<__half>(a, stream);
-    return launch_norm_w<float>(a, stream);
+cudaError_t rms_norm_i8(const NormI8Args& a, int sm_count, cudaStream_t stream) {
+    if (a.dtype == VDXS_DTYPE_BF16) return launch_norm_w<__nv_bfloat16>(a, sm_count, stream);
+    if (a.dtype == VDXS_DTYPE_F16) return launch_norm_w<__half>(a, sm_count, stream);
+    return launch_norm_w<float>(a, sm_count, stream);
 }
 
 cudaError_t quantise_rows_i8(const void* src, int format, int64_t row_stride, const I8Matrix& w, cudaStream_t stream) {

@@ -193,7 +193,7 @@ struct SmemLimit {
         return e;
     }
 };
-cudaError_t rms_norm_i8(const NormI8Args& a, cudaStream_t stream);
+cudaError_t rms_norm_i8(const NormI8Args& a, int sm_count, cudaStream_t stream);
 // Rows of fp32/bf16/fp16 (format 0..2) or Q4_0 blocks (4) to 8 bits with a scale per row.
 cudaError_t quantise_rows_i8(const void* src, int format, int64_t row_stride, const I8Matrix& w, cudaStream_t stream);
 // The product's form for its sizes.
