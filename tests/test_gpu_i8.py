@@ -62,6 +62,32 @@ def test_norm_many_rows(gpu_ctx, rows):
         _check_norm(q, scale, (x.float() + r.float()).to(x.dtype), w, 1e-5)
 
 
+def test_norm_of_fp32_products_on_a_border(gpu_ctx):
+    """fp32 values times fp32 weights, 48 bits, that lie exactly on a border or next to one: 127 times
+    such a product is no double. The expected steps are computed in whole numbers."""
+    import torch
+    from fractions import Fraction
+    rng = np.random.default_rng(3)
+    rows, xs, wants = 24, [], []
+    v = int(rng.integers(1 << 23, 1 << 24)) | 1
+    for i in range(rows):
+        u = int(rng.integers(1 << 15, 1 << 16)) | 1
+        # (2k + 1) u against 254 u: k + 1/2 steps; every third one is moved off its border by one unit.
+        x = [(2 * k + 1) * u + (0, 1, -1)[k % 3 if i % 2 else 0] for k in range(126)] + [254 * u, -254 * u]
+        x = [a * (-1) ** (i // 2 * j % 2) for j, a in enumerate(x)]
+        xs.append(x)
+        wants.append([round(Fraction(127 * a, 254 * u)) for a in x])  # to the even one
+    w = torch.full((128,), float(v), device="cuda")
+    x = torch.tensor(xs, dtype=torch.float32, device="cuda")
+    want = torch.tensor(wants, dtype=torch.int8, device="cuda")
+    assert (x.double().cpu() == torch.tensor(xs, dtype=torch.float64)).all()
+    wide = torch.zeros(rows, 129, device="cuda")
+    wide[:, 1:] = x
+    for case in (x, x.repeat(20, 1), wide[:, 1:]):  # vectors, more rows than SMs, rows off the 16-byte boundary
+        q, _, _ = gpu_ctx.rms_norm_i8(case, w, 1e-6)
+        assert torch.equal(q, want.repeat(case.shape[0] // rows, 1))
+
+
 def test_norm_about_a_row_for_each_sm(gpu_ctx):
     """Rows take more threads each while there is no more than one for every SM of this device."""
     import torch
