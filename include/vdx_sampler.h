@@ -345,7 +345,7 @@ VDXS_API int32_t vdxs_sample_sharded(vdxs_context* ctx, vdxs_comm* comm,
 /* Waits for `stream` and reads the context's device error word, which the kernels
  * set instead of trapping when a bounded wait gives up (VDXS_E_TIMEOUT) or an
  * internal selection check fails (VDXS_E_DEVICE_STATE). A non-zero word means the
- * tokens of the calls since the last check may be wrong; the word and the kernels'
+ * tokens (of vdxs_unembed_i8 the logits) of the calls since the last check may be wrong; the word and the kernels'
  * self-resetting counters are cleared before returning, so the context stays usable.
  * vdxs_sample_host and vdxs_sampler_process* perform this check themselves. */
 VDXS_API int32_t vdxs_device_status(vdxs_context* ctx, void* stream);
@@ -449,6 +449,8 @@ VDXS_API int32_t vdxs_i8_release(vdxs_i8_weights* w);
  *   d_scale   [batch] fp32
  *   d_logits  [batch, logits_stride] (logits_stride >= out_dim); what lies between
  *             out_dim and logits_stride is not written
+ * A wait inside the kernel that gives up (after two seconds) sets the context's error word and
+ * leaves logits unwritten or wrong: vdxs_device_status tells.
  * Uses no workspace and allocates nothing but the context's error word (4 bytes, with its
  * first product or sampling call), so it may be captured at once. */
 VDXS_API int32_t vdxs_unembed_i8(vdxs_context* ctx, const vdxs_i8_weights* w, const int8_t* d_q,

@@ -19,7 +19,7 @@ PROGRAM = r"""
 
 static std::mutex mu;
 static std::condition_variable cv;
-static int limit = 48 * 1024, calls = 0;  // the driver's side: the last value set stands
+static int limit = 48 * 1024, calls = 0;  // CUDA's side: the last value set stands
 static bool other_done = false;
 
 extern "C" cudaError_t cudaGetDevice(int* d) { *d = 0; return cudaSuccess; }

@@ -155,7 +155,7 @@ int32_t device_word_status(vdxs_context* ctx, int32_t word, cudaStream_t stream)
     cudaStreamSynchronize(stream);
     if (word == 3)
         return fail(ctx, VDXS_E_TIMEOUT, "a bounded device wait gave up (tensor-memory copy did not complete); "
-                                         "the tokens of the affected call are not valid");
+                                         "the tokens or logits of the affected call are not valid");
     return fail(ctx, VDXS_E_DEVICE_STATE, "device selection check failed (code %d); the tokens of the affected "
                                           "call are not valid", word);
 }
