@@ -490,9 +490,12 @@ VDXS_API int32_t vdxs_sample_unembed_i8(vdxs_context* ctx, const vdxs_config* cf
  *   - an offer whose score or quotient below is NaN or -infinity is none;
  *   - the `beams` offers with the highest score / max(length, 1)^length_alpha stay, in that
  *     order (equal ones: the lower beam, then the beam's own order).
- * Log-probabilities and the order of the offers are taken in 64 bits (exponentials in fp32;
- * values within 2^-39 of one another count as equal, and two such offers of one beam may
- * stand in either order); scores are stored in fp32. A slot that gets no offer has token pad_token, its own slot as the parent, score
+ * The logarithm of a row's sum of exponentials is off by less than 2e-5 (fp32 exponentials, a thread's
+ * sum in fp32; 3e-7 is the most that was measured), so offers of different beams that are
+ * nearer than that may change places. From there on scores and quotients are 64-bit: quotients
+ * within 2^-39 of one another, relatively, count as equal, and two such offers of one beam may
+ * stand in either order. Scores are stored in fp32.
+ * A slot that gets no offer has token pad_token, its own slot as the parent, score
  * -infinity, finished 0, and the length that stood there; it offers nothing in later steps.
  * ---------------------------------------------------------------------------- */
 #define VDXS_BEAM_MAX_BEAMS 64

@@ -11,15 +11,19 @@
 // found by counters that reset themselves.
 //
 // Rounding: exponentials and a thread's sum (at most 512 of them) are fp32, the sums of threads
-// and chunks and every score are 64-bit, so that the order of offers of different beams hangs
-// on 1e-8 and not on 1e-6; scores are stored in fp32.
+// and chunks and every score are 64-bit. The logarithm of a row's sum is off by less than 2e-5: a
+// thread adds 8 pairs in each of 32 tiles at most (41 roundings on a value's way, 2.4e-6) and
+// rescales its sum as often at most (2^-22 for the exponential, 2^-24 for the product, and the
+// argument's rounding: 1.1e-5), and three exponentials more make 9e-7. Measured over 512 rows each of 1000
+// to 262144 tokens of both types: 3e-7 at most, 6e-8 in the mean square. Offers of different beams
+// that are nearer may change places. Scores are stored in fp32.
 //
 // What bounds it: with many rows the logits' bytes and the selection behind each chunk's stream
-// (512 rows of 262144 fp32 of which 15 % are finished and not read: 444 MB in 92 us, 4.8 TB/s;
+// (512 rows of 262144 fp32 of which 15 % are finished and not read: 444 MB in 92-95 us, 4.8 TB/s;
 // the stream alone takes 75, 5.9 TB/s or 0.92 of the copy rate; deeper rings in shared memory
 // and a fetch of the next chunk into L2 changed neither). With few rows the chain of dependent
 // steps behind the stream (64 rows of bf16 with rings in 26.5 us, of which the logits take 6; 4
-// rows of 32000 in 8.7 us): bound, elements, selection, and a merge or two, each a count, loads
+// rows of 32000 in 8.6 us): bound, elements, selection, and a merge or two, each a count, loads
 // and a selection. Notes of group maxima instead of a list that the stream itself fills took the
 // 512 rows from 177 to 97 us: the list's code cost the loop its registers.
 #include "vdxs_internal.h"
@@ -461,6 +465,8 @@ __device__ __forceinline__ void select_prompt(const BeamArgs& p, int prompt) {
     }
 }
 
+// Registers for three CTAs on an SM, for four with bf16, whose tiles have half the bytes (64 x 8 of
+// 262144 bf16 59 us against 64 with three; fp32 with four 96 against 94).
 template <typename T, bool PEN>
 __global__ void __launch_bounds__(kBThreads, sizeof(T) == 2 ? 4 : 3) beam_select_kernel(const __grid_constant__ BeamArgs p) {
     SelectShared& sh = select_shared();
@@ -734,8 +740,9 @@ struct ReorderParams {
     } c[kMaxCaches];
 };
 
-// Bound by the bytes: two caches of 64 rows x 4 heads x 2500 x 256 bf16 and their rings move in
-// 160 us (0.66 GB written; parents that beams share are read once from memory and then from L2).
+// Bound by the bytes: with two caches of 64 rows x 4 heads x 2500 x 256 bf16 and their rings to move, a
+// step of 64 rows of 32000 fp32 takes 176-184 us, 149-160 of them here (0.66 GB written; parents
+// that beams share are read once from memory and then from L2).
 //
 // A thread owns one word of every row of a prompt: it reads the parents' words, then
 // writes, so a cache may be moved in place without a second buffer or a barrier.
@@ -822,9 +829,8 @@ void beam_plan(int rows, int vocab, int sm_count, int* chunks, int* chunk) {
     // A position is counted from a 16-byte boundary, so up to 7 lie before the row.
     const int64_t span = (int64_t)vocab + 7;
     const int64_t tiles = (span + kTile - 1) / kTile;
-    // Every CTA place once (three for each SM, four with bf16 logits, whose tiles have half the
-    // bytes: 64x8 of 262144 59 us against 64 with three, fp32 96 us against 94), at most kBeamMaxChunks lists to merge, and at
-    // most kMaxTiles tiles to a chunk.
+    // Three CTAs for each SM (for bf16 too, although four fit), at most kBeamMaxChunks lists to
+    // merge, and at most kMaxTiles tiles to a chunk.
     int64_t want = std::min<int64_t>(kBeamMaxChunks, std::max<int64_t>(1, (int64_t)sm_count * 3 / rows));
     want = std::min(std::max(want, (tiles + kMaxTiles - 1) / kMaxTiles), tiles);
     const int64_t per = (tiles + want - 1) / want;

@@ -7,7 +7,7 @@
 // neighbouring vocabulary entries, so the logits go out as whole 128-byte lines without a
 // stop in shared memory.
 //
-// Batches above 128 use pairs of CTAs: one product then spans both SMs of a pair (256 vocabulary
+// Batches above 128 with sums of 2048 and more use pairs of CTAs: one product then spans both SMs of a pair (256 vocabulary
 // entries, 128 to a CTA) and each CTA holds half of the batch columns' rows, which halves what
 // the batch operand costs each SM in shared-memory fills.
 // A small vocabulary has fewer tiles than the GPU has SMs, and one SM takes 0.3 us for each
@@ -20,10 +20,11 @@
 // exact 32-bit integers; the two scales are applied in fp32.
 //
 // What bounds it, on a B200 with 6456 GB/s and 1667 TFLOP/s in bf16 measured: to about 256
-// rows the weights' bytes (batch 1 of 262144 x 1152 in 54 us, 0.87 of the copy rate; batch 64
-// of 262144 x 2560 with fp32 logits in 115-119 us, 0.96-1.0). At batch 512 of the latter
-// (291 us, 2.36 POP/s) the products alone take 208 us, loads and stores alone 226, and together
-// they run into the power limit: the SM clock falls to 1.4-1.6 GHz.
+// rows the weights' bytes (batch 1 of 262144 x 1152 in 54-56 us, 0.84-0.87 of the copy rate; batch 64
+// of 262144 x 2560 with fp32 logits in 118-121 us, 0.95-0.97). At batch 512 of the latter
+// the products alone take 208 us, loads and stores alone 226, and together they run into the
+// power limit: 280-296 us for the first tens of calls (2.4 POP/s), 325-331 once the SM clock has
+// fallen (to about 1.16 GHz).
 #include "vdxs_internal.h"
 #include "../../include/vdx_sampler.h"
 

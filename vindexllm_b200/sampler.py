@@ -745,7 +745,8 @@ class BeamSearch:
     def step(self, state: BeamState, logits, out: BeamState | None = None, stop_ids=None, pad_token: int = 0,
              repeat_penalty: float = 1.0, length_alpha: float = 0.0, caches=(), tokens=None, parents=None, stream=None):
         """One step (vdxs_beam_step): (tokens, parents) as int32 [batch, beams]. ``out`` receives the
-        rows after it (``state`` itself, in place, when None)."""
+        rows after it (``state`` itself, in place, when None). A cache that layers share is listed
+        once."""
         import torch
         h = self._handle()
         dev, batch, beams, i32 = self.ctx.device, self.batch, self.beams, torch.int32
